@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -2233,3 +2233,127 @@ def token_side(x: torch.Tensor, y: Optional[torch.Tensor], scale: Optional[torch
     _check(lib().vk_token_side(_p(x), _p(y), _p(scale), _p(gate), _p(proj), dim, _p(side), side.shape[1], off, _p(z_norm), _p(table), _p(ids), side.shape[0],
                                _p(add), _p(wn), _p(bn), _p(out), T, n, ctypes.c_float(eps), ctypes.c_float(mult), _dt(gate), _stream()), "token_side")
     return out
+
+
+# ---------------------------------------------------------------------------
+# Beam search: attention over pages held in common, the choice of continuations, moves of cache rows
+# ---------------------------------------------------------------------------
+
+def _on_current(name: str, *tensors: torch.Tensor) -> None:
+    """Refuses tensors of another device than the current one, on whose stream the launch goes."""
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t.get_device() != here:
+            raise KernelError(f"{name}: a tensor is on device {t.get_device()} and the current device is {here}")
+
+
+SHARED_MAX_TOKENS, SHARED_MAX_HEADS, SHARED_MAX_KV_HEADS = 256, 64, 128      # tokens a launch, query heads a key-value head, key-value heads
+
+
+def attention_shared_takes(dtype: torch.dtype, nh: int, nkv: int, hd: int, tokens: int = 1) -> bool:
+    """Whether attention_shared takes these sizes (else the members' tables are read one by one, by attention_decode or attention_rows)."""
+    return (dtype in (torch.float32, torch.bfloat16) and 0 < hd <= 256 and hd % (4 if dtype == torch.float32 else 8) == 0 and 0 < nkv <= SHARED_MAX_KV_HEADS
+            and nh % nkv == 0 and 0 < nh // nkv <= SHARED_MAX_HEADS and tokens <= SHARED_MAX_TOKENS)
+
+
+def attention_shared_scratch_bytes(tokens: int, nh: int, nkv: int, hd: int) -> int:
+    fn = lib().vk_attention_shared_scratch_bytes
+    fn.restype = ctypes.c_size_t
+    return int(fn(tokens, nh, nkv, hd))
+
+
+def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: torch.Tensor, token_seg: torch.Tensor, positions: torch.Tensor,
+                     members: torch.Tensor, starts: torch.Tensor, shared: torch.Tensor, out: torch.Tensor, scratch: torch.Tensor, nh: int, nkv: int,
+                     hd: int, scale: float) -> torch.Tensor:
+    """Attention of single decoded tokens whose requests come in families that hold their first pages in common: the common keys and
+    values are read once for the whole family.
+
+    Family f is the tokens members[starts[f]:starts[f+1]] (int32, at most 256 in all; starts ascends, [families + 1]); the block tables of its members' requests
+    agree on the first shared[f] positions (any number: what lies at or behind the smallest of the members' positions is not counted).  A family
+    may have one member or none.  Every token reads the positions 0 .. positions[t] of its own request, as in attention_decode; rows of `out` whose token
+    is in no family are left as they were.  Block numbers outside the pool are not followed (their keys and values count as zeros).
+    scratch: a byte buffer of attention_shared_scratch_bytes(members, ...) or more, zeros at first use, for launches of one stream at a time (of any sizes it
+    is large enough for)."""
+    _req(q, "q", dims=2); _req(cache_layer, "cache_layer", q.dtype, 5); _req(block_tables, "block_tables", torch.int32, 2)
+    _req(token_seg, "token_seg", torch.int32, 1); _req(positions, "positions", torch.int32, 1); _req(out, "out", q.dtype, 2)
+    _req(members, "members", torch.int32, 1); _req(starts, "starts", torch.int32, 1); _req(shared, "shared", torch.int32, 1); _req(scratch, "scratch", torch.uint8, 1)
+    T, n, families, page_size = q.shape[0], members.shape[0], shared.shape[0], cache_layer.shape[3]
+    if not attention_shared_takes(q.dtype, nh, nkv, hd, n):
+        raise KernelError(f"attention_shared: {n} tokens of {nh} heads over {nkv} of {hd} in {q.dtype} are not taken")
+    if q.shape[1] != nh * hd or out.shape != q.shape or cache_layer.shape[1] != 2 or cache_layer.shape[2] != nkv or cache_layer.shape[4] != hd:
+        raise KernelError("attention_shared: shapes do not fit the head counts")
+    if token_seg.shape[0] != T or positions.shape[0] != T:
+        raise KernelError("attention_shared: per-token arrays differ in length")
+    if starts.shape[0] != families + 1 or families > SHARED_MAX_TOKENS:
+        raise KernelError("attention_shared: starts is not one longer than shared, or there are more than 256 families")
+    if scratch.numel() < attention_shared_scratch_bytes(n, nh, nkv, hd):
+        raise KernelError("attention_shared: the scratch is too small")
+    _on_current("attention_shared", q, cache_layer, block_tables, token_seg, positions, members, starts, shared, out, scratch)
+    _check(lib().vk_attention_shared(_p(q), _p(cache_layer), _p(block_tables), _p(token_seg), _p(positions), _p(members), _p(starts), _p(shared), _p(out),
+                                     _p(scratch), T, block_tables.shape[0], n, families, cache_layer.shape[0], nh, nkv, hd, page_size,
+                                     block_tables.shape[1], ctypes.c_float(scale), _dt(q), _stream()), "attention_shared")
+    return out
+
+
+BEAM_MAX_BEAMS, BEAM_MAX_KEEP, BEAM_MAX_ROWS, BEAM_MAX_VOCAB = 64, 128, 1024, 64 * 4096
+
+
+def beam_select_scratch_bytes(rows: int, vocab: int, keep: int) -> int:
+    fn = lib().vk_beam_select_scratch_bytes
+    fn.restype = ctypes.c_size_t
+    return int(fn(rows, vocab, keep))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: int, out: tuple, scratch: torch.Tensor) -> tuple:
+    """The `keep` best continuations of every request: of scores[r] + log_softmax(logits[r])[v] over the request's `beams` neighbouring rows r
+    and all v, in descending order, the lowest (row, v) first among equals.  logits float32 [requests * beams, vocab] (rows may lie apart); scores float32 [requests * beams], sums of log
+    probabilities.  out = (scores float32, row within the request int32, v int32), each [requests, keep]; returns it.  A row without a softmax (a
+    NaN, an infinite maximum, nothing above -inf) or whose score is not finite (a beam that does not live) offers its tokens at -inf.
+    scratch: a byte buffer of beam_select_scratch_bytes(rows, vocab, keep) or more, zeros at first use, for launches of one stream at a time."""
+    if not logits.is_cuda or logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise KernelError("beam_select: logits are not a float32 CUDA matrix with unit column stride")
+    _req(scores, "scores", torch.float32, 1); _req(scratch, "scratch", torch.uint8, 1)
+    best, parent, token = out
+    _req(best, "out[0]", torch.float32, 2); _req(parent, "out[1]", torch.int32, 2); _req(token, "out[2]", torch.int32, 2)
+    R, V = logits.shape
+    if not (1 <= beams <= BEAM_MAX_BEAMS and 1 <= keep <= BEAM_MAX_KEEP and R <= BEAM_MAX_ROWS and 1 <= V <= BEAM_MAX_VOCAB):
+        raise KernelError(f"beam_select: {beams} beams (of {R} rows) over {V} tokens, {keep} kept: at most {BEAM_MAX_BEAMS}, {BEAM_MAX_ROWS}, {BEAM_MAX_VOCAB} and {BEAM_MAX_KEEP}")
+    if R % beams or scores.shape[0] != R or keep > beams * V:
+        raise KernelError("beam_select: rows are not whole requests, scores are not one a row, or more is kept than there is")
+    if best.shape != (R // beams, keep) or parent.shape != best.shape or token.shape != best.shape:
+        raise KernelError("beam_select: out is not three of [requests, keep]")
+    if scratch.numel() < beam_select_scratch_bytes(R, V, keep):
+        raise KernelError("beam_select: the scratch is too small")
+    _on_current("beam_select", logits, scores, best, parent, token, scratch)
+    _check(lib().vk_beam_select(_p(logits), _p(scores), _p(best), _p(parent), _p(token), _p(scratch), R, beams, V,
+                                ctypes.c_longlong(max(V, logits.stride(0)) if R > 1 else V), keep, _stream()), "beam_select")
+    return out
+
+
+def copy_rows(arena: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> torch.Tensor:
+    """arena[l, dst[i]] = arena[l, src[i]] for every layer l and move i, in one launch (one a 128 moves).  arena [layers, rows, ...], any type; a row's
+    elements lie together, rows and layers may lie apart.  src and dst are row numbers on the host: no row is written twice, or read and written.
+    A captured graph repeats the moves it was captured with."""
+    if not arena.is_cuda or arena.dim() < 2:
+        raise KernelError("copy_rows: the arena is not a CUDA tensor [layers, rows, ...]")
+    L, N, size = arena.shape[0], arena.shape[1], arena.element_size()
+    numbers = 1
+    for d in range(arena.dim() - 1, 1, -1):
+        if arena.shape[d] != 1 and arena.stride(d) != numbers:
+            raise KernelError("copy_rows: a row's elements do not lie together")
+        numbers *= arena.shape[d]
+    n, written = len(src), set(dst)
+    if len(dst) != n or len(written) != n or not written.isdisjoint(src):
+        raise KernelError("copy_rows: src and dst differ in length, or a row is written twice, or read and written")
+    if n == 0 or L == 0 or numbers == 0:
+        return arena
+    if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= N:
+        raise KernelError(f"copy_rows: a row is outside the arena's {N}")
+    row, layer = arena.stride(1), arena.stride(0)
+    if row < numbers or (L > 1 and layer < (N - 1) * row + numbers):
+        raise KernelError("copy_rows: rows or layers overlap")
+    _on_current("copy_rows", arena)
+    ints = ctypes.c_int32 * n
+    _check(lib().vk_copy_rows(_p(arena), L, N, ctypes.c_longlong(layer * size if L > 1 else 0), ctypes.c_longlong(row * size), ctypes.c_longlong(numbers * size),
+                              ints(*src), ints(*dst), n, _stream()), "copy_rows")
+    return arena
