@@ -13,11 +13,11 @@
 
 namespace vk {
 
-constexpr int SG_KEYS = 32, SG_ROWS = SA_PREFIX_ROWS / (SA_THREADS / 32);      // rows a warp
+constexpr int SG_KEYS = 32, SG_PREFIX_ROWS = 64, SG_ROWS = SG_PREFIX_ROWS / (SA_THREADS / 32);      // rows a block, rows a warp
 
 // Shared memory: the plan, then the rows' queries [64][hd] and the keys' and values' tiles [32][hd + 4].
 __host__ __device__ inline size_t sg_plan_bytes() { return (sizeof(SaPlan) + 15) / 16 * 16; }
-static size_t sg_smem(int hd) { return sg_plan_bytes() + (size_t)(SA_PREFIX_ROWS * hd + 2 * SG_KEYS * (hd + 4)) * 4; }
+static size_t sg_smem(int hd) { return sg_plan_bytes() + (size_t)(SG_PREFIX_ROWS * hd + 2 * SG_KEYS * (hd + 4)) * 4; }
 
 // A block walks a part and leaves its rows; `alone`: they are all there is of the unit, and the result is written.
 template <typename T, int DIMS>
@@ -110,40 +110,148 @@ __global__ void __launch_bounds__(SA_THREADS) attention_shared_kernel(const SaAr
     extern __shared__ __align__(16) unsigned char smem[];
     SaPlan& p = *reinterpret_cast<SaPlan*>(smem);
     float* sq = reinterpret_cast<float*>(smem + sg_plan_bytes());
-    float* sk = sq + SA_PREFIX_ROWS * a.hd;
+    float* sk = sq + SG_PREFIX_ROWS * a.hd;
     float* sv = sk + SG_KEYS * (a.hd + 4);
-    __shared__ int last[SA_PREFIX_ROWS];
-    const int warp = threadIdx.x >> 5, worker = blockIdx.x;
+    const int worker = blockIdx.x;
+    sa_make_plan(a, p);                       // from the step's metadata, which no kernel writes
     dependency_wait();
     let_dependents_start();
-    sa_make_plan(a, p);
-    long long at = (long long)worker * p.lp, end = min(at + p.lp, p.pbase[SA_MAX_TOKENS]);
+    SaPart r;
+    int at = worker * p.lp, end = min(at + p.lp, p.pbase[SA_MAX_TOKENS]);
     while (at < end) {
-        const SaPart r = sa_prefix_part(a, p, at, end, worker);
+        if (!sa_prefix_part(a, p, at, end, worker, r)) continue;
         sg_walk<T, DIMS>(a, p, r, false, sq, sk, sv);
-        __syncthreads();
-        if ((int)threadIdx.x < r.i1 - r.i0) last[threadIdx.x] = p.pos[r.i0 + threadIdx.x] >= 0 && sa_last(a, p, r.i0 + threadIdx.x, r.kvh);
-        __syncthreads();
-        for (int i = r.i0; i < r.i1; i++)
-            if (last[i - r.i0])
-                for (int h = warp; h < a.gq; h += SA_THREADS / 32) sa_join<T, DIMS>(a, p, i, r.kvh, h);
-        at += r.k1 - r.k0;
     }
-    at = (long long)worker * p.lo;
+    at = worker * p.lo;
     end = min(at + p.lo, p.obase[SA_MAX_TOKENS]);
     while (at < end) {
         int parts;
-        const SaPart r = sa_own_part(a, p, at, end, worker, parts);
-        const bool alone = parts == 1 && p.shared[r.g] == 0;      // then the unit's rows need nobody else
-        sg_walk<T, DIMS>(a, p, r, alone, sq, sk, sv);
-        __syncthreads();
-        if (threadIdx.x == 0) last[0] = sa_last(a, p, r.i0, r.kvh);
-        __syncthreads();
-        if (last[0])
-            for (int h = warp; h < a.gq; h += SA_THREADS / 32)
-                if (!(p.shared[r.g] == 0 && sa_own_parts(p, r.i0, r.kvh, h / SA_OWN_ROWS) == 1)) sa_join<T, DIMS>(a, p, r.i0, r.kvh, h);
-        at += r.k1 - r.k0;
+        if (!sa_own_part(a, p, at, end, worker, r, parts)) continue;
+        sg_walk<T, DIMS>(a, p, r, parts == 1 && p.shared[r.g] == 0, sq, sk, sv);      // a unit that needs nobody else writes its result
     }
+    sa_write_rows(a, p);
+}
+
+// A row's parts meet: weights 2^(own maximum - row maximum), sums in the parts' order within a lane, then over the lanes, then over the warps, the same in every launch of
+// the same lengths.  WARPS warps a row: one where the rows alone fill the machine, four where few rows have many parts.  A part's row is read as 16-byte pieces by
+// L = 2, 4 .. 32 neighbouring lanes, 32 / L parts at once and four of those in flight.
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(128) attention_shared_join_kernel(const SaRow* __restrict__ rows, const float2* __restrict__ part_ml, const float* __restrict__ part_o,
+                                                                    const int32_t* __restrict__ members, T* __restrict__ out, int n_rows, int nh, int hd, int lanes) {
+    constexpr int PIECES = 2, FLIGHT = 4;          // pieces of 16 bytes a lane has of a row of up to 256
+    __shared__ float2 warp_ml[4];
+    __shared__ float4 warp_o[4][32 * PIECES];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WARPS, r = blockIdx.x * (4 / WARPS) + warp / WARPS;
+    dependency_wait();
+    let_dependents_start();
+    SaRow row = {0, 0, 0, 0};
+    if (r < n_rows) row = rows[r];
+    const int parts = row.prefix_parts + row.own_parts;
+    if (parts == 0) return;                                       // with several warps a row the whole block
+    const int at_once = 32 / lanes, slot = lane / lanes, piece = lane % lanes, vec = hd / 4;
+    float m = -INFINITY, l = 0.0f;
+    float4 o[PIECES];
+#pragma unroll
+    for (int d = 0; d < PIECES; d++) o[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j0 = sub * at_once + slot; j0 < parts; j0 += FLIGHT * WARPS * at_once) {
+        float2 ml[FLIGHT];
+        float4 v[FLIGHT][PIECES];
+#pragma unroll
+        for (int f = 0; f < FLIGHT; f++) {
+            const int j = j0 + f * WARPS * at_once;
+            const bool on = j < parts;
+            const int from = j < row.prefix_parts ? row.prefix_row + j : row.own_row + j - row.prefix_parts;
+            ml[f] = on ? __ldcg(part_ml + from) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int d = 0; d < PIECES; d++)
+                v[f][d] = on && piece + d * lanes < vec ? __ldcg(reinterpret_cast<const float4*>(part_o + (size_t)from * hd) + piece + d * lanes) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        float top = m;
+#pragma unroll
+        for (int f = 0; f < FLIGHT; f++) top = fmaxf(top, ml[f].x);
+        const float ref = top == -INFINITY ? 0.0f : top, keep = sa_ex2(m - ref);       // no score above -inf so far: every weight is 0
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < PIECES; d++) { o[d].x *= keep; o[d].y *= keep; o[d].z *= keep; o[d].w *= keep; }
+#pragma unroll
+        for (int f = 0; f < FLIGHT; f++) {
+            const float w = sa_ex2(ml[f].x - ref);
+            l += ml[f].y * w;
+#pragma unroll
+            for (int d = 0; d < PIECES; d++) { o[d].x += v[f][d].x * w; o[d].y += v[f][d].y * w; o[d].z += v[f][d].z * w; o[d].w += v[f][d].w * w; }
+        }
+        m = top;
+    }
+    __syncwarp();
+    for (int x = lanes; x < 32; x <<= 1) {                        // the lanes that had other parts of the same piece
+        const float om = __shfl_xor_sync(0xffffffffu, m, x), top = fmaxf(m, om), ref = top == -INFINITY ? 0.0f : top, wa = sa_ex2(m - ref), wb = sa_ex2(om - ref);
+        l = l * wa + __shfl_xor_sync(0xffffffffu, l, x) * wb;
+#pragma unroll
+        for (int d = 0; d < PIECES; d++) {
+            o[d].x = o[d].x * wa + __shfl_xor_sync(0xffffffffu, o[d].x, x) * wb;
+            o[d].y = o[d].y * wa + __shfl_xor_sync(0xffffffffu, o[d].y, x) * wb;
+            o[d].z = o[d].z * wa + __shfl_xor_sync(0xffffffffu, o[d].z, x) * wb;
+            o[d].w = o[d].w * wa + __shfl_xor_sync(0xffffffffu, o[d].w, x) * wb;
+        }
+        m = top;
+    }
+    if (WARPS > 1) {
+        if (slot == 0) {
+            if (piece == 0) warp_ml[warp] = make_float2(m, l);
+#pragma unroll
+            for (int d = 0; d < PIECES; d++) warp_o[warp][piece + d * lanes] = o[d];
+        }
+        __syncthreads();
+        if (warp != 0) return;
+        m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) m = fmaxf(m, warp_ml[w].x);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < PIECES; d++) o[d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const float e = sa_ex2(warp_ml[w].x - ref);
+            l += warp_ml[w].y * e;
+#pragma unroll
+            for (int d = 0; d < PIECES; d++) {
+                const float4 v = warp_o[w][piece + d * lanes];
+                o[d].x += v.x * e; o[d].y += v.y * e; o[d].z += v.z * e; o[d].w += v.w * e;
+            }
+        }
+    }
+    if (slot != 0) return;
+    const int i = r / nh;
+    T* to = out + ((size_t)members[i] * nh + r - i * nh) * hd;
+#pragma unroll
+    for (int d = 0; d < PIECES; d++) {
+        const int at = (piece + d * lanes) * 4;
+        if (at >= hd) continue;
+        if (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(to + at) = make_float4(o[d].x / l, o[d].y / l, o[d].z / l, o[d].w / l);
+        } else {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(o[d].x / l, o[d].y / l), y = __floats2bfloat162_rn(o[d].z / l, o[d].w / l);
+            *reinterpret_cast<uint2*>(to + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+        }
+    }
+}
+
+static int launch_join(const SaArgs& a, int dtype, cudaStream_t stream) {
+    const int rows = a.n * a.nh;
+    int lanes = 2;
+    while (lanes < 32 && lanes * 4 < a.hd) lanes *= 2;
+    const SaRow* table = reinterpret_cast<const SaRow*>(a.rows);
+#define GO(T, WARPS)                                                                                                                                          \
+    return launch_dependent(attention_shared_join_kernel<T, WARPS>, dim3((rows + 4 / WARPS - 1) / (4 / WARPS)), dim3(128), 0, stream, table, a.part_ml, a.part_o, a.members, \
+                            static_cast<T*>(a.out), rows, a.nh, a.hd, lanes)
+    if (rows >= 1024) {
+        if (dtype == 0) GO(float, 1);
+        GO(__nv_bfloat16, 1);
+    }
+    if (dtype == 0) GO(float, 4);
+    GO(__nv_bfloat16, 4);
+#undef GO
 }
 
 static int sa_multiprocessors() {
@@ -152,26 +260,20 @@ static int sa_multiprocessors() {
     return n;
 }
 
-constexpr int SA_MAX_MULTIPROCESSORS = 160;         // of the sm_100a parts; the scratch is laid out for this many
-
-// Rows of parts that a launch can need: a unit of `keys` keys and up to R rows leaves at most R (keys / L + 2), L is at least the line's
-// length / workers, and the units' rows are n nh together.
-static size_t sa_part_rows(int tokens, int nh, int nkv) {
-    const size_t gq = nh / nkv, prefix_rows = gq > SA_PREFIX_ROWS ? gq : SA_PREFIX_ROWS, own_rows = gq < SA_OWN_ROWS ? gq : SA_OWN_ROWS;
-    return prefix_rows * SA_MAX_MULTIPROCESSORS + own_rows * SA_MAX_MULTIPROCESSORS * 8 + 4 * (size_t)tokens * nh;
-}
-
+// Rows of parts that a launch can need: a unit of so many tiles of keys and up to R rows leaves at most R (tiles / L + 2), L is at least the line's
+// length / workers, and the units' rows are n nh together.  R is 128 for prefixes here and the workers a multiprocessor's blocks (2) and warps (16), which covers
+// both kernels.
+static size_t sa_part_rows(int tokens, int nh) { return (size_t)(128 * 2 + SA_OWN_ROWS * 16) * SA_MAX_MULTIPROCESSORS + 4 * (size_t)tokens * nh; }
 
 }  // namespace vk
 
 using namespace vk;
 
-VK_API size_t vk_attention_shared_scratch_bytes(int tokens, int nh, int nkv, int hd) {
-    return (size_t)SA_MAX_TOKENS * SA_MAX_KV_HEADS * 4 + sa_part_rows(tokens, nh, nkv) * ((size_t)hd * 4 + 8);
+VK_API size_t vk_attention_shared_scratch_bytes(int tokens, int nh, int, int hd) {
+    return sa_part_rows(tokens, nh) * ((size_t)hd * 4 + 8) + (size_t)tokens * nh * 16;
 }
 
-// dtype 0 = float32, 1 = bfloat16.  scratch: vk_attention_shared_scratch_bytes(n, ...) bytes whose counters (the first SA_MAX_TOKENS *
-// SA_MAX_KV_HEADS words) were zero at first use; the kernel leaves them zero.
+// dtype 0 = float32, 1 = bfloat16.  scratch: vk_attention_shared_scratch_bytes(n, ...) bytes, whatever they hold.
 VK_API int vk_attention_shared(const void* q, const void* cache, const int32_t* block_tables, const int32_t* token_seg, const int32_t* positions,
                                const int32_t* members, const int32_t* starts, const int32_t* shared, void* out, void* scratch, int tokens, int segments,
                                int n, int families, int pages, int nh, int nkv, int hd, int page_size, int max_blocks, float scale, int dtype,
@@ -179,33 +281,42 @@ VK_API int vk_attention_shared(const void* q, const void* cache, const int32_t* 
     if (n <= 0 || families <= 0) return VK_OK;
     if (n > SA_MAX_TOKENS || families > SA_MAX_TOKENS || nkv > SA_MAX_KV_HEADS || hd > 256) return VK_TOO_LARGE;
     const int vec = dtype == 0 ? 4 : 8;
-    if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > SA_PREFIX_ROWS || hd <= 0 || hd % vec || page_size <= 0 || max_blocks <= 0 || pages <= 0) return VK_BAD_SHAPE;
+    if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > SA_MAX_HEADS || hd <= 0 || hd % vec || page_size <= 0 || max_blocks <= 0 || pages <= 0) return VK_BAD_SHAPE;
     if ((long long)max_blocks * page_size > 0x7fffffffLL) return VK_TOO_LARGE;
+    // the lines' tiles and the parts' rows are counted in 31 bits
+    const long long tiles = (long long)max_blocks * page_size / SA_TILE + 64, units = (long long)n * nh;
+    if (tiles * units > 0x7fffffffLL || units * 4 * hd > 0x7fffffffLL) return VK_TOO_LARGE;
     if (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)out | (uintptr_t)scratch) % 16) return VK_BAD_ALIGNMENT;
     const int sms = sa_multiprocessors();
     if (sms > SA_MAX_MULTIPROCESSORS) return VK_TOO_LARGE;
     SaArgs a;
     a.q = q; a.cache = cache; a.block_tables = block_tables; a.token_seg = token_seg; a.positions = positions;
     a.members = members; a.starts = starts; a.shared = shared; a.out = out;
-    const size_t rows = sa_part_rows(n, nh, nkv);
-    a.counters = (int*)scratch;
-    a.part_o = (float*)((char*)scratch + (size_t)SA_MAX_TOKENS * SA_MAX_KV_HEADS * 4);
+    const size_t rows = sa_part_rows(n, nh);
+    a.rows = (int4*)scratch;
+    a.part_o = (float*)(a.rows + (size_t)n * nh);
     a.part_ml = (float2*)(a.part_o + rows * hd);
     a.n = n; a.families = families; a.tokens = tokens; a.segments = segments; a.pages = pages;
     a.nh = nh; a.nkv = nkv; a.gq = nh / nkv; a.hd = hd; a.page_size = page_size; a.max_blocks = max_blocks;
     a.page_shift = -1;
     for (int b = 0; b < 30; b++) if ((1 << b) == page_size) a.page_shift = b;
     a.scale_log2 = scale * 1.4426950408889634f;
+    if (attention_shared_mma_takes(a, dtype)) {
+        const int status = launch_attention_shared_mma(a, sms, stream);
+        return status != VK_OK ? status : launch_join(a, dtype, stream);
+    }
+    a.prefix_rows = SG_PREFIX_ROWS;
     a.prefix_workers = a.own_workers = sms;
-    a.min_prefix = 64;
-    a.min_own = 64;
+    a.min_prefix = a.min_own = 4;
+    a.prefix_cost = a.own_cost = 4;
     const size_t smem = sg_smem(hd);
 #define GO(T, DIMS)                                                                                                                     \
     do {                                                                                                                                \
         auto kern = attention_shared_kernel<T, DIMS>;                                                                                   \
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                             \
         if (e != cudaSuccess) return (int)e;                                                                                            \
-        return launch_dependent(kern, dim3(sms), dim3(SA_THREADS), smem, stream, a);                                                    \
+        const int status = launch_dependent(kern, dim3(sms), dim3(SA_THREADS), smem, stream, a);                                        \
+        return status != VK_OK ? status : launch_join(a, dtype, stream);                                                                \
     } while (0)
     if (dtype == 0) {
         if (hd <= 64) GO(float, 2);

@@ -1,0 +1,334 @@
+// Decode attention over pages held in common, bfloat16 heads of 64 and 128, on the tensor cores.
+//
+// The mathematics and the cut into parts are attention_shared.cu's and attention_shared_plan.cuh's.  A part's rows (a family's members times the heads
+// that read one key-value head) are the 16-row operands of m16n8k16 products, 16 rows a warp; R = 1, 2, 4 or 8 warps that cover a part's rows
+// make a group that works through the same keys, and the block's 8 / R groups take turns at the tiles of 16 R keys.  So a block holds up to 128 rows
+// against keys that are read once, and with few rows all eight warps still read keys of their own.
+//
+//   copy      three stages of 128 keys and values a block by cp.async, each warp asks for 16 keys of its group's tile and the group meets once a tile;
+//             16-byte pieces are stored at piece ^ (key & 7), so that ldmatrix meets no bank twice
+//   scores    S = Q K^T, the queries in registers
+//   softmax   a running maximum and sum a row, float32, in base 2; the output is scaled only when a row's maximum rose
+//   p v       the probabilities go from the score registers into the 16-row operand as a high and a low bfloat16 part (p to 2^-17)
+//
+// A member's own keys are walked by single warps with the same routine (R = 1): up to 16 rows of heads.
+#include "attention_shared_plan.cuh"
+
+namespace vk {
+
+constexpr int SM_STAGES = 3, SM_WARP_KEYS = 16, SM_KEYS = SM_WARP_KEYS * (SA_THREADS / 32), SM_PREFIX_ROWS = 128;
+
+template <int HD> struct SmSmem {
+    static constexpr int HALF = SM_KEYS * HD * 2;                                     // bytes of a stage's keys, or values
+    static constexpr int STAGE = 2 * HALF;
+    static constexpr int OUT = (SA_THREADS / 32) * 16 * (HD + 4) * 4;                 // the warps' outputs where a part's groups meet: over the stages
+    static constexpr int PLAN = (sizeof(SaPlan) + 127) / 128 * 128;
+    static constexpr size_t BYTES = PLAN + (size_t)SM_STAGES * STAGE;
+    static constexpr int ML = (SA_THREADS / 32) * 16 * 8;                             // and, behind them, their maxima and sums
+    static_assert(OUT + ML <= SM_STAGES * STAGE, "the warps' outputs lie over the stages");
+};
+
+__device__ __forceinline__ uint32_t sm_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void sm_copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void sm_ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void sm_ldsm4_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+__device__ __forceinline__ void sm_mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t sm_pack(float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// What a warp has of its 16 rows: lane (gq, qd) = (lane / 4, lane % 4) rows gq and gq + 8, dims 8 b + 2 qd and the next; the sums over this lane's keys alone.
+template <int HD> struct SmRows {
+    float o[HD / 8][4], m[2], l[2];
+};
+
+// A warp's walk over tiles tile0, tile0 + step, ... of 16 R keys of a part, for the rows whose queries are in qf.  `group` is the group's place among the block's, `wr` the
+// warp's in the group.
+template <int HD, int R>
+__device__ __forceinline__ void sm_walk(const SaArgs& a, const SaPart& part, int tile0, int step, int group, int wr, const uint32_t (&qf)[HD / 16][4], SmRows<HD>& x, uint32_t stages) {
+    constexpr int TK = SM_WARP_KEYS * R, CH = HD / 8, SUB = R == 1 ? 16 : 32, NB = SUB / 8;
+    const int lane = threadIdx.x & 31;
+    const __nv_bfloat16* cache = static_cast<const __nv_bfloat16*>(a.cache);
+    const uint32_t v_rows = (uint32_t)a.nkv * a.page_size;
+    const int tiles = (part.k1 - part.k0 + TK - 1) / TK, mine = tile0 < tiles ? (tiles - tile0 + step - 1) / step : 0;
+    const int base_row = group * TK;
+#pragma unroll
+    for (int b = 0; b < HD / 8; b++) { x.o[b][0] = x.o[b][1] = x.o[b][2] = x.o[b][3] = 0.0f; }
+    x.m[0] = x.m[1] = -INFINITY;
+    x.l[0] = x.l[1] = 0.0f;
+
+    // the row of the pool that holds key `lane % 16` of this warp's keys of the n-th tile; none: ~0
+    auto row_of = [&](int n) -> uint32_t {
+        const int key = part.k0 + (tile0 + n * step) * TK + wr * SM_WARP_KEYS + (lane & 15);
+        if (n >= mine || key >= part.k1) return 0xffffffffu;
+        const int block = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+        const int page = part.table[block];
+        if ((uint32_t)page >= (uint32_t)a.pages) return 0xffffffffu;
+        return ((uint32_t)page * 2u * a.nkv + part.kvh) * a.page_size + (key - block * a.page_size);
+    };
+    auto issue = [&](int n, uint32_t rows) {
+        if (n < mine) {
+            const uint32_t stage = stages + (n % SM_STAGES) * SmSmem<HD>::STAGE;
+#pragma unroll
+            for (int i = 0; i < SM_WARP_KEYS * CH / 32; i++) {
+                const int c = i * 32 + lane, kl = c / CH, piece = c % CH;
+                const uint32_t row = __shfl_sync(0xffffffffu, rows, kl);
+                const bool there = row != 0xffffffffu;
+                const __nv_bfloat16* src = cache + (there ? (size_t)row * HD + piece * 8 : 0);
+                const uint32_t dst = stage + ((base_row + wr * SM_WARP_KEYS + kl) * CH + (piece ^ (kl & 7))) * 16;
+                sm_copy16(dst, src, there);
+                sm_copy16(dst + SmSmem<HD>::HALF, there ? src + (size_t)v_rows * HD : src, there);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    issue(0, row_of(0));
+    issue(1, row_of(1));
+    uint32_t rows = row_of(2);
+    for (int n = 0; n < mine; n++) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (R == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(R * 32) : "memory");
+        issue(n + 2, rows);                                // into the stage of the tile before, which the whole group is past
+        rows = row_of(n + 3);
+        const uint32_t sk = stages + (n % SM_STAGES) * SmSmem<HD>::STAGE, sv = sk + SmSmem<HD>::HALF;
+        const int key0 = part.k0 + (tile0 + n * step) * TK;
+#pragma unroll
+        for (int sub = 0; sub < TK; sub += SUB) {
+            if (key0 + sub >= part.k1) break;
+            float s[NB][4];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) { s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.0f; }
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ks++)
+#pragma unroll
+                for (int nb = 0; nb < NB; nb += 2) {
+                    const int kl = sub + nb * 8 + (lane & 7) + ((lane >> 4) << 3);
+                    uint32_t b[4];
+                    sm_ldsm4(b, sk + ((base_row + kl) * CH + ((ks * 2 + ((lane >> 3) & 1)) ^ (kl & 7))) * 16);
+                    sm_mma(s[nb], qf[ks], b[0], b[1]);
+                    sm_mma(s[nb + 1], qf[ks], b[2], b[3]);
+                }
+            const bool edge = key0 + sub + SUB > part.k1;
+            float top[2] = {x.m[0], x.m[1]};
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float v = s[nb][e] * a.scale_log2;
+                    if (edge && key0 + sub + nb * 8 + (lane & 3) * 2 + (e & 1) >= part.k1) v = -INFINITY;
+                    s[nb][e] = v;
+                    top[e >> 1] = fmaxf(top[e >> 1], v);
+                }
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            }
+            if (__any_sync(0xffffffffu, top[0] > x.m[0] || top[1] > x.m[1])) {
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const float keep = top[r] == -INFINITY ? 0.0f : sa_ex2(x.m[r] - top[r]);
+                    x.l[r] *= keep;
+#pragma unroll
+                    for (int b = 0; b < HD / 8; b++) { x.o[b][2 * r] *= keep; x.o[b][2 * r + 1] *= keep; }
+                    x.m[r] = top[r];
+                }
+            }
+            const float ref[2] = {x.m[0] == -INFINITY ? 0.0f : x.m[0], x.m[1] == -INFINITY ? 0.0f : x.m[1]};       // no score above -inf so far: p = 0
+            uint32_t ph[NB / 2][4], pl[NB / 2][4];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const float p0 = sa_ex2(s[nb][2 * r] - ref[r]), p1 = sa_ex2(s[nb][2 * r + 1] - ref[r]);
+                    x.l[r] += p0 + p1;
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+                    ph[nb >> 1][(nb & 1) * 2 + r] = *reinterpret_cast<const uint32_t*>(&h);
+                    pl[nb >> 1][(nb & 1) * 2 + r] = sm_pack(p0 - __bfloat162float(h.x), p1 - __bfloat162float(h.y));
+                }
+#pragma unroll
+            for (int kk = 0; kk < NB / 2; kk++)
+#pragma unroll
+                for (int db = 0; db < HD / 8; db += 2) {
+                    const int kl = sub + kk * 16 + (lane & 15);
+                    uint32_t b[4];
+                    sm_ldsm4_trans(b, sv + ((base_row + kl) * CH + ((db + (lane >> 4)) ^ (kl & 7))) * 16);
+                    sm_mma(x.o[db], ph[kk], b[0], b[1]);
+                    sm_mma(x.o[db + 1], ph[kk], b[2], b[3]);
+                    sm_mma(x.o[db], pl[kk], b[0], b[1]);
+                    sm_mma(x.o[db + 1], pl[kk], b[2], b[3]);
+                }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        x.l[r] += __shfl_xor_sync(0xffffffffu, x.l[r], 1);
+        x.l[r] += __shfl_xor_sync(0xffffffffu, x.l[r], 2);
+    }
+}
+
+// The queries of rows row0 + gq and row0 + gq + 8 of a part as the 16-row operand (zeros where there is no such row, or its member is not there).
+template <int HD>
+__device__ __forceinline__ void sm_queries(const SaArgs& a, const SaPlan& p, const SaPart& part, int row0, uint32_t (&qf)[HD / 16][4]) {
+    const int lane = threadIdx.x & 31, rows = (part.i1 - part.i0) * part.heads;
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int row = row0 + (lane >> 2) + 8 * r, i = part.i0 + row / part.heads;
+        const bool on = row < rows && p.pos[min(i, SA_MAX_TOKENS - 1)] >= 0;
+        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (on ? ((size_t)p.tok[i] * a.nh + part.kvh * a.gq + part.h0 + row % part.heads) * HD : 0) + 2 * (lane & 3);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ks++) {
+            qf[ks][r] = on ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
+            qf[ks][r + 2] = on ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
+        }
+    }
+}
+
+// A block's part of a family's prefix: 8 / R groups of R warps; their outputs meet in shared memory and the part's rows are written.
+template <int HD, int R>
+__device__ __forceinline__ void sm_prefix(const SaArgs& a, const SaPlan& p, const SaPart& part, unsigned char* stages) {
+    constexpr int GROUPS = (SA_THREADS / 32) / R, LD = HD + 4;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp / R, wr = warp % R;
+    const int rows = (part.i1 - part.i0) * part.heads;
+    uint32_t qf[HD / 16][4];
+    sm_queries<HD>(a, p, part, wr * 16, qf);
+    SmRows<HD> x;
+    sm_walk<HD, R>(a, part, group, GROUPS, group, wr, qf, x, sm_addr(stages));
+    if (GROUPS == 1) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int row = wr * 16 + (lane >> 2) + 8 * r;
+            if (row >= rows) continue;
+            const int at = part.row0 + row * part.stride;
+#pragma unroll
+            for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(a.part_o + (size_t)at * HD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
+            if ((lane & 3) == 0) a.part_ml[at] = make_float2(x.m[r], x.l[r]);
+        }
+        return;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                                       // every group is past its tiles
+    float* out = reinterpret_cast<float*>(stages);         // [8 warps][16][LD]
+    float2 (*ml)[16] = reinterpret_cast<float2 (*)[16]>(stages + SmSmem<HD>::OUT);
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int row = (lane >> 2) + 8 * r;
+#pragma unroll
+        for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(out + (warp * 16 + row) * LD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
+        if ((lane & 3) == 0) ml[warp][row] = make_float2(x.m[r], x.l[r]);
+    }
+    __syncthreads();
+    for (int c = tid; c < rows * (HD / 4); c += SA_THREADS) {
+        const int row = c / (HD / 4), d = c % (HD / 4) * 4, w0 = row / 16, rr = row % 16;
+        float m = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) m = fmaxf(m, ml[g * R + w0][rr].x);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) {
+            const float2 s = ml[g * R + w0][rr];
+            const float w = sa_ex2(s.x - ref);
+            const float4 v = *reinterpret_cast<const float4*>(out + ((g * R + w0) * 16 + rr) * LD + d);
+            l += s.y * w;
+            o.x += v.x * w; o.y += v.y * w; o.z += v.z * w; o.w += v.w * w;
+        }
+        const int at = part.row0 + row * part.stride;
+        *reinterpret_cast<float4*>(a.part_o + (size_t)at * HD + d) = o;
+        if (d == 0) a.part_ml[at] = make_float2(m, l);
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared_mma_kernel(const SaArgs a) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    SaPlan& p = *reinterpret_cast<SaPlan*>(smem);
+    unsigned char* stages = smem + SmSmem<HD>::PLAN;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    sa_make_plan(a, p);                       // from the step's metadata, which no kernel writes
+    dependency_wait();
+    let_dependents_start();
+    SaPart part;
+    int at = blockIdx.x * p.lp, end = min(at + p.lp, p.pbase[SA_MAX_TOKENS]);
+    while (at < end) {
+        if (!sa_prefix_part(a, p, at, end, blockIdx.x, part)) continue;
+        const int rows = (part.i1 - part.i0) * part.heads;
+        if (rows <= 16) sm_prefix<HD, 1>(a, p, part, stages);
+        else if (rows <= 32) sm_prefix<HD, 2>(a, p, part, stages);
+        else if (rows <= 64) sm_prefix<HD, 4>(a, p, part, stages);
+        else sm_prefix<HD, 8>(a, p, part, stages);
+        __syncthreads();
+    }
+    // from here on every warp is by itself: neighbouring parts of the own keys go to different multiprocessors, first to those without a part of a prefix
+    const int worker = warp * gridDim.x + gridDim.x - 1 - blockIdx.x;
+    at = worker * p.lo;
+    end = min(at + p.lo, p.obase[SA_MAX_TOKENS]);
+    while (at < end) {
+        int parts;
+        if (!sa_own_part(a, p, at, end, worker, part, parts)) continue;
+        const bool alone = parts == 1 && p.shared[part.g] == 0;      // the unit needs nobody else
+        uint32_t qf[HD / 16][4];
+        sm_queries<HD>(a, p, part, 0, qf);
+        SmRows<HD> x;
+        __syncwarp();                                      // the lanes are past the tiles of the part before
+        sm_walk<HD, 1>(a, part, 0, 1, warp, 0, qf, x, sm_addr(stages));
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int row = (lane >> 2) + 8 * r;
+            if (row >= part.heads) continue;
+            if (alone) {
+                __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + ((size_t)p.tok[part.i0] * a.nh + part.kvh * a.gq + part.h0 + row) * HD + 2 * (lane & 3);
+                const float w = 1.0f / x.l[r];
+#pragma unroll
+                for (int b = 0; b < HD / 8; b++) *reinterpret_cast<uint32_t*>(out + b * 8) = sm_pack(x.o[b][2 * r] * w, x.o[b][2 * r + 1] * w);
+            } else {
+                const int to = part.row0 + row * part.stride;
+#pragma unroll
+                for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(a.part_o + (size_t)to * HD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
+                if ((lane & 3) == 0) a.part_ml[to] = make_float2(x.m[r], x.l[r]);
+            }
+        }
+    }
+    sa_write_rows(a, p);
+}
+
+// Rows of the pool are counted in 32 bits here.
+bool attention_shared_mma_takes(const SaArgs& a, int dtype) {
+    return dtype == 1 && (a.hd == 64 || a.hd == 128) && (long long)a.pages * 2 * a.nkv * a.page_size < 0x7fffffffLL;
+}
+
+int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream) {
+    a.prefix_rows = SM_PREFIX_ROWS;
+    const int blocks = multiprocessors * (a.hd == 64 ? 2 : 1);
+    a.prefix_workers = blocks;
+    a.own_workers = blocks * (SA_THREADS / 32);
+    a.min_prefix = 8;
+    a.min_own = 4;
+    a.prefix_cost = 16;
+    a.own_cost = 8;
+#define GO(HD)                                                                                                                                  \
+    do {                                                                                                                                        \
+        auto kern = attention_shared_mma_kernel<HD>;                                                                                            \
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SmSmem<HD>::BYTES);                        \
+        if (e != cudaSuccess) return (int)e;                                                                                                    \
+        return launch_dependent(kern, dim3(blocks), dim3(SA_THREADS), SmSmem<HD>::BYTES, stream, a);                                            \
+    } while (0)
+    if (a.hd == 64) GO(64);
+    GO(128);
+#undef GO
+}
+
+}  // namespace vk

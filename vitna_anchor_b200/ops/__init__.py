@@ -2272,8 +2272,8 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
     agree on the first shared[f] positions (any number: what lies at or behind the smallest of the members' positions is not counted).  A family
     may have one member or none.  Every token reads the positions 0 .. positions[t] of its own request, as in attention_decode; rows of `out` whose token
     is in no family are left as they were.  Block numbers outside the pool are not followed (their keys and values count as zeros).
-    scratch: a byte buffer of attention_shared_scratch_bytes(members, ...) or more, zeros at first use, for launches of one stream at a time (of any sizes it
-    is large enough for)."""
+    scratch: a byte buffer of attention_shared_scratch_bytes(members, ...) or more, whatever it holds, for launches of one stream at a time.  The lists and
+    lengths are read while the kernel before this one in the stream may still run: that must not be a kernel of this library which writes them."""
     _req(q, "q", dims=2); _req(cache_layer, "cache_layer", q.dtype, 5); _req(block_tables, "block_tables", torch.int32, 2)
     _req(token_seg, "token_seg", torch.int32, 1); _req(positions, "positions", torch.int32, 1); _req(out, "out", q.dtype, 2)
     _req(members, "members", torch.int32, 1); _req(starts, "starts", torch.int32, 1); _req(shared, "shared", torch.int32, 1); _req(scratch, "scratch", torch.uint8, 1)
@@ -2292,6 +2292,7 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
     _check(lib().vk_attention_shared(_p(q), _p(cache_layer), _p(block_tables), _p(token_seg), _p(positions), _p(members), _p(starts), _p(shared), _p(out),
                                      _p(scratch), T, block_tables.shape[0], n, families, cache_layer.shape[0], nh, nkv, hd, page_size,
                                      block_tables.shape[1], ctypes.c_float(scale), _dt(q), _stream()), "attention_shared")
+    add_launches(1)                       # the walk, and the launch that joins the rows' parts
     return out
 
 
