@@ -1,0 +1,226 @@
+"""The host side of beam search: requests that hold pages in common, who takes over whom, and what is refused; no GPU is needed."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from vitna_anchor_b200 import ops
+from vitna_anchor_b200.cache import CacheError, CacheManager, KVSpec, OutOfPages, PageGroup, PagePool, PageTables, StateSpec, UNMAPPED
+from vitna_anchor_b200.engine.beam import attainable, normalised, plan_moves
+
+
+def test_a_page_goes_back_with_its_last_holder():
+    pool = PagePool(2)
+    a = pool.alloc("x")
+    pool.share(a, "y")
+    pool.share(a, "z")
+    assert pool.holders(a) == ["x", "y", "z"] and pool.is_shared(a) and pool.free_pages == 1
+    with pytest.raises(CacheError):
+        pool.share(a, "y")
+    with pytest.raises(CacheError):
+        pool.free(a, "w")
+    pool.free(a, "x")
+    with pytest.raises(CacheError):
+        pool.free(a, "x")
+    pool.check()
+    pool.free(a, "z")
+    assert pool.holders(a) == ["y"] and not pool.is_shared(a) and pool.free_pages == 1
+    pool.free(a, "y")
+    assert pool.free_pages == 2 and pool.holders(a) == []
+    for page in (a, 1 - a, 5):
+        with pytest.raises(CacheError):
+            pool.share(page, "q")
+    pool.check()
+
+
+class Model:
+    """What the pages hold: every position a request wrote, by (group, page, offset)."""
+
+    def __init__(self, tables):
+        self.t, self.cells, self.history, self.next = tables, {}, {}, 0
+
+    def write(self, rid, n):
+        rc = self.t.get(rid)
+        first = rc.length
+        self.t.reserve(rid, n)
+        for pos in range(first, first + n):
+            self.next += 1
+            self.history[rid].append(self.next)
+            for g in range(len(self.t.groups)):
+                slot = self.t.slot_of_position(rid, g, pos)
+                assert len(self.t.pools[g].holders(slot // self.t.page_size)) == 1       # nobody else's page is written
+                self.cells[g, slot] = self.next
+        self.t.commit(rid)
+
+    def copy(self, moves):
+        read = [(g, a, b, [self.cells.get((g, a * self.t.page_size + o)) for o in range(self.t.page_size)]) for g, a, b in moves]
+        assert len({(g, b) for g, _, b, _ in read}) == len(read) and not {(g, b) for g, _, b, _ in read} & {(g, a) for g, a, _, _ in read}
+        for g, _, b, content in read:
+            for o, v in enumerate(content):
+                self.cells[g, b * self.t.page_size + o] = v
+
+    def check(self):
+        self.t.check()
+        for rid, history in self.history.items():
+            rc = self.t.get(rid)
+            assert rc.length == len(history)
+            for g, group in enumerate(self.t.groups):
+                lo = 0 if group.window == 0 else max(0, rc.length - group.window + 1)
+                for pos in range(lo, rc.length):
+                    assert self.cells[g, self.t.slot_of_position(rid, g, pos)] == history[pos]
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_forks_and_adoptions_keep_everybodys_positions(seed):
+    rng = random.Random(seed)
+    ps = rng.choice([1, 3, 4])
+    t = PageTables([PageGroup((0,), 1, 8, 0), PageGroup((1,), 1, 8, rng.choice([0, 5, 9]))], ps, [60, 60], 8)
+    m, n = Model(t), 0
+    for _ in range(200):
+        live = list(m.history)
+        what = rng.choice(["open", "write", "write", "fork", "adopt", "adopt", "close", "truncate"])
+        before = {r: (list(t.get(r).tables[0].blocks), t.get(r).length) for r in live}
+        try:
+            if what == "open" and len(live) < 8:
+                n += 1
+                t.open(n)
+                m.history[n] = []
+            elif what == "write" and live:
+                rid, count = rng.choice(live), rng.randint(1, 6)
+                if t.can_reserve([(rid, count)]):
+                    m.write(rid, count)
+            elif what == "fork" and live and len(live) < 8:
+                source = rng.choice(live)
+                n += 1
+                m.copy(t.fork(source, n))
+                m.history[n] = list(m.history[source])
+                assert t.get(n).family == t.get(source).family
+            elif what == "adopt" and len(live) > 1:
+                rng.shuffle(live)
+                k = rng.randint(1, len(live) - 1)
+                pairs = [(r, rng.choice(live[k:])) for r in live[:k]]
+                m.copy(t.adopt(pairs))
+                for r, source in pairs:
+                    m.history[r] = list(m.history[source])
+            elif what == "close" and live and rng.random() < 0.3:
+                rid = rng.choice(live)
+                t.close(rid)
+                del m.history[rid]
+            elif what == "truncate" and live:
+                rid = rng.choice(live)
+                length = rng.randint(0, t.get(rid).length)
+                t.truncate(rid, length)
+                del m.history[rid][length:]
+        except OutOfPages:
+            assert {r: (list(t.get(r).tables[0].blocks), t.get(r).length) for r in before} == before and len(t.requests) == len(m.history)
+        except CacheError as e:
+            assert what == "truncate", e                      # behind a window, or inside a page that others hold
+        m.check()
+    for rid in list(m.history):
+        t.close(rid)
+    assert [p.free_pages for p in t.pools] == [60, 60]
+
+
+def test_what_fork_and_adopt_refuse():
+    t = PageTables([PageGroup((0,), 1, 8, 0)], 4, [5], 3)
+    t.open("a")
+    t.reserve("a", 6)
+    with pytest.raises(CacheError):
+        t.fork("a", "b")                                      # a step is in flight
+    t.commit("a")
+    t.fork("a", "b")
+    t.open("c")
+    for pairs in [[("a", "a")], [("a", "b"), ("a", "c")], [("a", "b"), ("b", "c")], [("q", "a")], [("a", "q")]]:
+        with pytest.raises(CacheError):
+            t.adopt(pairs)
+    with pytest.raises(CacheError):
+        t.fork("a", "c")                                      # open already
+    t.close("c")
+    with pytest.raises(CacheError):
+        t.truncate("b", 2)                                    # inside the page both hold
+    t.truncate("b", 4)
+    assert t.get("b").length == 4
+    t.reserve("b", 12); t.commit("b")
+    t.open("d")
+    with pytest.raises(OutOfPages):
+        t.adopt([("d", "a")])                                 # a page for the end is wanted and none is free
+    assert t.get("d").length == 0
+    t.check()
+
+
+def test_states_of_one_shape_lie_in_one_arena():
+    specs = [StateSpec((3, 5)), KVSpec(2, 8), StateSpec((7,), torch.float64), StateSpec((3, 5))]
+    c = CacheManager(specs, page_size=4, num_pages=6, max_requests=5, dtype=torch.float32, device="cpu")
+    assert len(c._arenas) == 2 and c._arenas[0].shape == (2, 5, 15) and c._arenas[1].shape == (1, 5, 7)
+    for i, cid in enumerate([0, 3]):
+        view = c.views[cid].state
+        assert view.shape == (5, 3, 5) and view.is_contiguous() and (view.data_ptr() - c._arenas[0].data_ptr()) % 512 == 0
+        view[2] = i + 1.0
+        assert bool((c._arenas[0][i, 2] == i + 1.0).all())
+    assert c.views[2].state.dtype == torch.float64 and bool((c._arenas[1] == 0).all())
+
+
+def test_who_takes_over_whom():
+    assert plan_moves([0, 1, 2], "abc") == (["a", "b", "c"], [], [])
+    assert plan_moves([2, 2, 0], "abc") == (["c", "b", "a"], [("b", "c")], [])
+    assert plan_moves([1, 1, 1, 1], "abcd") == (["b", "a", "c", "d"], [("a", "b"), ("c", "b"), ("d", "b")], [])
+    assert plan_moves([0, 0, 0], "a") == (["a", None, None], [], [])
+    assert plan_moves([2], "abc") == (["c"], [], ["a", "b"])
+    rng = random.Random(1)
+    for _ in range(300):
+        live = list(range(100, 100 + rng.randint(1, 9)))
+        parents = [rng.randrange(len(live)) for _ in range(rng.randint(1, 9))]
+        requests, pairs, left = plan_moves(parents, live)
+        named = [r for r in requests if r is not None]
+        assert len(set(named)) == len(named) and not set(left) & set(named)
+        assert not {r for r, _ in pairs} & {s for _, s in pairs}
+        source = dict(pairs)
+        for r, p in zip(requests, parents):
+            assert r is None or source.get(r, r) == live[p]
+        assert (None in requests) <= (not left)
+
+
+def test_scores():
+    assert normalised(-6.0, 4, 0.5) == -3.0 and normalised(-6.0, 4, 0.0) == -6.0
+    assert attainable(-6.0, 4, 16, 0.5) == -1.5 and attainable(-6.0, 4, 16, -0.5) == -12.0 and attainable(-6.0, 4, 16, 0.0) == -6.0
+
+
+def test_entries_refuse_before_anything_runs():
+    """The C entries say no to sizes they do not take; nothing is launched, so no device is needed."""
+    lib, null = ops.lib(), ctypes.c_void_p(0)
+    some = ctypes.c_void_p(64)
+    LL = ctypes.c_longlong
+
+    def attention(n=4, families=1, nh=4, nkv=2, hd=64, ps=16, maxb=8, dtype=1, scratch=some):
+        return lib.vk_attention_shared(some, some, some, some, some, some, some, some, some, scratch, 4, 4, n, families, 10, nh, nkv, hd, ps, maxb, ctypes.c_float(0.1), dtype, null)
+
+    assert attention(n=0) == 0 and attention(families=0) == 0
+    for kw in [dict(n=257), dict(families=257), dict(hd=264), dict(nkv=129, nh=129), dict(hd=12), dict(nh=5), dict(nh=130), dict(ps=0), dict(maxb=0), dict(maxb=1 << 28),
+               dict(hd=6, dtype=0), dict(scratch=ctypes.c_void_p(72))]:
+        assert attention(**kw) < 0, kw
+
+    def select(rows=8, beams=4, vocab=100, ld=100, keep=8, scratch=some):
+        return lib.vk_beam_select(some, some, some, some, some, scratch, rows, beams, vocab, LL(ld), keep, null)
+
+    assert select(rows=0) == 0
+    for kw in [dict(beams=3), dict(beams=0), dict(keep=0), dict(keep=129), dict(vocab=0), dict(ld=99), dict(beams=1, keep=101), dict(rows=1028), dict(rows=130, beams=65),
+               dict(vocab=64 * 4096 + 1, ld=1 << 20), dict(scratch=null), dict(scratch=ctypes.c_void_p(8))]:
+        assert select(**kw) < 0, kw
+
+    def copy(rows=4, src=(0,), dst=(1,), stride=16, size=16, layers=1):
+        i = ctypes.c_int32 * len(src)
+        return lib.vk_copy_rows(some, layers, rows, LL(0), LL(stride), LL(size), i(*src), i(*dst), len(src), null)
+
+    assert copy(src=(), dst=()) == 0 and copy(layers=0) == 0 and copy(size=0) == 0
+    for kw in [dict(src=(4,)), dict(dst=(4,)), dict(src=(-1,)), dict(dst=(-1,)), dict(rows=0), dict(stride=8), dict(layers=70000)]:
+        assert copy(**kw) < 0, kw
+
+
+def test_command_line_of_a_search():
+    from vitna_anchor_b200.cli.main import main, parse_args
+    a = parse_args(["--beams", "4", "--length-penalty", "0.7", "--ids", "1"])
+    assert a["beams"] == 4 and a["length_penalty"] == 0.7
+    for argv in [["generate", "--model", "x", "--ids", "1", "--length-penalty", "1"], ["generate", "--model", "x", "--ids", "1", "--beams", "2", "--temperature", "0.5"],
+                 ["generate", "--model", "x", "--ids", "1", "--beams", "2", "--logits-out", "f"], ["generate", "--model", "x", "--ids", "1", "--beams", "two"]]:
+        assert main(argv) == 1

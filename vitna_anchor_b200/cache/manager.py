@@ -10,13 +10,16 @@ KVSpec form a group that shares page ids and has a pool of its own:
                   a page's keys [kv heads, page_size, head_dim] followed by its values [kv heads, page_size, v_dim];
                   values inside the keys: [layers, pages, kv heads * page_size * head_dim];
                   v_share key heads to a value head: the values are [kv heads / v_share, page_size, v_dim])
-    state[cache]  [max_requests, *shape]     one row per request slot
+    state[cache]  [max_requests, *shape]     one row per request slot (cache layers of one shape lie at equal distances in one allocation)
 
 A request holds one slot from open() to close(); its state rows are zeroed
-when the slot is taken.
+when the slot is taken.  fork() and adopt() let requests go on from where others
+stand: full pages are held in common, the page in the middle and the state rows are
+copied, one launch for each group of pages and each shape of states.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Dict, Hashable, List, Optional, Sequence, Tuple, Union
 
@@ -95,9 +98,19 @@ class CacheManager:
             for i, cid in enumerate(grp.cache_ids):
                 self.views[cid].group = g
                 self.views[cid].pages = pool[i] if pool is not None else None
+        self._arenas: List[torch.Tensor] = []            # [cache layers of the shape, max_requests, numbers]
+        by_state: Dict[StateSpec, List[int]] = {}
         for cid, spec in enumerate(self.specs):
             if isinstance(spec, StateSpec) and allocate:
-                self.views[cid].state = torch.zeros((max_requests, *spec.shape), dtype=spec.dtype, device=self.device)
+                by_state.setdefault(spec, []).append(cid)
+        for spec, ids in by_state.items():
+            numbers = math.prod(spec.shape)
+            size = torch.empty((), dtype=spec.dtype).element_size()
+            apart = -(-max_requests * numbers * size // 512) * 512 // size      # every layer begins as an allocation of its own would
+            whole = torch.zeros((len(ids) * apart,), dtype=spec.dtype, device=self.device)
+            self._arenas.append(whole.as_strided((len(ids), max_requests, numbers), (apart, numbers, 1)))
+            for i, cid in enumerate(ids):
+                self.views[cid].state = whole[i * apart:i * apart + max_requests * numbers].view(max_requests, *spec.shape)
 
     # -- sizes --------------------------------------------------------------------------------
     def bytes_per_token(self) -> int:
@@ -122,6 +135,27 @@ class CacheManager:
 
     def close(self, request_id: Hashable) -> None:
         self.tables.close(request_id)
+
+    def fork(self, source_id: Hashable, request_id: Hashable) -> int:
+        """Open request_id as one that goes on from where source_id stands (its keys, values and states); returns its slot."""
+        copies = self.tables.fork(source_id, request_id)
+        self._copy(copies, [(request_id, source_id)])
+        return self.tables.get(request_id).slot
+
+    def adopt(self, pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
+        """For every (request, source): the request forgets what it has and goes on from where the source stands.  No request is named
+        twice, or as a source too."""
+        if pairs:
+            self._copy(self.tables.adopt(list(pairs)), pairs)
+
+    def _copy(self, pages: Sequence[tuple], pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
+        from .. import ops
+        for g, pool in enumerate(self.pools):
+            moves = [(a, b) for group, a, b in pages if group == g]
+            if moves and pool is not None:
+                ops.copy_rows(pool, [a for a, _ in moves], [b for _, b in moves])
+        for arena in self._arenas:
+            ops.copy_rows(arena, [self.tables.get(s).slot for _, s in pairs], [self.tables.get(r).slot for r, _ in pairs])
 
     def length(self, request_id: Hashable) -> int:
         return self.tables.get(request_id).length

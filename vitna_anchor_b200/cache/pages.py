@@ -6,6 +6,12 @@ number (position // page_size) to a page id, or -1 where no page is held
 (before the first, or behind a window).  Pages are handed out from a LIFO
 stack, so a page that was just given back is the next one used.
 
+Requests may hold pages in common: fork() opens a request that goes on from
+where another stands, adopt() makes open requests go on from others.  Full
+pages are shared (a page goes back to its pool when its last holder gives it
+up); the page a request is in the middle of is always its own, since it will be
+written, so a fork takes a new page for it and names the copy to make.
+
 The reference keeps a contiguous cache per sequence slot
 (engine/include/model.h:106-110) and so never runs out in mid-request; its
 unused kv_cache.c names the vocabulary only (block, block table, unmapped =
@@ -14,7 +20,7 @@ all-ones).  The paging here is this engine's own.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, Hashable, List, Optional
+from typing import Dict, Hashable, List, Optional, Sequence
 
 UNMAPPED = -1
 
@@ -28,7 +34,8 @@ class OutOfPages(CacheError):
 
 
 class PagePool:
-    """`num_pages` page ids with an owner tag each.  alloc/free are O(1)."""
+    """`num_pages` page ids with an owner tag each, and further holders where a page is shared.  alloc/free are O(1) (free of a
+    shared page: in its holders)."""
 
     def __init__(self, num_pages: int):
         if num_pages < 1:
@@ -36,6 +43,7 @@ class PagePool:
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages - 1, -1, -1))  # pop() gives 0 first
         self._owner: List[Optional[Hashable]] = [None] * num_pages
+        self._more: Dict[int, List[Hashable]] = {}                  # shared pages: who holds them besides the owner
 
     @property
     def free_pages(self) -> int:
@@ -55,10 +63,36 @@ class PagePool:
             raise CacheError(f"page {page} is not in the pool")
         if self._owner[page] is None:
             raise CacheError(f"page {page} is freed twice")
+        more = self._more.get(page)
         if self._owner[page] != owner:
-            raise CacheError(f"page {page} belongs to {self._owner[page]!r}, not to {owner!r}")
-        self._owner[page] = None
-        self._free.append(page)
+            if more is None or owner not in more:
+                raise CacheError(f"page {page} belongs to {self._owner[page]!r}, not to {owner!r}")
+            more.remove(owner)
+        elif more is not None:
+            self._owner[page] = more.pop(0)
+        else:
+            self._owner[page] = None
+            self._free.append(page)
+            return
+        if not more:
+            del self._more[page]
+
+    def share(self, page: int, owner: Hashable) -> None:
+        """`owner` holds the page too, until it frees it."""
+        if owner is None:
+            raise CacheError("a page needs an owner")
+        if not (0 <= page < self.num_pages) or self._owner[page] is None:
+            raise CacheError(f"page {page} is held by nobody")
+        if owner in self.holders(page):
+            raise CacheError(f"page {page} is held by {owner!r} already")
+        self._more.setdefault(page, []).append(owner)
+
+    def holders(self, page: int) -> List[Hashable]:
+        """Who holds the page (nobody: it is free)."""
+        return [] if self._owner[page] is None else [self._owner[page], *self._more.get(page, ())]
+
+    def is_shared(self, page: int) -> bool:
+        return page in self._more
 
     def owner(self, page: int) -> Optional[Hashable]:
         return self._owner[page]
@@ -69,7 +103,7 @@ class PagePool:
         for p in self._free:
             if p in seen:
                 raise CacheError(f"page {p} is on the free list twice")
-            if self._owner[p] is not None:
+            if self._owner[p] is not None or p in self._more:
                 raise CacheError(f"page {p} is free and owned")
             seen.add(p)
         owned = sum(1 for o in self._owner if o is not None)
@@ -117,6 +151,7 @@ class RequestCache:
     slot: int
     length: int = 0                # positions whose keys and values are in the cache (committed)
     reserved: int = 0              # positions reserved beyond `length` for the step in flight
+    family: Hashable = None        # the request this one's pages began with: its own id, or that of the request it was forked from
     tables: Dict[int, GroupTable] = field(default_factory=dict)   # group index -> table
 
 
@@ -149,8 +184,89 @@ class PageTables:
             raise CacheError(f"request {request_id!r} is already open")
         rc = RequestCache(request_id, self.slots.acquire(request_id))
         rc.tables = {g: GroupTable() for g in range(len(self.groups))}
+        rc.family = request_id
         self.requests[request_id] = rc
         return rc
+
+    # -- requests that hold pages in common ---------------------------------------------------
+    def _tail_copies(self, rc: RequestCache) -> List[int]:
+        """The groups in which a request that goes on from rc needs a page of its own for the page rc is in the middle of."""
+        if rc.length % self.page_size == 0:
+            return []
+        return [g for g, t in rc.tables.items() if t.blocks[rc.length // self.page_size] != UNMAPPED]
+
+    def _continue(self, rc: RequestCache, source: RequestCache, kept: Sequence[int]) -> List[tuple]:
+        """rc, which holds source's first kept[g] blocks of every group and no others, holds what source has; returns (group, source's page, rc's
+        page) for each page to copy."""
+        copies = []
+        tails = self._tail_copies(source)
+        full = source.length // self.page_size
+        for g, table in source.tables.items():
+            mine = rc.tables[g]
+            mine.blocks += table.blocks[kept[g]:full]
+            mine.first_held = table.first_held
+            for page in mine.blocks[kept[g]:]:
+                if page != UNMAPPED:
+                    self.pools[g].share(page, rc.request_id)
+            if source.length % self.page_size:
+                if g in tails:
+                    mine.blocks.append(self.pools[g].alloc(rc.request_id))
+                    copies.append((g, table.blocks[full], mine.blocks[full]))
+                else:
+                    mine.blocks.append(UNMAPPED)
+        rc.length, rc.reserved, rc.family = source.length, 0, source.family
+        return copies
+
+    def fork(self, source_id: Hashable, request_id: Hashable) -> List[tuple]:
+        """Open request_id as a request that goes on from where source_id stands.  Returns (group, from page, to page) for the
+        pages whose content has to be copied.  Pages and a slot are there, or nothing is changed."""
+        source = self.get(source_id)
+        if source.reserved:
+            raise CacheError("fork during a step")
+        for g in self._tail_copies(source):
+            if self.pools[g].free_pages < 1:
+                raise OutOfPages(f"group {g} has no page for the end of request {request_id!r}")
+        return self._continue(self.open(request_id), source, [0] * len(self.groups))
+
+    def adopt(self, pairs: List[tuple]) -> List[tuple]:
+        """For every (request, source): the request forgets what it holds and goes on from where the source stands.  No request is named
+        twice, or as a source too.  Returns the pages to copy, as fork() does.  Enough pages, or nothing is changed."""
+        requests = [r for r, _ in pairs]
+        if len(set(requests)) != len(requests) or set(requests) & {s for _, s in pairs}:
+            raise CacheError("a request is adopted into twice, or is a source too")
+        rcs = [(self.get(r), self.get(s)) for r, s in pairs]
+        if any(rc.reserved or source.reserved for rc, source in rcs):
+            raise CacheError("adopt during a step")
+        # what a request and its source hold in common already stays where it is
+        kept = [[self._common(rc.tables[g], source.tables[g], source.length // self.page_size) for g in range(len(self.groups))] for rc, source in rcs]
+        for g, pool in enumerate(self.pools):
+            need = sum(1 for _, source in rcs if g in self._tail_copies(source))
+            if need > pool.free_pages:
+                # a page comes back when everybody who holds it is among the requests that let go of it
+                leaving = {}
+                for (rc, _), k in zip(rcs, kept):
+                    for page in rc.tables[g].blocks[k[g]:]:
+                        if page != UNMAPPED:
+                            leaving.setdefault(page, set()).add(rc.request_id)
+                back = sum(1 for page, who in leaving.items() if who.issuperset(pool.holders(page)))
+                if need > pool.free_pages + back:
+                    raise OutOfPages(f"group {g} needs {need} pages and has {pool.free_pages + back}")
+        for (rc, _), k in zip(rcs, kept):
+            for g, table in rc.tables.items():
+                for page in table.blocks[k[g]:]:
+                    if page != UNMAPPED:
+                        self.pools[g].free(page, rc.request_id)
+                del table.blocks[k[g]:]
+        copies = []
+        for (rc, source), k in zip(rcs, kept):
+            copies += self._continue(rc, source, k)
+        return copies
+
+    @staticmethod
+    def _common(a: GroupTable, b: GroupTable, limit: int) -> int:
+        """How many leading blocks two tables have alike, at most `limit`."""
+        n = min(len(a.blocks), len(b.blocks), limit)
+        return next((i for i, (x, y) in enumerate(zip(a.blocks[:n], b.blocks)) if x != y), n)
 
     def get(self, request_id: Hashable) -> RequestCache:
         try:
@@ -238,6 +354,10 @@ class PageTables:
         for g in range(len(self.groups)):
             if self._first_needed_block(g, length) < rc.tables[g].first_held:
                 raise CacheError(f"group {g} has already given back pages that position {length} needs")
+            if length % self.page_size and length < rc.length:
+                page = rc.tables[g].blocks[length // self.page_size]
+                if page != UNMAPPED and self.pools[g].is_shared(page):
+                    raise CacheError(f"position {length} of request {request_id!r} lies inside a page that others hold too")
         rc.length = length
         self._trim(rc, length)
 
@@ -258,7 +378,7 @@ class PageTables:
         return page * self.page_size + pos % self.page_size
 
     def check(self) -> None:
-        """Pool consistency, and every held page is in exactly one table."""
+        """Pool consistency, and every held page is in exactly the tables of those who hold it."""
         for g, pool in enumerate(self.pools):
             pool.check()
             held = {}
@@ -266,10 +386,13 @@ class PageTables:
                 for page in rc.tables[g].blocks:
                     if page == UNMAPPED:
                         continue
-                    if page in held:
-                        raise CacheError(f"page {page} of group {g} is held by {held[page]!r} and {rc.request_id!r}")
-                    if pool.owner(page) != rc.request_id:
+                    if rc.request_id not in pool.holders(page):
+                        if page in held:
+                            raise CacheError(f"page {page} of group {g} is held by {held[page]!r} and {rc.request_id!r}")
                         raise CacheError(f"page {page} of group {g} is in a table but owned by {pool.owner(page)!r}")
-                    held[page] = rc.request_id
+                    held.setdefault(page, []).append(rc.request_id)
+            for page, requests in held.items():
+                if len(requests) != len(pool.holders(page)) or len(set(requests)) != len(requests):
+                    raise CacheError(f"page {page} of group {g} is in the tables of {requests!r} and held by {pool.holders(page)!r}")
             if len(held) + pool.free_pages != pool.num_pages:
                 raise CacheError(f"group {g}: {pool.num_pages - pool.free_pages - len(held)} pages are owned but in no table")

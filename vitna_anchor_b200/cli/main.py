@@ -1,7 +1,7 @@
 """The command line, in the manner of the reference's engine binary (engine/src/main.c:38-141, 211-303).
 
     vitna-anchor generate --model <dir> (--ids a,b,... | --ids-file f) [--max-new n] [--greedy |
-                 --temperature t [--top-k k] [--top-p p] [--seed s]] [--logits-out file] [--timing]
+                 --temperature t [--top-k k] [--top-p p] [--seed s] | --beams n [--length-penalty x]] [--logits-out file] [--timing]
                  [--ctx n] [--parallel n] [--stop-at-special] [--device cuda] [--dtype bfloat16|float32]
                  [--kv-block n] [--num-pages n] [--max-batch-tokens n] [--max-prompt-portion n]
     vitna-anchor logits   --model <dir> (--ids ... | --ids-file f) --out file [--ctx n] [--dtype ...]
@@ -9,7 +9,7 @@
     vitna-anchor info     --model <dir>
 
 generate prints JSON {"prompt_ids": [...], "ids": [...]} (main.c:1118-1124; there is no tokenizer
-here, so no text).  logits writes every prompt position's logits as float32, little-endian,
+here, so no text); with --beams the best of the search's results as "ids" and all of them, best first, as "beams".  logits writes every prompt position's logits as float32, little-endian,
 positions x vocab (main.c:900-937).  An unknown option is an error and the exit code is 1
 (main.c:296-299).
 """
@@ -21,7 +21,7 @@ from typing import List, Optional
 
 VALUE_OPTIONS = {"--model", "--ids", "--ids-file", "--max-new", "--temperature", "--top-k", "--top-p", "--seed", "--logits-out",
                  "--out", "--ctx", "--device", "--dtype", "--parallel", "--kv-block", "--num-pages", "--max-batch-tokens",
-                 "--max-prompt-portion", "--config", "--std", "--norm-noise", "--weights-dtype"}
+                 "--max-prompt-portion", "--beams", "--length-penalty", "--config", "--std", "--norm-noise", "--weights-dtype"}
 FLAG_OPTIONS = {"--greedy", "--timing", "--stop-at-special"}
 COMMANDS = ("generate", "logits", "random-model", "info")
 
@@ -47,10 +47,10 @@ def parse_args(argv: List[str]) -> dict:
         else:
             raise UsageError(f"Unknown or incomplete option: {k}")
     try:
-        for key in ("max_new", "top_k", "seed", "ctx", "parallel", "kv_block", "num_pages", "max_batch_tokens", "max_prompt_portion"):
+        for key in ("max_new", "top_k", "seed", "ctx", "parallel", "kv_block", "num_pages", "max_batch_tokens", "max_prompt_portion", "beams"):
             if key in a:
                 a[key] = int(a[key])
-        for key in ("temperature", "top_p", "std", "norm_noise"):
+        for key in ("temperature", "top_p", "std", "norm_noise", "length_penalty"):
             if key in a:
                 a[key] = float(a[key])
     except ValueError as e:
@@ -88,16 +88,27 @@ def make_engine(a: dict):
                       ("max_batch_tokens", "max_batch_tokens"), ("max_prompt_portion", "max_prompt_portion")):
         if key in a:
             kw[name] = a[key]
-    kw.setdefault("parallel", 1)
+    kw.setdefault("parallel", max(1, min(64, a.get("beams", 1))))
     return Engine(a["model"], dtype=a["dtype"], device=a["device"], **kw)
 
 
 def cmd_generate(a: dict) -> int:
     ids = read_ids(a)
+    if "length_penalty" in a and "beams" not in a:
+        raise UsageError("--length-penalty goes with --beams")
+    if "beams" in a:
+        for key in ("temperature", "top_k", "top_p", "logits_out", "timing"):
+            if a.get(key) not in (None, False, 0, 0.0) and not (key == "top_p" and a[key] == 1.0):
+                raise UsageError(f"--{key.replace('_', '-')} does not go with --beams")
     eng = make_engine(a)
     stop = set()
     if a.get("stop_at_special") and getattr(eng.model.config, "eos_token_id", None) is not None:
         stop.add(eng.model.config.eos_token_id)
+    if "beams" in a:
+        found = eng.beam_search(ids, beams=a["beams"], max_new=a["max_new"], length_penalty=a.get("length_penalty", 1.0), stop_ids=stop)
+        print(json.dumps({"prompt_ids": ids, "ids": found[0].ids if found else [],
+                          "beams": [{"ids": r.ids, "score": r.score, "log_prob": r.log_prob, "finish": r.finish_reason} for r in found]}))
+        return 0
     out = eng.generate(ids, max_new=a["max_new"], temperature=a["temperature"], top_k=a["top_k"], top_p=a["top_p"],
                        seed=a["seed"], stop_ids=stop, logits_out=a.get("logits_out"))
     print(json.dumps({"prompt_ids": ids, "ids": out}))

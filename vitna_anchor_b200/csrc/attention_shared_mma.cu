@@ -104,7 +104,7 @@ __device__ __forceinline__ void sm_walk(const SaArgs& a, const SaPart& part, int
         rows = row_of(n + 3);
         const uint32_t sk = stages + (n % SM_STAGES) * SmSmem<HD>::STAGE, sv = sk + SmSmem<HD>::HALF;
         const int key0 = part.k0 + (tile0 + n * step) * TK;
-#pragma unroll
+#pragma unroll 1                                           // four copies of the body would not stay in the instruction cache
         for (int sub = 0; sub < TK; sub += SUB) {
             if (key0 + sub >= part.k1) break;
             float s[NB][4];

@@ -66,7 +66,7 @@ class ContextBuilder:
         self.max_blocks = -(-max_model_len // self.page_size)
         self.max_segments = max_segments
         n_groups = len(cache.groups)
-        decode_words = 7 * max_segments + 1 + n_groups * (max_segments + max_segments * self.max_blocks)
+        decode_words = 7 * max_segments + 1 + n_groups * (max_segments + max_segments * self.max_blocks + 3 * max_segments + 1)
         self.meta_len = max(meta_words(max_batch_tokens, max_segments, self.max_blocks, n_groups), decode_words) + 8
         self._staging = [_Staging(self.meta_len, True) for _ in range(4)]
         self._turn = 0
@@ -174,16 +174,26 @@ class ContextBuilder:
         return ctx, (dev[s_rows] if R else None)
 
     # -- single tokens, padded to a fixed number of segments -----------------------------------------------
-    def build_decode(self, requests: Sequence[Hashable], tokens: Sequence[int], B: int, views: bool = True, reach: int = 0):
+    def families(self, requests: Sequence[Hashable]) -> Optional[List[List[int]]]:
+        """The requests' places in the batch, family by family (requests that were forked from one another); None where nobody shares."""
+        by_family = {}
+        for i, rid in enumerate(requests):
+            by_family.setdefault(self.cache.tables.get(rid).family, []).append(i)
+        return list(by_family.values()) if len(by_family) < len(requests) else None
+
+    def build_decode(self, requests: Sequence[Hashable], tokens: Sequence[int], B: int, views: bool = True, reach: int = 0,
+                     families: Optional[List[List[int]]] = None):
         """The context of a batch of single tokens, padded to B segments, at offsets that depend on B alone, so
         that a captured graph finds every array where it was at capture.  A padding segment has one token at
-        position 0 that writes nothing (slot mapping -1, state slot -1) and reads page 0.  views=False: only fill the buffer."""
+        position 0 that writes nothing (slot mapping -1, state slot -1) and reads page 0.  views=False: only fill the buffer.
+        families: as families() has them; the page groups without a window then carry what their members share."""
         S, ps, maxb = len(requests), self.page_size, self.max_blocks
         tables = self.cache.tables
         st = self._next_staging()
         buf = st.np
         n_groups = len(self.cache.groups)
-        total = 7 * B + 1 + n_groups * (B + B * maxb)
+        o_families = 7 * B + 1 + n_groups * (B + B * maxb)
+        total = o_families + (n_groups * (3 * B + 1) if families else 0)
         if total > self.meta_len:
             raise MetaOverflow(f"a decode batch of {B} needs more than the {self.meta_len} words of the metadata buffer")
         buf[:total] = 0
@@ -213,6 +223,19 @@ class ContextBuilder:
                 buf[o_sm + i] = row[first[i] // ps] * ps + first[i] % ps
                 np.maximum(row, 0, out=row)
                 bt[i, :len(row)] = row
+            if families:
+                o = o_families + g * (3 * B + 1)
+                order = [i for f in families for i in f] + list(range(S, B))
+                sizes = [len(f) for f in families] + [1] * (B - S)
+                buf[o:o + B] = order
+                buf[o + B + 1:o + B + 1 + len(sizes)] = np.cumsum(sizes)
+                buf[o + B + 1 + len(sizes):o + 2 * B + 1] = B
+                if self.cache.groups[g].window == 0:
+                    for k, f in enumerate(families):
+                        if len(f) > 1:
+                            n = min(len(rcs[i].tables[g].blocks) for i in f)
+                            apart = (bt[f[1:], :n] != bt[f[0], :n]).any(0)
+                            buf[o + 2 * B + 1 + k] = (int(apart.argmax()) if apart.any() else n) * ps
         self._send(st, total)
         if not views:               # a replay needs the arrays in place, not their description
             return None, None
@@ -220,7 +243,11 @@ class ContextBuilder:
         groups = []
         for g in range(n_groups):
             o_sm = o_groups + g * (B + B * maxb)
-            groups.append(GroupMeta(dev[o_sm:o_sm + B], dev[o_sm + B:o_sm + B + B * maxb].view(B, maxb), maxb))
+            meta = GroupMeta(dev[o_sm:o_sm + B], dev[o_sm + B:o_sm + B + B * maxb].view(B, maxb), maxb)
+            if families and self.cache.groups[g].window == 0:
+                o = o_families + g * (3 * B + 1)
+                meta.members, meta.starts, meta.shared = dev[o:o + B], dev[o + B:o + 2 * B + 1], dev[o + 2 * B + 1:o + 3 * B + 1]
+            groups.append(meta)
         ctx = StepContext(
             num_tokens=B, num_segments=B, dtype=self.dtype, tokens=dev[o_tok:o_tok + B], positions=dev[o_pos:o_pos + B],
             token_seg=dev[o_seg:o_seg + B], seg_starts=dev[o_starts:o_starts + B + 1], seg_context=dev[o_ctx:o_ctx + B],

@@ -11,14 +11,17 @@ engine/src/api.c:48-49, 2216-2224).
 """
 from __future__ import annotations
 
+import math
 import time
 from typing import Dict, Hashable, Iterable, List, Optional, Sequence, Union
 
 import numpy as np
 import torch
 
+from .. import ops
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler
+from .beam import BeamResult, BeamSelector, beam_search
 from .loading import load_model
 from .runner import DeviceStepFailed, ModelRunner, StepEntry, StepFailed
 from .scheduler import PENDING, Planned, Request, RequestRefused, Scheduler  # noqa: F401
@@ -54,6 +57,7 @@ class Engine:
         self._inflight = None            # (requests, index of the pending token in each request's output, host ids, event)
         self._ids_host = [torch.empty(parallel, dtype=torch.int32).pin_memory() for _ in range(2)]
         self._ids_turn = 0
+        self._selectors: Dict[int, BeamSelector] = {}
         self._held: List[Request] = []   # finished, but their last token has not arrived yet
 
     # -- requests -----------------------------------------------------------------------------
@@ -231,6 +235,38 @@ class Engine:
                 raise StepFailed(f"a step of request {r.request_id!r} failed after {len(r.output)} new tokens")
         outs = [list(r.output) for r in reqs]
         return outs[0] if single else outs
+
+    def beam_search(self, ids: Sequence[int], *, beams: int = 4, max_new: int = 64, length_penalty: float = 1.0,
+                    stop_ids: Iterable[int] = ()) -> List[BeamResult]:
+        """The `beams` best continuations of one prompt, best first (engine/beam.py says what is best and when the search ends; fewer where
+        the vocabulary or the stop ids leave fewer).  The beams take `beams` of the engine's request slots and run by themselves: while requests that were
+        added are not finished the search is refused."""
+        ids = [int(t) for t in ids]
+        if not ids:
+            raise RequestRefused("the prompt is empty")
+        for t in ids:
+            if not (0 <= t < self.model.vocab_size):
+                raise RequestRefused(f"token id {t} is outside the vocabulary of {self.model.vocab_size}")
+        most = min(self.runner.cache.max_requests, ops.BEAM_MAX_BEAMS)
+        if not (1 <= beams <= most):
+            raise RequestRefused(f"beams is between 1 and {most} (the engine's parallel requests)")
+        if max_new < 1:
+            raise RequestRefused("max_new must be at least 1")
+        if len(ids) + max_new > self.ctx:
+            raise RequestRefused(f"the prompt ({len(ids)} tokens) and max_new ({max_new}) do not fit the context of {self.ctx} positions")
+        if self.model.vocab_size > ops.BEAM_MAX_VOCAB:
+            raise RequestRefused(f"a vocabulary of {self.model.vocab_size} is more than the {ops.BEAM_MAX_VOCAB} that the choice takes")
+        if not math.isfinite(length_penalty):
+            raise RequestRefused("length_penalty is a number")
+        if self.scheduler.has_work() or self._inflight is not None:
+            raise RequestRefused("requests are running; a beam search has the engine to itself")
+        selector = self._selectors.get(beams)
+        if selector is None:
+            selector = self._selectors[beams] = BeamSelector(self.model.vocab_size, beams, "cuda")
+        name = ("beam", self._next_id)
+        self._next_id += 1
+        return beam_search(self.runner, selector, ids, beams=beams, max_new=max_new, length_penalty=float(length_penalty),
+                           stop_ids=[int(t) for t in stop_ids], name=name)
 
     def logits(self, ids: Sequence[int], piece: int = 256) -> torch.Tensor:
         """float32 logits [positions, vocab] of every position of one prompt, run in pieces of `piece` tokens

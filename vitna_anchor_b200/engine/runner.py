@@ -103,7 +103,7 @@ class ModelRunner:
         # A model is run from captured graphs only if every part of it says that a capture replays it faithfully.
         self.cuda_graphs = bool(cuda_graphs) and model.capture_safe
         self._chunk_rules = list(getattr(model, "chunk_rules", ()))      # the parts' launches also depend on what these say of a step
-        self._decode_graphs: "OrderedDict[tuple, tuple]" = OrderedDict()    # (batch bucket, context bucket) -> (graph, kernels)
+        self._decode_graphs: "OrderedDict[tuple, tuple]" = OrderedDict()    # (batch bucket, context bucket, families) -> (graph, kernels)
         self._mixed_graphs: Dict[tuple, tuple] = {}                          # the counts of a mixed step -> (graph, logits, kernels)
         self._seen_shapes: Dict[tuple, int] = {}
         self.graph_mixed_steps = True            # steps with prompt portions are captured too, once their counts repeat
@@ -121,6 +121,10 @@ class ModelRunner:
 
     def close(self, request_id: Hashable) -> None:
         self.cache.close(request_id)
+
+    def fork(self, source_id: Hashable, request_id: Hashable) -> int:
+        """Open a request that goes on from where another stands (CacheManager.fork)."""
+        return self.cache.fork(source_id, request_id)
 
     def length(self, request_id: Hashable) -> int:
         return self.cache.length(request_id)
@@ -321,10 +325,13 @@ class ModelRunner:
         # bucket runs eagerly and is then captured (a stall of about two steps, once per bucket).
         longest = max(self.cache.tables.get(e.request_id).length for e in entries) + 1
         reach = self.context_bucket(longest, self.max_model_len)
-        key = (B, reach)
+        # Requests that hold pages in common (and are not alone in their family) take the attention that reads those once: a graph of its own.
+        requests = [e.request_id for e in entries]
+        families = self.builder.families(requests)
+        key = (B, reach, families is not None)
         held = self._decode_graphs.get(key)
-        ctx, rows = self.builder.build_decode([e.request_id for e in entries], [e.tokens[0] for e in entries], B,
-                                              views=held is None, reach=reach)
+        ctx, rows = self.builder.build_decode(requests, [e.tokens[0] for e in entries], B, views=held is None, reach=reach,
+                                              families=families)
         if token_source is not None:
             ids, src = token_source
             if self._src_dev is None:

@@ -54,10 +54,14 @@ class Workspace:
 
 @dataclass
 class GroupMeta:
-    """Per page group: where each token's keys and values go, and each segment's block table."""
+    """Per page group: where each token's keys and values go, and each segment's block table; in a batch of single tokens some of whose requests hold
+    pages in common also the families (None elsewhere): family f is the tokens members[starts[f]:starts[f+1]], whose tables agree on the first shared[f] positions."""
     slot_mapping: torch.Tensor      # int32 [T]: page * page_size + offset
     block_tables: torch.Tensor      # int32 [S, max_blocks]
     max_blocks: int
+    members: Optional[torch.Tensor] = None      # int32 [T]
+    starts: Optional[torch.Tensor] = None       # int32 [T + 1], empty families behind the last
+    shared: Optional[torch.Tensor] = None       # int32 [T]
 
 
 class ChunkRule(NamedTuple):
