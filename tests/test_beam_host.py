@@ -190,22 +190,22 @@ def test_entries_refuse_before_anything_runs():
     """The C entries say no to sizes they do not take; nothing is launched, so no device is needed."""
     lib, null = ops.lib(), ctypes.c_void_p(0)
     some = ctypes.c_void_p(64)
-    LL = ctypes.c_longlong
+    LL, SIZE = ctypes.c_longlong, ctypes.c_size_t
 
-    def attention(n=4, families=1, nh=4, nkv=2, hd=64, ps=16, maxb=8, dtype=1, scratch=some):
-        return lib.vk_attention_shared(some, some, some, some, some, some, some, some, some, scratch, 4, 4, n, families, 10, nh, nkv, hd, ps, maxb, ctypes.c_float(0.1), dtype, null)
+    def attention(n=4, families=1, nh=4, nkv=2, hd=64, ps=16, maxb=8, dtype=1, scratch=some, room=1 << 40):
+        return lib.vk_attention_shared(some, some, some, some, some, some, some, some, some, scratch, SIZE(room), 4, 4, n, families, 10, nh, nkv, hd, ps, maxb, ctypes.c_float(0.1), dtype, null)
 
     assert attention(n=0) == 0 and attention(families=0) == 0
     for kw in [dict(n=257), dict(families=257), dict(hd=264), dict(nkv=129, nh=129), dict(hd=12), dict(nh=5), dict(nh=130), dict(ps=0), dict(maxb=0), dict(maxb=1 << 28),
-               dict(hd=6, dtype=0), dict(scratch=ctypes.c_void_p(72))]:
+               dict(hd=6, dtype=0), dict(scratch=ctypes.c_void_p(72)), dict(room=1 << 20)]:
         assert attention(**kw) < 0, kw
 
-    def select(rows=8, beams=4, vocab=100, ld=100, keep=8, scratch=some):
-        return lib.vk_beam_select(some, some, some, some, some, scratch, rows, beams, vocab, LL(ld), keep, null)
+    def select(rows=8, beams=4, vocab=100, ld=100, keep=8, scratch=some, room=1 << 40):
+        return lib.vk_beam_select(some, some, some, some, some, scratch, SIZE(room), rows, beams, vocab, LL(ld), keep, null)
 
     assert select(rows=0) == 0
     for kw in [dict(beams=3), dict(beams=0), dict(keep=0), dict(keep=129), dict(vocab=0), dict(ld=99), dict(beams=1, keep=101), dict(rows=1028), dict(rows=130, beams=65),
-               dict(vocab=64 * 4096 + 1, ld=1 << 20), dict(scratch=null), dict(scratch=ctypes.c_void_p(8))]:
+               dict(vocab=64 * 4096 + 1, ld=1 << 20), dict(scratch=null), dict(scratch=ctypes.c_void_p(8)), dict(room=4600)]:
         assert select(**kw) < 0, kw
 
     def copy(rows=4, src=(0,), dst=(1,), stride=16, size=16, layers=1):

@@ -11,6 +11,8 @@
 // attention_shared_mma.cu has bfloat16 heads of 64 and 128 on the tensor cores.
 #include "attention_shared_plan.cuh"
 
+#include <atomic>
+
 namespace vk {
 
 constexpr int SG_KEYS = 32, SG_PREFIX_ROWS = 64, SG_ROWS = SG_PREFIX_ROWS / (SA_THREADS / 32);      // rows a block, rows a warp
@@ -254,9 +256,14 @@ static int launch_join(const SaArgs& a, int dtype, cudaStream_t stream) {
 #undef GO
 }
 
+// The current device's multiprocessors, asked for once a device.
 static int sa_multiprocessors() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
@@ -275,7 +282,7 @@ VK_API size_t vk_attention_shared_scratch_bytes(int tokens, int nh, int, int hd)
 
 // dtype 0 = float32, 1 = bfloat16.  scratch: vk_attention_shared_scratch_bytes(n, ...) bytes, whatever they hold.
 VK_API int vk_attention_shared(const void* q, const void* cache, const int32_t* block_tables, const int32_t* token_seg, const int32_t* positions,
-                               const int32_t* members, const int32_t* starts, const int32_t* shared, void* out, void* scratch, int tokens, int segments,
+                               const int32_t* members, const int32_t* starts, const int32_t* shared, void* out, void* scratch, size_t scratch_bytes, int tokens, int segments,
                                int n, int families, int pages, int nh, int nkv, int hd, int page_size, int max_blocks, float scale, int dtype,
                                cudaStream_t stream) {
     if (n <= 0 || families <= 0) return VK_OK;
@@ -287,6 +294,7 @@ VK_API int vk_attention_shared(const void* q, const void* cache, const int32_t* 
     const long long tiles = (long long)max_blocks * page_size / SA_TILE + 64, units = (long long)n * nh;
     if (tiles * units > 0x7fffffffLL || units * 4 * hd > 0x7fffffffLL) return VK_TOO_LARGE;
     if (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)out | (uintptr_t)scratch) % 16) return VK_BAD_ALIGNMENT;
+    if (scratch_bytes < vk_attention_shared_scratch_bytes(n, nh, nkv, hd)) return VK_SMALL_SCRATCH;
     const int sms = sa_multiprocessors();
     if (sms > SA_MAX_MULTIPROCESSORS) return VK_TOO_LARGE;
     SaArgs a;
@@ -313,8 +321,8 @@ VK_API int vk_attention_shared(const void* q, const void* cache, const int32_t* 
 #define GO(T, DIMS)                                                                                                                     \
     do {                                                                                                                                \
         auto kern = attention_shared_kernel<T, DIMS>;                                                                                   \
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                             \
-        if (e != cudaSuccess) return (int)e;                                                                                            \
+        const int e = sa_allow_smem(kern, smem);                                                                                        \
+        if (e != VK_OK) return e;                                                                                                       \
         const int status = launch_dependent(kern, dim3(sms), dim3(SA_THREADS), smem, stream, a);                                        \
         return status != VK_OK ? status : launch_join(a, dtype, stream);                                                                \
     } while (0)

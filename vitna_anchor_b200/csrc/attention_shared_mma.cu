@@ -322,8 +322,8 @@ int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stre
 #define GO(HD)                                                                                                                                  \
     do {                                                                                                                                        \
         auto kern = attention_shared_mma_kernel<HD>;                                                                                            \
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SmSmem<HD>::BYTES);                        \
-        if (e != cudaSuccess) return (int)e;                                                                                                    \
+        const int e = sa_allow_smem(kern, SmSmem<HD>::BYTES);                                                                                   \
+        if (e != VK_OK) return e;                                                                                                               \
         return launch_dependent(kern, dim3(blocks), dim3(SA_THREADS), SmSmem<HD>::BYTES, stream, a);                                            \
     } while (0)
     if (a.hd == 64) GO(64);

@@ -254,6 +254,24 @@ __device__ __forceinline__ float sa_ex2(float x) {
 
 constexpr int SA_MAX_MULTIPROCESSORS = 160;         // of the sm_100a parts; the scratch is laid out for this many
 
+// Allows a kernel more than 48 KB of shared memory on the current device, asked for again only where a launch needs more than was allowed before.
+template <typename... Args> inline int sa_allow_smem(void (*kernel)(Args...), size_t bytes) {
+    struct Allowed { void (*kernel)(Args...); int device; size_t bytes; };
+    static thread_local Allowed known[8];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    Allowed* slot = nullptr;
+    for (Allowed& k : known) {
+        if (k.kernel == kernel && k.device == dev) { slot = &k; break; }
+        if (!slot && !k.kernel) slot = &k;
+    }
+    if (slot && slot->kernel == kernel && slot->bytes >= bytes) return VK_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && slot) *slot = Allowed{kernel, dev, bytes};
+    return (int)e;
+}
+
 // attention_shared_mma.cu
 bool attention_shared_mma_takes(const SaArgs& a, int dtype);
 int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream);

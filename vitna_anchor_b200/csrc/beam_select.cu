@@ -5,21 +5,23 @@
 // the `keep` largest in descending order, the lowest (beam, token) first among equals.  A row that has no softmax (a NaN, an infinite maximum, nothing
 // above -inf) or whose score is not finite offers its tokens at -inf, in their order.
 //
-// One launch, one read of the logits.  A block holds 4,096 or 8,192 values of a row in registers (float32, as the logits come) and leaves the values'
-// maximum, their sum of exponentials against it and their `keep` best in order: within a row c and x have the same order, so neither needs the row's sum.
-// The block that completes a request joins the sums in float64 and merges its lists; c is computed there, in float64, for the few values that are left,
-// so that two beams' candidates are told apart where float32 sums would tie.  Where the lists are long together, the block that completes a row
-// merges that row's lists first.
+// One launch, one read of the logits.  A block walks a stretch of a row, 4,096 values at a time in registers (float32, as the logits come) with the next ones on their way, and leaves
+// the values' maximum, their sum of exponentials against it and their `keep` best in order: within a row c and x have the same order, so neither needs the row's sum.
+// The block that completes a request joins the sums and merges its lists; c is computed there, in float64, for the few values that are left, so that two
+// beams' candidates are told apart where float32 sums would tie.
 //
 // Choosing `keep` of many, without sorting them: the block's threads make 32 to 256 groups, at least twice as many as are kept; the keep-th largest of the groups'
 // best is a bound that at least `keep` values reach and few others do (17 values of 4,096 normal ones above the bound for keep = 8, 150 for 64).  Those are put in a list
-// in shared memory and each counts how many of the list are larger: its place.  Where too many reach the bound (values laid out against the groups) it is raised bit by bit
-// to the keep-th largest itself.
+// in shared memory and each counts how many of the list are larger: its place.  The merge does the same with the lists' first entries, and goes on down a list whose last
+// one of those still reaches the bound.  Where too many reach the bound (many equal values, values laid out against the groups) the choice is made by value and token together, and at last the bound
+// raised bit by bit to the keep-th largest itself.
 #include "common.cuh"
+
+#include <cuda_fp16.h>
 
 namespace vk {
 
-constexpr int BS_THREADS = 256, BS_MAX_KEEP = 128, BS_MAX_BEAMS = 64, BS_LIST = 1024, BS_MAX_PARTS = 64, BS_MAX_ROWS = 1024;
+constexpr int BS_THREADS = 256, BS_VALUES = 16, BS_MAX_KEEP = 128, BS_MAX_BEAMS = 64, BS_LIST = 1024, BS_MAX_PARTS = 64, BS_MAX_ROWS = 1024, BS_HELD = 2048;
 
 typedef unsigned long long u64;
 
@@ -64,18 +66,21 @@ template <typename K> struct BsPick {
     int count;
 };
 
+__device__ __forceinline__ int bs_lanes(int keep) { return keep <= 16 ? 8 : keep <= 32 ? 4 : keep <= 64 ? 2 : 1; }
+
 // The `keep` largest of the block's candidates into out[0 .. keep), in descending order, none where there are fewer.  each(f) calls f(candidate) for every
-// candidate of this thread.  out is shared memory.  Every thread of the block calls it.
+// candidate of this thread.  out is shared memory.  Every thread of the block calls it.  The way for candidates that the quick ones do not tell apart: by all of a candidate.
 template <typename K, typename Each>
-__device__ __forceinline__ void bs_pick(BsPick<K>& s, int keep, K* out, const Each& each) {
+__device__ __noinline__ void bs_pick(BsPick<K>& s, int keep, K* out, const Each& each) {
     const int tid = threadIdx.x, lane = tid & 31;
     K best = bs_none<K>();
     each([&](const K& c) { if (bs_above(c, best)) best = c; });
-    const int lanes = keep <= 16 ? 8 : keep <= 32 ? 4 : keep <= 64 ? 2 : 1, groups = BS_THREADS / lanes;
+    const int lanes = bs_lanes(keep), groups = BS_THREADS / lanes;
     for (int o = 1; o < lanes; o <<= 1) {
         const K other = bs_shfl_xor(best, o);
         if (bs_above(other, best)) best = other;
     }
+    __syncthreads();
     if (lane % lanes == 0) s.group[tid / lanes] = best;
     if (tid == 0) { s.bound = bs_none<K>(); s.count = 0; }
     for (int i = tid; i < keep; i += BS_THREADS) out[i] = bs_none<K>();
@@ -83,7 +88,6 @@ __device__ __forceinline__ void bs_pick(BsPick<K>& s, int keep, K* out, const Ea
     if (tid < groups) {
         const K mine = s.group[tid];
         int above = 0;
-#pragma unroll 8
         for (int i = 0; i < groups; i++) above += bs_above(s.group[i], mine);
         if (above == keep - 1 && !bs_is_none(mine)) s.bound = mine;          // groups' best are different candidates
     }
@@ -122,7 +126,6 @@ __device__ __forceinline__ void bs_pick(BsPick<K>& s, int keep, K* out, const Ea
     for (int i = tid; i < n; i += BS_THREADS) {
         const K mine = s.list[i];
         int above = 0;
-#pragma unroll 8
         for (int j = 0; j < n; j++) above += bs_above(s.list[j], mine);
         if (above < keep) out[above] = mine;
     }
@@ -135,157 +138,385 @@ struct BsArgs {
     float* out_score;         // [requests][keep]
     int32_t* out_parent;
     int32_t* out_token;
-    int* arrived;             // [BS_MAX_ROWS] of the rows and, behind them, as many of the requests: zero between launches
+    int* arrived;             // [requests]: zero between launches
     float2* sums;             // [rows][parts] maximum and sum of exponentials
     u64* lists;               // [rows][parts][keep]
-    u64* row_lists;           // [rows][keep], where a row's lists are merged first
     long long ld;
-    int beams, vocab, keep, parts, merge_rows;
+    int beams, vocab, keep, parts, stretch;
 };
 
-template <int VALUES>
-__global__ void __launch_bounds__(BS_THREADS) beam_select_kernel(const BsArgs a) {
-    __shared__ union { BsPick<u64> one; BsPick<BsPair> two; } pick;
+__device__ __forceinline__ float bs_exp(float x) {           // relative error 2^-22 and 2^-24 |x|
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
+// Maximum and sum of the warp's lanes: one exponential a lane.
+__device__ __forceinline__ void bs_join_warp(float& m, float& s) {
+    const float top = bs_value(__reduce_max_sync(0xffffffffu, bs_order(m))), r = top == -INFINITY ? 0.0f : top;
+    s = warp_sum(s * bs_exp(m - r));
+    m = top;
+}
+
+// (m, s) and (om, os) together: maximum, and sum of exponentials against it.  Of nothing above -inf the sum is 0; a NaN stays one.
+__device__ __forceinline__ void bs_join(float& m, float& s, float om, float os) {
+    const float both = fmaxf(m, om), r = both == -INFINITY ? 0.0f : both;
+    s = s * bs_exp(m - r) + os * bs_exp(om - r);
+    m = both;
+}
+
+// The bound: the largest number that at least `keep` of the block's 256 threads reach together with their neighbours, from the groups of threads' largest values rounded down to 11 bits (a
+// bound may be lower, and two of those are compared in an instruction).  -inf where there is none.  group: BS_THREADS halves; bound: an ordered number, 0 before.  Two barriers.
+__device__ __forceinline__ float bs_bound(float best, int lanes, int keep, __half* group, uint32_t* bound) {
+    const int tid = threadIdx.x, lane = tid & 31, groups = BS_THREADS / lanes;
+    for (int o = 1; o < lanes; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane % lanes == 0) group[tid / lanes] = __float2half_rd(best);
+    __syncthreads();
+    if (tid < groups) {
+        const __half mine = group[tid];
+        const __half2 pair = __half2half2(mine);
+        __half2 reach = __float2half2_rn(0.0f);
+#pragma unroll 2
+        for (int i = 0; i < groups; i += 8) {
+            const uint4 g = *reinterpret_cast<const uint4*>(group + i);
+            reach = __hadd2(reach, __hadd2(__hadd2(__hge2(*reinterpret_cast<const __half2*>(&g.x), pair), __hge2(*reinterpret_cast<const __half2*>(&g.y), pair)),
+                                           __hadd2(__hge2(*reinterpret_cast<const __half2*>(&g.z), pair), __hge2(*reinterpret_cast<const __half2*>(&g.w), pair))));
+        }
+        const uint32_t can = __low2float(reach) + __high2float(reach) >= (float)keep ? bs_order(__half2float(mine)) : 0u;
+        const uint32_t most = __reduce_max_sync(0xffffffffu, can);
+        if (lane == 0) atomicMax(bound, most);
+    }
+    __syncthreads();
+    return *bound ? bs_value(*bound) : -INFINITY;
+}
+
+__global__ void __launch_bounds__(BS_THREADS, 4) beam_select_kernel(const BsArgs a) {
+    __shared__ union {
+        struct {                                       // this block's values that reach the bound, and their tokens
+            float value[BS_LIST + 4];
+            int token[BS_LIST];
+        } part;
+        struct {                                       // the request's entries, and those of them that reach the bound
+            u64 entry[BS_HELD];
+            uint32_t place[BS_HELD];
+            u64 value[BS_LIST];
+            uint32_t flat[BS_LIST];
+        } merge;
+        BsPick<u64> one;
+        BsPick<BsPair> two;
+    } sm;
     __shared__ union { u64 one[BS_MAX_KEEP]; BsPair two[BS_MAX_KEEP]; } top;
     __shared__ double base[BS_MAX_BEAMS];
+    __shared__ __align__(16) __half group[BS_THREADS];
     __shared__ float2 warp_sums[BS_THREADS / 32];
-    __shared__ int done;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = blockIdx.x, row = blockIdx.y;
+    __shared__ uint32_t bound_s;
+    __shared__ int taken[BS_MAX_KEEP], count, done;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = blockIdx.x, row = blockIdx.y, keep = a.keep;
+    if (tid == 0) { bound_s = 0; count = 0; }
+    if (tid < keep) { taken[tid] = 0; top.one[tid] = 0; }
     dependency_wait();
+    let_dependents_start();
 
     // ---- this block's values: thread t has four neighbours of every 1,024 (wherever the row begins, so that equal rows have equal sums)
     const float* x = a.logits + (size_t)row * a.ld;
     const bool aligned = (uintptr_t)x % 16 == 0;
-    const int first = part * (BS_THREADS * VALUES) + tid * 4;
-    float v[VALUES];
+    const int from = part * a.stretch, to = min(a.vocab, from + a.stretch), lanes = bs_lanes(keep);
+    float v[BS_VALUES], next[BS_VALUES];
+    auto load = [&](int first) {
 #pragma unroll
-    for (int j = 0; j < VALUES / 4; j++) {
-        const int i = first + j * BS_THREADS * 4;
-        if (aligned && i + 3 < a.vocab) {
-            const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
-            v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
-        } else {
+        for (int j = 0; j < BS_VALUES / 4; j++) {
+            const int i = first + (j * BS_THREADS + tid) * 4;
+            if (aligned && i + 3 < to) {
+                const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
+                next[4 * j] = f.x; next[4 * j + 1] = f.y; next[4 * j + 2] = f.z; next[4 * j + 3] = f.w;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[4 * j + e] = i + e < a.vocab ? x[i + e] : -INFINITY;
+                for (int e = 0; e < 4; e++) next[4 * j + e] = i + e < to ? x[i + e] : -INFINITY;
+            }
         }
-    }
-    float m = -INFINITY, s = 0.0f;
-#pragma unroll
-    for (int j = 0; j < VALUES; j++) m = fmaxf(m, v[j]);
-    const float ref = m == -INFINITY ? 0.0f : m;              // -inf - 0: nothing; a NaN stays one
-#pragma unroll
-    for (int j = 0; j < VALUES; j++) s += expf(v[j] - ref);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, s, o), both = fmaxf(m, om), r = both == -INFINITY ? 0.0f : both;
-        s = s * expf(m - r) + os * expf(om - r);
-        m = both;
-    }
-    if (lane == 0) warp_sums[warp] = make_float2(m, s);
-    bs_pick(pick.one, a.keep, top.one, [&](auto&& take) {
-#pragma unroll
-        for (int j = 0; j < VALUES; j++) {
-            const int i = first + j / 4 * BS_THREADS * 4 + j % 4;
-            if (i < a.vocab) take(bs_pack(v[j], (uint32_t)i));
-        }
-    });
-    if (tid == 0) {
-        for (int w = 0; w < BS_THREADS / 32; w++) {
-            const float2 o = warp_sums[w];
-            const float both = w ? fmaxf(m, o.x) : o.x, r = both == -INFINITY ? 0.0f : both;
-            s = (w ? s * expf(m - r) : 0.0f) + o.y * expf(o.x - r);
-            m = both;
-        }
-        a.sums[(size_t)row * a.parts + part] = make_float2(m, s);
-    }
-    for (int i = tid; i < a.keep; i += BS_THREADS) a.lists[((size_t)row * a.parts + part) * a.keep + i] = top.one[i];
-
-    // ---- the block that completes the row merges its lists, where they are merged row by row
-    const int request = row / a.beams;
-    const u64* lists = a.lists;
-    int per_row = a.parts;
-    auto count = [&](int* counter, int want) {
-        __syncthreads();
-        if (tid == 0) {
-            int old;
-            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
-            done = old == want - 1;
-            if (done) *counter = 0;                           // ready for the next launch
-        }
-        __syncthreads();
-        return done != 0;
     };
-    if (a.merge_rows) {
-        if (!count(a.arrived + row, a.parts)) return;
-        const u64* mine = a.lists + (size_t)row * a.parts * a.keep;
-        // rank by rank over the parts: the groups' best are then the parts' first ones
-        bs_pick(pick.one, a.keep, top.one, [&](auto&& take) {
-            for (int e = tid; e < a.parts * a.keep; e += BS_THREADS) take(__ldcg(mine + (size_t)(e % a.parts) * a.keep + e / a.parts));
-        });
-        for (int i = tid; i < a.keep; i += BS_THREADS) a.row_lists[(size_t)row * a.keep + i] = top.one[i];
-        if (!count(a.arrived + BS_MAX_ROWS + request, a.beams)) return;
-        lists = a.row_lists;
-        per_row = 1;
-    } else if (!count(a.arrived + BS_MAX_ROWS + request, a.beams * a.parts)) {
-        return;
+    load(from);
+    float m = -INFINITY, s = 0.0f;
+    int round = 0, refresh = 1;
+    float bound = -INFINITY;
+#pragma unroll 1
+    for (int at = from; at < to; at += BS_THREADS * BS_VALUES, round++) {
+#pragma unroll
+        for (int j = 0; j < BS_VALUES; j++) v[j] = next[j];
+        if (at + BS_THREADS * BS_VALUES < to) load(at + BS_THREADS * BS_VALUES);
+        float here = v[0];
+#pragma unroll
+        for (int j = 1; j < BS_VALUES; j++) here = fmaxf(here, v[j]);
+        // the sum of exponentials: of nothing above -inf nothing; a NaN stays one
+        const float more = fmaxf(m, here), ref = more == -INFINITY ? 0.0f : more;
+        s *= bs_exp(m - ref);
+        m = more;
+#pragma unroll
+        for (int j = 0; j < BS_VALUES; j++) s += bs_exp(v[j] - ref);
+        // the values that reach the bound of what has been seen so far, which is taken anew after 1, 2, 4 ... rounds (and as long as there is none)
+        if (round + 1 == refresh || bound == -INFINITY) {
+            bound = bs_bound(m, lanes, keep, group, &bound_s);
+            refresh = 2 * (round + 1);
+        }
+        if (__any_sync(0xffffffffu, here >= bound && here > -INFINITY)) {
+            const float least = fmaxf(bound, -3.402823466e38f);            // -inf comes in behind, if at all
+            uint32_t hits = 0;
+#pragma unroll
+            for (int j = 0; j < BS_VALUES; j++) hits |= v[j] >= least ? 1u << j : 0u;
+            int place = hits ? atomicAdd(&count, __popc(hits)) : 0;
+#pragma unroll
+            for (int j = 0; j < BS_VALUES; j++)
+                if (hits >> j & 1) {
+                    if (place < BS_LIST) sm.part.token[place] = at + j / 4 * (BS_THREADS * 4) + tid * 4 + j % 4;
+                    place++;
+                }
+        }
     }
-
-    // ---- the block that completes the request: the rows' sums, then the best of the rows' lists
-    for (int b = warp; b < a.beams; b += BS_THREADS / 32) {
-        const float2* ms = a.sums + ((size_t)request * a.beams + b) * a.parts;
-        float rm = -INFINITY;
-        for (int i = lane; i < a.parts; i += 32) rm = fmaxf(rm, __ldcg(ms + i).x);
-        rm = warp_max(rm);
-        double sum = 0.0;
-        for (int i = lane; i < a.parts; i += 32) {
-            const float2 o = __ldcg(ms + i);
-            sum += o.x == rm ? (double)o.y : (double)o.y * exp((double)o.x - (double)rm);      // a part without a value above -inf has the sum 0, or NaN
+    bs_join_warp(m, s);
+    if (lane == 0) warp_sums[warp] = make_float2(m, s);
+    __syncthreads();
+    int n = count;
+    if (warp == 0) {
+        const float2 o = lane < BS_THREADS / 32 ? warp_sums[lane] : make_float2(-INFINITY, 0.0f);
+        m = o.x;
+        s = o.y;
+        bs_join_warp(m, s);
+        if (lane == 0) a.sums[(size_t)row * a.parts + part] = make_float2(m, s);
+    }
+    for (int i = tid; i < min(n, BS_LIST); i += BS_THREADS) sm.part.value[i] = x[sm.part.token[i]];
+    if (n < keep && warp == 1) {
+        // everything above -inf is in the list: behind it come the first tokens that are -inf
+        int have = n;
+        for (int i = from + lane; have < keep && i - lane < to; i += 32) {
+            const bool none = i < to && x[i] == -INFINITY;
+            const uint32_t all = __ballot_sync(0xffffffffu, none);
+            const int place = have + __popc(all & ((1u << lane) - 1));
+            if (none && place < keep) { sm.part.value[place] = -INFINITY; sm.part.token[place] = i; }
+            have += __popc(all);
         }
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) {
-            const double score = (double)a.scores[request * a.beams + b], lse = (double)rm + log(sum);
-            base[b] = isfinite(score) && isfinite(lse) ? score - lse : (double)-INFINITY;
-        }
+        if (lane == 0) done = min(have, keep);
     }
     __syncthreads();
-    const int n_lists = a.beams * per_row;
-    const u64* mine = lists + (size_t)request * n_lists * a.keep;
-    bs_pick(pick.two, a.keep, top.two, [&](auto&& take) {
-        for (int e = tid; e < n_lists * a.keep; e += BS_THREADS) {
-            const int l = e % n_lists, rank = e / n_lists, b = l / per_row;
-            const u64 c = __ldcg(mine + (size_t)l * a.keep + rank);
-            uint32_t token = 0xffffffffu - (uint32_t)c;
-            double value = base[b] + (double)bs_value((uint32_t)(c >> 32));
-            bool there = c != 0;
-            if (base[b] == (double)-INFINITY) {                  // its tokens in their order, once a row
-                token = (uint32_t)rank;
-                value = (double)-INFINITY;
-                there = l == b * per_row && rank < a.vocab;
+    if (n < keep) n = done;
+    if (n <= BS_LIST && n > 2 * keep && n > 64) {
+        // a second bound, of the list itself: the first let through what reached the bounds of the values before
+        float best = -INFINITY;
+        for (int i = tid; i < n; i += BS_THREADS) best = fmaxf(best, sm.part.value[i]);
+        const float bound = bs_bound(best, 1, keep, group, &bound_s);
+        float kept_value[BS_LIST / BS_THREADS];
+        int kept_token[BS_LIST / BS_THREADS];
+#pragma unroll
+        for (int j = 0; j < BS_LIST / BS_THREADS; j++)
+            if (tid + j * BS_THREADS < n) { kept_value[j] = sm.part.value[tid + j * BS_THREADS]; kept_token[j] = sm.part.token[tid + j * BS_THREADS]; }
+        if (tid == 0) count = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < BS_LIST / BS_THREADS; j++)
+            if (tid + j * BS_THREADS < n && kept_value[j] >= bound) {
+                const int place = atomicAdd(&count, 1);
+                sm.part.value[place] = kept_value[j];
+                sm.part.token[place] = kept_token[j];
             }
-            if (there) take(BsPair{bs_order64(value), 0xffffffffu - ((uint32_t)b * (uint32_t)a.vocab + token)});
+        __syncthreads();
+        n = count;
+    }
+    if (n <= BS_LIST) {
+        // each counts the larger ones: its place; where several have the same place they have the same value, and are told apart by their tokens
+        if (tid < 4) sm.part.value[n + tid] = -INFINITY;
+        __syncthreads();
+        for (int i = tid; i < n; i += BS_THREADS) {
+            const float mine = sm.part.value[i];
+            int above = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; j += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(sm.part.value + j);
+                above += (f.x > mine) + (f.y > mine) + (f.z > mine) + (f.w > mine);
+            }
+            if (above < keep && atomicAdd(&taken[above], 1) == 0) top.one[above] = bs_pack(mine, (uint32_t)sm.part.token[i]);
         }
-    });
-    for (int i = tid; i < a.keep; i += BS_THREADS) {
+        __syncthreads();
+        bool equal = false;
+        if (tid < keep) equal = taken[tid] > 1;
+        if (__syncthreads_or(equal))
+            for (int i = tid; i < n; i += BS_THREADS) {
+                const float mine = sm.part.value[i];
+                int above = 0, before = 0;
+                for (int j = 0; j < n; j++) {
+                    above += sm.part.value[j] > mine;
+                    before += sm.part.value[j] == mine && sm.part.token[j] < sm.part.token[i];
+                }
+                if (above + before < keep) top.one[above + before] = bs_pack(mine, (uint32_t)sm.part.token[i]);
+            }
+    } else {
+        bs_pick(sm.one, keep, top.one, [x, from, to, tid](auto&& take) {      // from memory again
+            for (int i = from + tid; i < to; i += BS_THREADS) {
+                const float f = x[i];
+                take(f == f ? bs_pack(f, (uint32_t)i) : bs_pack(-INFINITY, (uint32_t)i));
+            }
+        });
+    }
+    __syncthreads();
+    for (int i = tid; i < keep; i += BS_THREADS) a.lists[((size_t)row * a.parts + part) * keep + i] = top.one[i];
+
+    // ---- the block that completes the request goes on
+    const int request = row / a.beams;
+    __syncthreads();
+    if (tid == 0) {
+        int old;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(a.arrived + request) : "memory");
+        done = old == a.beams * a.parts - 1;
+        if (done) a.arrived[request] = 0;                     // ready for the next launch
+    }
+    __syncthreads();
+    if (!done) return;
+
+    // ---- its rows' lists: of each the first entries, as many as can be held, are asked for now
+    const int n_lists = a.beams * a.parts, held = min(keep, BS_HELD / n_lists), entries = n_lists * held;
+    const u64* mine = a.lists + (size_t)request * n_lists * keep;
+    auto over = [](int x, float by) { return (int)(((float)x + 0.5f) * by); };        // x / n for x below 2^22
+    const float per_list = 1.0f / (float)held, per_row = 1.0f / (float)a.parts;
+    {
+        u64 raw[BS_HELD / BS_THREADS];
+#pragma unroll
+        for (int j = 0; j < BS_HELD / BS_THREADS; j++) {
+            const int e = tid + j * BS_THREADS, list = over(e, per_list);
+            raw[j] = e < entries ? __ldcg(mine + list * keep + e - list * held) : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < BS_HELD / BS_THREADS; j++) sm.merge.entry[tid + j * BS_THREADS] = raw[j];
+    }
+    // ---- its rows' sums: 4 to 32 threads a row.  base = score - log sum exp; -inf for a row that has no softmax or does not live
+    {
+        int each = 32;
+        while (each * a.beams > BS_THREADS) each >>= 1;
+        const int b = tid / each, sub = tid % each;
+        const float score = b < a.beams ? a.scores[request * a.beams + b] : 0.0f;
+        m = -INFINITY;
+        s = 0.0f;
+        if (b < a.beams)
+            for (int i = sub; i < a.parts; i += each) {
+                const float2 o = __ldcg(a.sums + ((size_t)request * a.beams + b) * a.parts + i);
+                bs_join(m, s, o.x, o.y);
+            }
+#pragma unroll 1
+        for (int o = 1; o < each; o <<= 1) bs_join(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+        if (b < a.beams && sub == 0) {
+            const double lse = (double)m + log((double)s);
+            base[b] = isfinite(score) && isfinite(lse) ? (double)score - lse : (double)-INFINITY;
+        }
+        if (tid == 0) { count = 0; bound_s = 0; }
+        if (tid < keep) { taken[tid] = 0; top.two[tid] = bs_none<BsPair>(); }
+    }
+    __syncthreads();
+    // ---- the best of its rows' lists
+    auto of_entry = [&](u64 c, int list, int rank) {
+        const int b = over(list, per_row);
+        if (base[b] == (double)-INFINITY)                       // the row's tokens in their order, once a row
+            return list == b * a.parts && rank < a.vocab ? BsPair{bs_order64((double)-INFINITY), 0xffffffffu - ((uint32_t)b * (uint32_t)a.vocab + (uint32_t)rank)} : bs_none<BsPair>();
+        if (c == 0) return bs_none<BsPair>();
+        return BsPair{bs_order64(base[b] + (double)bs_value((uint32_t)(c >> 32))), 0xffffffffu - ((uint32_t)b * (uint32_t)a.vocab + (0xffffffffu - (uint32_t)c))};
+    };
+    auto candidate = [&](int list, int rank) { return of_entry(__ldcg(mine + (size_t)list * keep + rank), list, rank); };
+    auto into_list = [&](u64 value, uint32_t flat) {
+        const int at = atomicAdd(&count, 1);
+        if (at < BS_LIST) {
+            sm.merge.value[at] = value;
+            sm.merge.flat[at] = flat;
+        }
+    };
+    auto rounded = [](const BsPair& c) { return bs_is_none(c) ? -INFINITY : __double2float_rd(bs_value64(c.hi)); };
+    float reaches = -INFINITY;
+#pragma unroll 1
+    for (int e = tid; e < entries; e += BS_THREADS) {
+        const int list = over(e, per_list);
+        const BsPair c = of_entry(sm.merge.entry[e], list, e - list * held);
+        sm.merge.entry[e] = c.hi;
+        sm.merge.place[e] = c.lo;
+        reaches = fmaxf(reaches, rounded(c));
+    }
+    const float lowest = bs_bound(reaches, 1, keep, group, &bound_s);
+    const u64 least = lowest == -INFINITY ? 0 : bs_order64((double)lowest);
+#pragma unroll 1
+    for (int e = tid; e < entries; e += BS_THREADS) {
+        if (sm.merge.place[e] == 0 || sm.merge.entry[e] < least) continue;
+        into_list(sm.merge.entry[e], sm.merge.place[e]);
+        const int list = over(e, per_list);
+        if (e - list * held + 1 == held)                        // a list's last held entry reaches the bound: on from there
+#pragma unroll 1
+            for (int rank = held; rank < keep; rank += 8) {
+                BsPair c[8];
+#pragma unroll
+                for (int f = 0; f < 8; f++) c[f] = rank + f < keep ? candidate(list, rank + f) : bs_none<BsPair>();
+#pragma unroll
+                for (int f = 0; f < 8; f++)
+                    if (!bs_is_none(c[f]) && c[f].hi >= least) into_list(c[f].hi, c[f].lo);
+                if (bs_is_none(c[7]) || c[7].hi < least) break;
+            }
+    }
+    __syncthreads();
+    int n2 = count;
+    if (n2 <= BS_LIST && n2 > 2 * keep && n2 > 64) {
+        // a second bound, of the list itself, where the first let many through (beams far apart): the list moves to where the entries were
+        float mine_best = -INFINITY;
+        for (int i = tid; i < n2; i += BS_THREADS) mine_best = fmaxf(mine_best, __double2float_rd(bs_value64(sm.merge.value[i])));
+        __syncthreads();
+        if (tid == 0) { count = 0; bound_s = 0; }
+        __syncthreads();
+        const float second = bs_bound(mine_best, 1, keep, group, &bound_s);
+        const u64 least2 = second == -INFINITY ? 0 : bs_order64((double)second);
+        for (int i = tid; i < n2; i += BS_THREADS)
+            if (sm.merge.value[i] >= least2) {
+                const int at = atomicAdd(&count, 1);
+                sm.merge.entry[at] = sm.merge.value[i];
+                sm.merge.place[at] = sm.merge.flat[i];
+            }
+        __syncthreads();
+        n2 = count;
+        for (int i = tid; i < n2; i += BS_THREADS) { sm.merge.value[i] = sm.merge.entry[i]; sm.merge.flat[i] = sm.merge.place[i]; }
+        __syncthreads();
+    }
+    if (n2 <= BS_LIST) {
+        for (int i = tid; i < n2; i += BS_THREADS) {
+            const u64 value = sm.merge.value[i];
+            int above = 0;
+#pragma unroll 4
+            for (int j = 0; j < n2; j++) above += sm.merge.value[j] > value;
+            if (above < keep && atomicAdd(&taken[above], 1) == 0) top.two[above] = BsPair{value, sm.merge.flat[i]};
+        }
+        __syncthreads();
+        bool equal = false;
+        if (tid < keep) equal = taken[tid] > 1;
+        if (__syncthreads_or(equal))
+            for (int i = tid; i < n2; i += BS_THREADS) {
+                const BsPair c = {sm.merge.value[i], sm.merge.flat[i]};
+                int above = 0;
+                for (int j = 0; j < n2; j++) above += bs_above(BsPair{sm.merge.value[j], sm.merge.flat[j]}, c);
+                if (above < keep) top.two[above] = c;
+            }
+        __syncthreads();
+    } else {
+        bs_pick(sm.two, keep, top.two, [&](auto&& take) {
+            for (int e = tid; e < n_lists * keep; e += BS_THREADS) {
+                const BsPair c = candidate(e / keep, e % keep);
+                if (!bs_is_none(c)) take(c);
+            }
+        });
+    }
+    for (int i = tid; i < keep; i += BS_THREADS) {
         const BsPair c = top.two[i];
         const uint32_t flat = 0xffffffffu - c.lo;
-        const size_t at = (size_t)request * a.keep + i;
+        const size_t at = (size_t)request * keep + i;
         a.out_score[at] = (float)bs_value64(c.hi);
         a.out_parent[at] = (int)(flat / (uint32_t)a.vocab);
         a.out_token[at] = (int)(flat % (uint32_t)a.vocab);
     }
 }
 
-struct BsShape { int values, parts, merge_rows; };
-
-// Values a thread holds, blocks a row, and whether rows are merged first; by sizes alone, so that the scratch can be asked for without a device.
-static BsShape bs_shape(long long rows, int vocab, int keep, int beams) {
-    BsShape s;
-    const int small = BS_THREADS * 16, large = BS_THREADS * 32;
-    s.values = rows * ((vocab + small - 1) / small) <= 4 * 148 ? 16 : 32;
-    const int chunk = s.values == 16 ? small : large;
-    s.parts = (vocab + chunk - 1) / chunk;
-    s.merge_rows = (long long)beams * s.parts * keep > 4096;
-    return s;
+// How long a block's stretch of a row is, in values, and how many make a row: as many rounds of loads a block as keep all blocks running at once (four a multiprocessor).
+struct BsShape { int stretch, parts; };
+static BsShape bs_shape(int rows, int vocab) {
+    const int round = BS_THREADS * BS_VALUES, rounds = (vocab + round - 1) / round, each = (int)(((long long)rows * rounds + 4 * 148 - 1) / (4 * 148));
+    return BsShape{each * round, (rounds + each - 1) / each};
 }
 
 }  // namespace vk
@@ -293,29 +524,28 @@ static BsShape bs_shape(long long rows, int vocab, int keep, int beams) {
 using namespace vk;
 
 VK_API size_t vk_beam_select_scratch_bytes(int rows, int vocab, int keep) {
-    // rows of either shape: as many parts as the shorter chunks make
-    const size_t parts = (size_t)(vocab + BS_THREADS * 16 - 1) / (BS_THREADS * 16);
-    return (size_t)2 * BS_MAX_ROWS * 4 + rows * parts * 8 + ((size_t)rows * parts * keep + (size_t)rows * keep) * 8;
+    // the shortest stretches' parts, whatever the rows
+    const size_t parts = (size_t)(vocab + BS_THREADS * BS_VALUES - 1) / (BS_THREADS * BS_VALUES);
+    return (size_t)BS_MAX_ROWS * 4 + rows * parts * 8 + (size_t)rows * parts * keep * 8;
 }
 
-// scratch: vk_beam_select_scratch_bytes bytes for at least as many rows, as large a vocabulary and as many kept; its first 2 * BS_MAX_ROWS words were zero
+// scratch: vk_beam_select_scratch_bytes bytes for at least as many rows, as large a vocabulary and as many kept; its first BS_MAX_ROWS words were zero
 // at first use and are zero again after every launch.
-VK_API int vk_beam_select(const float* logits, const float* scores, float* out_score, int32_t* out_parent, int32_t* out_token, void* scratch, int rows,
-                          int beams, int vocab, long long ld, int keep, cudaStream_t stream) {
+VK_API int vk_beam_select(const float* logits, const float* scores, float* out_score, int32_t* out_parent, int32_t* out_token, void* scratch, size_t scratch_bytes,
+                          int rows, int beams, int vocab, long long ld, int keep, cudaStream_t stream) {
     if (rows <= 0) return VK_OK;
     if (beams <= 0 || rows % beams || vocab <= 0 || ld < vocab || keep <= 0 || !scratch) return VK_BAD_SHAPE;
     if (beams > BS_MAX_BEAMS || keep > BS_MAX_KEEP || vocab > BS_MAX_PARTS * BS_THREADS * 16 || rows > BS_MAX_ROWS) return VK_TOO_LARGE;
     if ((long long)beams * vocab < keep) return VK_BAD_SHAPE;
     if ((uintptr_t)logits % 4 || (uintptr_t)scratch % 16) return VK_BAD_ALIGNMENT;
-    const BsShape s = bs_shape(rows, vocab, keep, beams);
+    if (scratch_bytes < vk_beam_select_scratch_bytes(rows, vocab, keep)) return VK_SMALL_SCRATCH;
+    const BsShape s = bs_shape(rows, vocab);
     BsArgs a;
     a.logits = logits; a.scores = scores; a.out_score = out_score; a.out_parent = out_parent; a.out_token = out_token;
     char* at = (char*)scratch;
-    a.arrived = (int*)at; at += (size_t)2 * BS_MAX_ROWS * 4;
+    a.arrived = (int*)at; at += (size_t)BS_MAX_ROWS * 4;
     a.lists = (u64*)at; at += (size_t)rows * s.parts * keep * 8;
-    a.row_lists = (u64*)at; at += (size_t)rows * keep * 8;
     a.sums = (float2*)at;
-    a.ld = ld; a.beams = beams; a.vocab = vocab; a.keep = keep; a.parts = s.parts; a.merge_rows = s.merge_rows;
-    if (s.values == 16) return launch_dependent(beam_select_kernel<16>, dim3(s.parts, rows), dim3(BS_THREADS), 0, stream, a);
-    return launch_dependent(beam_select_kernel<32>, dim3(s.parts, rows), dim3(BS_THREADS), 0, stream, a);
+    a.ld = ld; a.beams = beams; a.vocab = vocab; a.keep = keep; a.parts = s.parts; a.stretch = s.stretch;
+    return launch_dependent(beam_select_kernel, dim3(s.parts, rows), dim3(BS_THREADS), 0, stream, a);
 }

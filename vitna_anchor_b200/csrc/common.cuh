@@ -19,6 +19,7 @@
 #define VK_BAD_SHAPE (-1)      // a size this kernel does not take
 #define VK_BAD_ALIGNMENT (-2)  // a pointer or stride that is not aligned as needed
 #define VK_TOO_LARGE (-3)      // beyond a stated maximum
+#define VK_SMALL_SCRATCH (-4)  // fewer bytes of scratch than the call needs
 
 namespace vk {
 

@@ -7,6 +7,7 @@ VK_API const char* vk_error_string(int status) {
         case VK_OK: return "ok";
         case VK_BAD_SHAPE: return "a size this kernel does not take";
         case VK_BAD_ALIGNMENT: return "a pointer or stride is not aligned as the kernel needs";
+        case VK_SMALL_SCRATCH: return "the scratch is too small";
         case VK_TOO_LARGE: return "a size beyond the kernel's stated maximum";
         default: return "unknown status";
     }

@@ -8,6 +8,7 @@ not on a CUDA device, the call raises.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from typing import Optional, Sequence
@@ -2243,12 +2244,27 @@ def token_side(x: torch.Tensor, y: Optional[torch.Tensor], scale: Optional[torch
 # Beam search: attention over pages held in common, the choice of continuations, moves of cache rows
 # ---------------------------------------------------------------------------
 
-def _on_current(name: str, *tensors: torch.Tensor) -> None:
-    """Refuses tensors of another device than the current one, on whose stream the launch goes."""
-    here = torch._C._cuda_getDevice()
-    for t in tensors:
-        if t.get_device() != here:
-            raise KernelError(f"{name}: a tensor is on device {t.get_device()} and the current device is {here}")
+_entries = {}
+_C_POINTER, _C_INT, _C_LONG, _C_SIZE, _C_FLOAT = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_size_t, ctypes.c_float
+
+
+def _entry(name: str, types: str):
+    """The library's function `name` with its arguments' types (p pointer, i int, l long long, z size_t, f float), so that plain integers go in: half
+    the host's time of a call that wraps every pointer."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes = [{"p": _C_POINTER, "i": _C_INT, "l": _C_LONG, "z": _C_SIZE, "f": _C_FLOAT}[c] for c in types]
+        _entries[name] = fn
+    return fn
+
+
+def _fit(t: torch.Tensor, name: str, dtype, dims: int, here: int) -> int:
+    """_req, on the current device (`here`), on whose stream the launch goes; returns the address."""
+    if t.get_device() != here or t.dtype is not dtype or t.dim() != dims or not t.is_contiguous():
+        _req(t, name, dtype, dims)
+        raise KernelError(f"{name} is on device {t.get_device()} and the current device is {here}")
+    return t.data_ptr()
 
 
 SHARED_MAX_TOKENS, SHARED_MAX_HEADS, SHARED_MAX_KV_HEADS = 256, 64, 128      # tokens a launch, query heads a key-value head, key-value heads
@@ -2278,24 +2294,25 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
     is in no family are left as they were.  Block numbers outside the pool are not followed (their keys and values count as zeros).
     scratch: a byte buffer of attention_shared_scratch_bytes(members, ...) or more, whatever it holds, for launches of one stream at a time.  The lists and
     lengths are read while the kernel before this one in the stream may still run: that must not be a kernel of this library which writes them."""
-    _req(q, "q", dims=2); _req(cache_layer, "cache_layer", q.dtype, 5); _req(block_tables, "block_tables", torch.int32, 2)
-    _req(token_seg, "token_seg", torch.int32, 1); _req(positions, "positions", torch.int32, 1); _req(out, "out", q.dtype, 2)
-    _req(members, "members", torch.int32, 1); _req(starts, "starts", torch.int32, 1); _req(shared, "shared", torch.int32, 1); _req(scratch, "scratch", torch.uint8, 1)
-    T, n, families, page_size = q.shape[0], members.shape[0], shared.shape[0], cache_layer.shape[3]
-    if not attention_shared_takes(q.dtype, nh, nkv, hd, n):
-        raise KernelError(f"attention_shared: {n} tokens of {nh} heads over {nkv} of {hd} in {q.dtype} are not taken")
-    if q.shape[1] != nh * hd or out.shape != q.shape or cache_layer.shape[1] != 2 or cache_layer.shape[2] != nkv or cache_layer.shape[4] != hd:
+    here, dtype, i32 = torch._C._cuda_getDevice(), q.dtype, torch.int32
+    pq, pc, po = _fit(q, "q", dtype, 2, here), _fit(cache_layer, "cache_layer", dtype, 5, here), _fit(out, "out", dtype, 2, here)
+    pt, ps, pp = _fit(block_tables, "block_tables", i32, 2, here), _fit(token_seg, "token_seg", i32, 1, here), _fit(positions, "positions", i32, 1, here)
+    pm, pst, psh = _fit(members, "members", i32, 1, here), _fit(starts, "starts", i32, 1, here), _fit(shared, "shared", i32, 1, here)
+    T, width = q.shape
+    n, families = members.shape[0], shared.shape[0]
+    pages, two, kv_heads, page_size, dim = cache_layer.shape
+    segments, max_blocks = block_tables.shape
+    if not attention_shared_takes(dtype, nh, nkv, hd, n):
+        raise KernelError(f"attention_shared: {n} tokens of {nh} heads over {nkv} of {hd} in {dtype} are not taken")
+    if width != nh * hd or out.shape != q.shape or two != 2 or kv_heads != nkv or dim != hd:
         raise KernelError("attention_shared: shapes do not fit the head counts")
     if token_seg.shape[0] != T or positions.shape[0] != T:
         raise KernelError("attention_shared: per-token arrays differ in length")
     if starts.shape[0] != families + 1 or families > SHARED_MAX_TOKENS:
         raise KernelError("attention_shared: starts is not one longer than shared, or there are more than 256 families")
-    if scratch.numel() < attention_shared_scratch_bytes(n, nh, nkv, hd):
-        raise KernelError("attention_shared: the scratch is too small")
-    _on_current("attention_shared", q, cache_layer, block_tables, token_seg, positions, members, starts, shared, out, scratch)
-    _check(lib().vk_attention_shared(_p(q), _p(cache_layer), _p(block_tables), _p(token_seg), _p(positions), _p(members), _p(starts), _p(shared), _p(out),
-                                     _p(scratch), T, block_tables.shape[0], n, families, cache_layer.shape[0], nh, nkv, hd, page_size,
-                                     block_tables.shape[1], ctypes.c_float(scale), _dt(q), _stream()), "attention_shared")
+    fn = _entry("vk_attention_shared", "ppppppppppziiiiiiiiiifip")
+    _check(fn(pq, pc, pt, ps, pp, pm, pst, psh, po, _fit(scratch, "scratch", torch.uint8, 1, here), scratch.numel(), T, segments, n, families, pages, nh, nkv, hd,
+              page_size, max_blocks, scale, 0 if dtype == torch.float32 else 1, torch._C._cuda_getCurrentRawStream(here)), "attention_shared")
     add_launches(1)                       # the walk, and the launch that joins the rows' parts
     return out
 
@@ -2315,11 +2332,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
     probabilities.  out = (scores float32, row within the request int32, v int32), each [requests, keep]; returns it.  A row without a softmax (a
     NaN, an infinite maximum, nothing above -inf) or whose score is not finite (a beam that does not live) offers its tokens at -inf.
     scratch: a byte buffer of beam_select_scratch_bytes(rows, vocab, keep) or more, zeros at first use, for launches of one stream at a time."""
-    if not logits.is_cuda or logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
-        raise KernelError("beam_select: logits are not a float32 CUDA matrix with unit column stride")
-    _req(scores, "scores", torch.float32, 1); _req(scratch, "scratch", torch.uint8, 1)
-    best, parent, token = out
-    _req(best, "out[0]", torch.float32, 2); _req(parent, "out[1]", torch.int32, 2); _req(token, "out[2]", torch.int32, 2)
+    here, best, parent, token = torch._C._cuda_getDevice(), *out
+    if logits.get_device() != here or logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1:
+        raise KernelError("beam_select: logits are not a float32 matrix with unit column stride on the current CUDA device")
+    ps, pb = _fit(scores, "scores", torch.float32, 1, here), _fit(best, "out[0]", torch.float32, 2, here)
+    pp, pt = _fit(parent, "out[1]", torch.int32, 2, here), _fit(token, "out[2]", torch.int32, 2, here)
     R, V = logits.shape
     if not (1 <= beams <= BEAM_MAX_BEAMS and 1 <= keep <= BEAM_MAX_KEEP and R <= BEAM_MAX_ROWS and 1 <= V <= BEAM_MAX_VOCAB):
         raise KernelError(f"beam_select: {beams} beams (of {R} rows) over {V} tokens, {keep} kept: at most {BEAM_MAX_BEAMS}, {BEAM_MAX_ROWS}, {BEAM_MAX_VOCAB} and {BEAM_MAX_KEEP}")
@@ -2327,11 +2344,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
         raise KernelError("beam_select: rows are not whole requests, scores are not one a row, or more is kept than there is")
     if best.shape != (R // beams, keep) or parent.shape != best.shape or token.shape != best.shape:
         raise KernelError("beam_select: out is not three of [requests, keep]")
-    if scratch.numel() < beam_select_scratch_bytes(R, V, keep):
-        raise KernelError("beam_select: the scratch is too small")
-    _on_current("beam_select", logits, scores, best, parent, token, scratch)
-    _check(lib().vk_beam_select(_p(logits), _p(scores), _p(best), _p(parent), _p(token), _p(scratch), R, beams, V,
-                                ctypes.c_longlong(max(V, logits.stride(0)) if R > 1 else V), keep, _stream()), "beam_select")
+    fn = _entry("vk_beam_select", "ppppppziiilip")
+    _check(fn(logits.data_ptr(), ps, pb, pp, pt, _fit(scratch, "scratch", torch.uint8, 1, here), scratch.numel(), R, beams, V, logits.stride(0) if R > 1 else V, keep,
+              torch._C._cuda_getCurrentRawStream(here)), "beam_select")
     return out
 
 
@@ -2339,26 +2354,30 @@ def copy_rows(arena: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> to
     """arena[l, dst[i]] = arena[l, src[i]] for every layer l and move i, in one launch (one a 128 moves).  arena [layers, rows, ...], any type; a row's
     elements lie together, rows and layers may lie apart.  src and dst are row numbers on the host: no row is written twice, or read and written.
     A captured graph repeats the moves it was captured with."""
-    if not arena.is_cuda or arena.dim() < 2:
-        raise KernelError("copy_rows: the arena is not a CUDA tensor [layers, rows, ...]")
+    here = torch._C._cuda_getDevice()
+    if arena.get_device() != here or arena.dim() < 2:
+        raise KernelError("copy_rows: the arena is not a tensor [layers, rows, ...] on the current CUDA device")
     L, N, size = arena.shape[0], arena.shape[1], arena.element_size()
-    numbers = 1
-    for d in range(arena.dim() - 1, 1, -1):
-        if arena.shape[d] != 1 and arena.stride(d) != numbers:
-            raise KernelError("copy_rows: a row's elements do not lie together")
-        numbers *= arena.shape[d]
+    row, layer = arena.stride(1), arena.stride(0)
+    if arena.is_contiguous() and N > 1:
+        numbers = row
+    else:
+        numbers = 1
+        for d in range(arena.dim() - 1, 1, -1):
+            if arena.shape[d] != 1 and arena.stride(d) != numbers:
+                raise KernelError("copy_rows: a row's elements do not lie together")
+            numbers *= arena.shape[d]
+        if (N > 1 and row < numbers) or (L > 1 and layer < (N - 1) * row + numbers):
+            raise KernelError("copy_rows: rows or layers overlap")
     n, written = len(src), set(dst)
     if len(dst) != n or len(written) != n or not written.isdisjoint(src):
         raise KernelError("copy_rows: src and dst differ in length, or a row is written twice, or read and written")
     if n == 0 or L == 0 or numbers == 0:
         return arena
-    if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= N:
+    if min(src) < 0 or min(dst) < 0 or max(src) >= N or max(dst) >= N:
         raise KernelError(f"copy_rows: a row is outside the arena's {N}")
-    row, layer = arena.stride(1), arena.stride(0)
-    if row < numbers or (L > 1 and layer < (N - 1) * row + numbers):
-        raise KernelError("copy_rows: rows or layers overlap")
-    _on_current("copy_rows", arena)
-    ints = ctypes.c_int32 * n
-    _check(lib().vk_copy_rows(_p(arena), L, N, ctypes.c_longlong(layer * size if L > 1 else 0), ctypes.c_longlong(row * size), ctypes.c_longlong(numbers * size),
-                              ints(*src), ints(*dst), n, _stream()), "copy_rows")
+    s, d = array.array("i", src), array.array("i", dst)
+    fn = _entry("vk_copy_rows", "piilllppip")
+    _check(fn(arena.data_ptr(), L, N, layer * size if L > 1 else 0, row * size, numbers * size, s.buffer_info()[0], d.buffer_info()[0], n,
+              torch._C._cuda_getCurrentRawStream(here)), "copy_rows")
     return arena
