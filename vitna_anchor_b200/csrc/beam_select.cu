@@ -11,17 +11,17 @@
 // beams' candidates are told apart where float32 sums would tie.
 //
 // Choosing `keep` of many, without sorting them: the block's threads make 32 to 256 groups, at least twice as many as are kept; the keep-th largest of the groups'
-// best is a bound that at least `keep` values reach and few others do (17 values of 4,096 normal ones above the bound for keep = 8, 150 for 64).  Those are put in a list
-// in shared memory and each counts how many of the list are larger: its place.  The merge does the same with the lists' first entries, and goes on down a list whose last
-// one of those still reaches the bound.  Where too many reach the bound (many equal values, values laid out against the groups) the choice is made by value and token together, and at last the bound
-// raised bit by bit to the keep-th largest itself.
+// best is a bound that at least `keep` values reach and few others do (17 values of 4,096 normal ones above the bound for keep = 8, 150 for 64).  Every thread knows its largest value of each
+// round of loads, so only the sixteens that hold such a value are read again; the values are put in a list in shared memory and each counts how many of the list are larger: its
+// place.  The merge does the same with the lists' first entries, and goes on down a list whose last one of those still reaches the bound.  Where too many reach
+// the bound (many equal values, values laid out against the groups) the choice is made by value and token together, and at last the bound raised bit by bit to the keep-th largest itself.
 #include "common.cuh"
 
 #include <cuda_fp16.h>
 
 namespace vk {
 
-constexpr int BS_THREADS = 256, BS_VALUES = 16, BS_MAX_KEEP = 128, BS_MAX_BEAMS = 64, BS_LIST = 1024, BS_MAX_PARTS = 64, BS_MAX_ROWS = 1024, BS_HELD = 2048;
+constexpr int BS_THREADS = 256, BS_VALUES = 16, BS_MAX_KEEP = 128, BS_MAX_BEAMS = 64, BS_LIST = 1024, BS_MAX_PARTS = 64, BS_MAX_ROWS = 1024, BS_HELD = 2048, BS_ROUND = BS_THREADS * BS_VALUES, BS_MAX_ROUNDS = 8;
 
 typedef unsigned long long u64;
 
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_select_kernel(const BsArgs
     __shared__ union {
         struct {                                       // this block's values that reach the bound, and their tokens
             float value[BS_LIST + 4];
-            int token[BS_LIST];
+            int token[BS_LIST], slot[BS_LIST];
         } part;
         struct {                                       // the request's entries, and those of them that reach the bound
             u64 entry[BS_HELD];
@@ -210,9 +210,11 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_select_kernel(const BsArgs
     __shared__ __align__(16) __half group[BS_THREADS];
     __shared__ float2 warp_sums[BS_THREADS / 32];
     __shared__ uint32_t bound_s;
-    __shared__ int taken[BS_MAX_KEEP], count, done;
+    __shared__ int taken[BS_MAX_KEEP], slots, count, done;
+    float* best = reinterpret_cast<float*>(sm.merge.entry) + sizeof(sm.part) / 4;      // a thread's largest value of every round: behind the list
+    static_assert(sizeof(sm.part) + BS_MAX_ROUNDS * BS_THREADS * 4 <= sizeof(sm.merge), "the rounds' largest values lie behind the list");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, part = blockIdx.x, row = blockIdx.y, keep = a.keep;
-    if (tid == 0) { bound_s = 0; count = 0; }
+    if (tid == 0) { bound_s = 0; slots = 0; count = 0; }
     if (tid < keep) { taken[tid] = 0; top.one[tid] = 0; }
     dependency_wait();
     let_dependents_start();
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_select_kernel(const BsArgs
     // ---- this block's values: thread t has four neighbours of every 1,024 (wherever the row begins, so that equal rows have equal sums)
     const float* x = a.logits + (size_t)row * a.ld;
     const bool aligned = (uintptr_t)x % 16 == 0;
-    const int from = part * a.stretch, to = min(a.vocab, from + a.stretch), lanes = bs_lanes(keep);
+    const int from = part * a.stretch, to = min(a.vocab, from + a.stretch);
     float v[BS_VALUES], next[BS_VALUES];
     auto load = [&](int first) {
 #pragma unroll
@@ -237,45 +239,53 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_select_kernel(const BsArgs
     };
     load(from);
     float m = -INFINITY, s = 0.0f;
-    int round = 0, refresh = 1;
-    float bound = -INFINITY;
 #pragma unroll 1
-    for (int at = from; at < to; at += BS_THREADS * BS_VALUES, round++) {
+    for (int at = from, round = 0; at < to; at += BS_ROUND, round++) {
 #pragma unroll
         for (int j = 0; j < BS_VALUES; j++) v[j] = next[j];
-        if (at + BS_THREADS * BS_VALUES < to) load(at + BS_THREADS * BS_VALUES);
+        if (at + BS_ROUND < to) load(at + BS_ROUND);
         float here = v[0];
 #pragma unroll
         for (int j = 1; j < BS_VALUES; j++) here = fmaxf(here, v[j]);
+        best[round * BS_THREADS + tid] = here;
         // the sum of exponentials: of nothing above -inf nothing; a NaN stays one
         const float more = fmaxf(m, here), ref = more == -INFINITY ? 0.0f : more;
         s *= bs_exp(m - ref);
         m = more;
 #pragma unroll
         for (int j = 0; j < BS_VALUES; j++) s += bs_exp(v[j] - ref);
-        // the values that reach the bound of what has been seen so far, which is taken anew after 1, 2, 4 ... rounds (and as long as there is none)
-        if (round + 1 == refresh || bound == -INFINITY) {
-            bound = bs_bound(m, lanes, keep, group, &bound_s);
-            refresh = 2 * (round + 1);
-        }
-        if (__any_sync(0xffffffffu, here >= bound && here > -INFINITY)) {
-            const float least = fmaxf(bound, -3.402823466e38f);            // -inf comes in behind, if at all
-            uint32_t hits = 0;
-#pragma unroll
-            for (int j = 0; j < BS_VALUES; j++) hits |= v[j] >= least ? 1u << j : 0u;
-            int place = hits ? atomicAdd(&count, __popc(hits)) : 0;
-#pragma unroll
-            for (int j = 0; j < BS_VALUES; j++)
-                if (hits >> j & 1) {
-                    if (place < BS_LIST) sm.part.token[place] = at + j / 4 * (BS_THREADS * 4) + tid * 4 + j % 4;
-                    place++;
-                }
-        }
     }
+    const float bound = bs_bound(m, bs_lanes(keep), keep, group, &bound_s), enough = fmaxf(bound, -3.402823466e38f);      // -inf comes in behind, if at all
     bs_join_warp(m, s);
     if (lane == 0) warp_sums[warp] = make_float2(m, s);
+    // ---- the sixteens that hold a value that reaches the bound, and then those values
+    for (int at = from, slot = tid; at < to; at += BS_ROUND, slot += BS_THREADS)
+        if (best[slot] >= enough) {
+            const int place = atomicAdd(&slots, 1);
+            if (place < BS_LIST) sm.part.slot[place] = slot;
+        }
     __syncthreads();
-    int n = count;
+    const int fours = min(slots, BS_LIST) * (BS_VALUES / 4);
+    for (int c = tid; c < fours; c += BS_THREADS) {
+        const int slot = sm.part.slot[c / (BS_VALUES / 4)], i = from + slot / BS_THREADS * BS_ROUND + (c % (BS_VALUES / 4) * BS_THREADS + slot % BS_THREADS) * 4;
+        float f[4];
+        if (aligned && i + 3 < to) {
+            const float4 g = *reinterpret_cast<const float4*>(x + i);
+            f[0] = g.x; f[1] = g.y; f[2] = g.z; f[3] = g.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) f[e] = i + e < to ? x[i + e] : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (f[e] >= enough) {
+                const int place = atomicAdd(&count, 1);
+                if (place < BS_LIST) {
+                    sm.part.value[place] = f[e];
+                    sm.part.token[place] = i + e;
+                }
+            }
+    }
     if (warp == 0) {
         const float2 o = lane < BS_THREADS / 32 ? warp_sums[lane] : make_float2(-INFINITY, 0.0f);
         m = o.x;
@@ -283,42 +293,23 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_select_kernel(const BsArgs
         bs_join_warp(m, s);
         if (lane == 0) a.sums[(size_t)row * a.parts + part] = make_float2(m, s);
     }
-    for (int i = tid; i < min(n, BS_LIST); i += BS_THREADS) sm.part.value[i] = x[sm.part.token[i]];
-    if (n < keep && warp == 1) {
-        // everything above -inf is in the list: behind it come the first tokens that are -inf
-        int have = n;
-        for (int i = from + lane; have < keep && i - lane < to; i += 32) {
-            const bool none = i < to && x[i] == -INFINITY;
-            const uint32_t all = __ballot_sync(0xffffffffu, none);
-            const int place = have + __popc(all & ((1u << lane) - 1));
-            if (none && place < keep) { sm.part.value[place] = -INFINITY; sm.part.token[place] = i; }
-            have += __popc(all);
-        }
-        if (lane == 0) done = min(have, keep);
-    }
     __syncthreads();
-    if (n < keep) n = done;
-    if (n <= BS_LIST && n > 2 * keep && n > 64) {
-        // a second bound, of the list itself: the first let through what reached the bounds of the values before
-        float best = -INFINITY;
-        for (int i = tid; i < n; i += BS_THREADS) best = fmaxf(best, sm.part.value[i]);
-        const float bound = bs_bound(best, 1, keep, group, &bound_s);
-        float kept_value[BS_LIST / BS_THREADS];
-        int kept_token[BS_LIST / BS_THREADS];
-#pragma unroll
-        for (int j = 0; j < BS_LIST / BS_THREADS; j++)
-            if (tid + j * BS_THREADS < n) { kept_value[j] = sm.part.value[tid + j * BS_THREADS]; kept_token[j] = sm.part.token[tid + j * BS_THREADS]; }
-        if (tid == 0) count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < BS_LIST / BS_THREADS; j++)
-            if (tid + j * BS_THREADS < n && kept_value[j] >= bound) {
-                const int place = atomicAdd(&count, 1);
-                sm.part.value[place] = kept_value[j];
-                sm.part.token[place] = kept_token[j];
+    int n = slots > BS_LIST ? BS_LIST + 1 : count;
+    if (n < keep) {
+        // everything above -inf is in the list: behind it come the first tokens that are -inf
+        if (warp == 0) {
+            int have = n;
+            for (int i = from + lane; have < keep && i - lane < to; i += 32) {
+                const bool none = i < to && x[i] == -INFINITY;
+                const uint32_t all = __ballot_sync(0xffffffffu, none);
+                const int place = have + __popc(all & ((1u << lane) - 1));
+                if (none && place < keep) { sm.part.value[place] = -INFINITY; sm.part.token[place] = i; }
+                have += __popc(all);
             }
+            if (lane == 0) done = min(have, keep);
+        }
         __syncthreads();
-        n = count;
+        n = done;
     }
     if (n <= BS_LIST) {
         // each counts the larger ones: its place; where several have the same place they have the same value, and are told apart by their tokens
@@ -512,11 +503,14 @@ __global__ void __launch_bounds__(BS_THREADS, 4) beam_select_kernel(const BsArgs
     }
 }
 
-// How long a block's stretch of a row is, in values, and how many make a row: as many rounds of loads a block as keep all blocks running at once (four a multiprocessor).
+// How long a block's stretch of a row is, in values, and how many make a row: as many rounds of loads a block as keep all blocks running at once (four a multiprocessor), at
+// most eight.
 struct BsShape { int stretch, parts; };
 static BsShape bs_shape(int rows, int vocab) {
-    const int round = BS_THREADS * BS_VALUES, rounds = (vocab + round - 1) / round, each = (int)(((long long)rows * rounds + 4 * 148 - 1) / (4 * 148));
-    return BsShape{each * round, (rounds + each - 1) / each};
+    const int rounds = (vocab + BS_ROUND - 1) / BS_ROUND;
+    const long long fit = ((long long)rows * rounds + 4 * 148 - 1) / (4 * 148);
+    const int each = fit > BS_MAX_ROUNDS ? BS_MAX_ROUNDS : (int)fit;
+    return BsShape{each * BS_ROUND, (rounds + each - 1) / each};
 }
 
 }  // namespace vk
