@@ -114,18 +114,19 @@ __global__ void __launch_bounds__(SA_THREADS) attention_shared_kernel(const SaAr
     float* sq = reinterpret_cast<float*>(smem + sg_plan_bytes());
     float* sk = sq + SG_PREFIX_ROWS * a.hd;
     float* sv = sk + SG_KEYS * (a.hd + 4);
-    const int worker = blockIdx.x;
     sa_make_plan(a, p);                       // from the step's metadata, which no kernel writes
     dependency_wait();
     let_dependents_start();
     SaPart r;
-    int at = worker * p.lp, end = min(at + p.lp, p.pbase[SA_MAX_TOKENS]);
+    const bool prefix = (int)blockIdx.x < p.prefix_blocks;
+    const int worker = (int)blockIdx.x - (prefix ? 0 : p.prefix_blocks);
+    int at = worker * p.lp, end = prefix ? min(at + p.lp, p.pbase[SA_MAX_TOKENS]) : 0;
     while (at < end) {
         if (!sa_prefix_part(a, p, at, end, worker, r)) continue;
         sg_walk<T, DIMS>(a, p, r, false, sq, sk, sv);
     }
     at = worker * p.lo;
-    end = min(at + p.lo, p.obase[SA_MAX_TOKENS]);
+    end = prefix ? 0 : min(at + p.lo, p.obase[SA_MAX_TOKENS]);
     while (at < end) {
         int parts;
         if (!sa_own_part(a, p, at, end, worker, r, parts)) continue;
@@ -280,11 +281,20 @@ VK_API size_t vk_attention_shared_scratch_bytes(int tokens, int nh, int, int hd)
     return sa_part_rows(tokens, nh) * ((size_t)hd * 4 + 8) + (size_t)tokens * nh * 16;
 }
 
-// dtype 0 = float32, 1 = bfloat16.  scratch: vk_attention_shared_scratch_bytes(n, ...) bytes, whatever they hold.
-VK_API int vk_attention_shared(const void* q, const void* cache, const int32_t* block_tables, const int32_t* token_seg, const int32_t* positions,
-                               const int32_t* members, const int32_t* starts, const int32_t* shared, void* out, void* scratch, size_t scratch_bytes, int tokens, int segments,
-                               int n, int families, int pages, int nh, int nkv, int hd, int page_size, int max_blocks, float scale, int dtype,
-                               cudaStream_t stream) {
+// The arguments of vk_attention_shared, in one piece.  dtype 0 = float32, 1 = bfloat16.  scratch: vk_attention_shared_scratch_bytes(n, ...) bytes, whatever they hold.
+struct VkAttentionShared {
+    const void *q, *cache;
+    const int32_t *block_tables, *token_seg, *positions, *members, *starts, *shared;
+    void *out, *scratch;
+    uint64_t scratch_bytes;
+    int32_t tokens, segments, n, families, pages, nh, nkv, hd, page_size, max_blocks;
+    float scale;
+    int32_t dtype;
+};
+
+VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t stream) {
+    const auto [q, cache, block_tables, token_seg, positions, members, starts, shared, out, scratch, scratch_bytes, tokens, segments, n, families, pages, nh, nkv, hd, page_size,
+                max_blocks, scale, dtype] = *args;
     if (n <= 0 || families <= 0) return VK_OK;
     if (n > SA_MAX_TOKENS || families > SA_MAX_TOKENS || nkv > SA_MAX_KV_HEADS || hd > 256) return VK_TOO_LARGE;
     const int vec = dtype == 0 ? 4 : 8;
@@ -314,7 +324,8 @@ VK_API int vk_attention_shared(const void* q, const void* cache, const int32_t* 
         return status != VK_OK ? status : launch_join(a, dtype, stream);
     }
     a.prefix_rows = SG_PREFIX_ROWS;
-    a.prefix_workers = a.own_workers = sms;
+    a.blocks = sms;
+    a.own_per_block = 1;
     a.min_prefix = a.min_own = 4;
     a.prefix_cost = a.own_cost = 4;
     const size_t smem = sg_smem(hd);

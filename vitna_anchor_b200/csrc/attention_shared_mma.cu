@@ -29,7 +29,10 @@ template <int HD> struct SmSmem {
 };
 
 __device__ __forceinline__ uint32_t sm_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void sm_copy16(uint32_t dst, const void* src, bool there) {
+__device__ __forceinline__ void sm_copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void sm_copy16_or_zero(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void sm_ldsm4(uint32_t (&r)[4], uint32_t at) {
@@ -42,10 +45,87 @@ __device__ __forceinline__ void sm_mma(float* d, const uint32_t* a, uint32_t b0,
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t sm_turn(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t sm_pack(float x, float y) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+
+// Two weights as a high and a low pair of bfloat16: x = high + low to 2^-17.
+__device__ __forceinline__ void sm_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    hi = sm_pack(x, y);
+    lo = sm_pack(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+}
+
+// How a group of R warps brings tiles tile0, tile0 + step, ... of 16 R keys of a part into its place in the stages: every warp 16 keys of each.
+template <int HD, int R> struct SmCopy {
+    static constexpr int TK = SM_WARP_KEYS * R, CH = HD / 8, AT_ONCE = 32 / CH, PIECES = SM_WARP_KEYS / AT_ONCE;      // 16-byte pieces a row; rows and pieces a warp asks for at once
+    const SaArgs& a;
+    const SaPart& part;
+    const __nv_bfloat16* lane_src;      // this lane's piece of its row of a page's first AT_ONCE
+    uint32_t lane_dst, stages;          // where it goes in a stage
+    size_t to_values;                   // elements from a key to its value
+    int key, step_keys, mine;           // the warp's first key of tile 0, keys from one tile to the next, tiles
+    bool whole_pages;                   // sixteen keys lie in one page
+
+    __device__ __forceinline__ SmCopy(const SaArgs& a_, const SaPart& part_, int tile0, int step, int first_row, uint32_t stages_) : a(a_), part(part_), stages(stages_) {
+        const int lane = threadIdx.x & 31, row = lane / CH, piece = lane % CH;
+        const int tiles = (part.k1 - part.k0 + TK - 1) / TK;
+        mine = tile0 < tiles ? (tiles - tile0 + step - 1) / step : 0;
+        key = part.k0 + tile0 * TK + first_row % TK;
+        step_keys = step * TK;
+        whole_pages = a.page_size % SM_WARP_KEYS == 0 && part.k0 % SM_WARP_KEYS == 0;
+        to_values = (size_t)a.nkv * a.page_size * HD;
+        lane_src = static_cast<const __nv_bfloat16*>(a.cache) + row * HD + piece * 8;
+        lane_dst = (first_row + row) * (HD * 2) + ((piece ^ row) << 4);
+    }
+    // The page of key `lane % 16` of this warp's keys of the n-th tile; none: -1.  Only asked for: what hangs on it is worked out a tile later, so that nobody waits for it.
+    __device__ __forceinline__ int page_of(int n) const {
+        const int k = key + n * step_keys + (threadIdx.x & 15);
+        return n < mine && k < part.k1 ? part.table[a.page_shift >= 0 ? k >> a.page_shift : k / a.page_size] : -1;
+    }
+    // The row of the pool that holds the key; none: ~0.
+    __device__ __forceinline__ uint32_t row_of(int n, int page) const {
+        const int k = key + n * step_keys + (threadIdx.x & 15), block = a.page_shift >= 0 ? k >> a.page_shift : k / a.page_size;
+        return (uint32_t)page < (uint32_t)a.pages ? ((uint32_t)page * 2u * a.nkv + part.kvh) * a.page_size + (k - block * a.page_size) : 0xffffffffu;
+    }
+    __device__ __forceinline__ void issue(int n, int page) const {
+        if (n < mine) {
+            const uint32_t rows = row_of(n, page);
+            const uint32_t stage = stages + (n % SM_STAGES) * SmSmem<HD>::STAGE;
+            const uint32_t first = __shfl_sync(0xffffffffu, rows, 0);
+            if (whole_pages && key + n * step_keys + SM_WARP_KEYS <= part.k1 && first != 0xffffffffu) {      // sixteen neighbouring rows
+                const __nv_bfloat16* src = lane_src + (size_t)first * HD;
+                const __nv_bfloat16* val = src + to_values;
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) {
+                    const uint32_t dst = stage + (lane_dst ^ ((i * AT_ONCE & 7) << 4)) + i * AT_ONCE * HD * 2;
+                    sm_copy16(dst, src + i * AT_ONCE * HD);
+                    sm_copy16(dst + SmSmem<HD>::HALF, val + i * AT_ONCE * HD);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) {
+                    const uint32_t row = __shfl_sync(0xffffffffu, rows, i * AT_ONCE + (threadIdx.x & 31) / CH);
+                    const bool there = row != 0xffffffffu;
+                    const __nv_bfloat16* src = lane_src + ((there ? (size_t)row : 0) - (threadIdx.x & 31) / CH) * HD;
+                    const uint32_t dst = stage + (lane_dst ^ ((i * AT_ONCE & 7) << 4)) + i * AT_ONCE * HD * 2;
+                    sm_copy16_or_zero(dst, there ? src : static_cast<const __nv_bfloat16*>(a.cache), there);
+                    sm_copy16_or_zero(dst + SmSmem<HD>::HALF, there ? src + to_values : static_cast<const __nv_bfloat16*>(a.cache), there);
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+};
+
+// A row's reference: scores count as 2^(score - reference), and the reference is moved to the largest score so far only when one is more than 8 above it: a weight
+// is at most 2^8, float32 has room for that, and most tiles need no maximum over the row's lanes.
+constexpr float SM_AHEAD = 8.0f;
 
 // What a warp has of its 16 rows: lane (gq, qd) = (lane / 4, lane % 4) rows gq and gq + 8, dims 8 b + 2 qd and the next; the sums over this lane's keys alone.
 template <int HD> struct SmRows {
@@ -57,51 +137,23 @@ template <int HD> struct SmRows {
 template <int HD, int R>
 __device__ __forceinline__ void sm_walk(const SaArgs& a, const SaPart& part, int tile0, int step, int group, int wr, const uint32_t (&qf)[HD / 16][4], SmRows<HD>& x, uint32_t stages) {
     constexpr int TK = SM_WARP_KEYS * R, CH = HD / 8, SUB = R == 1 ? 16 : 32, NB = SUB / 8;
-    const int lane = threadIdx.x & 31;
-    const __nv_bfloat16* cache = static_cast<const __nv_bfloat16*>(a.cache);
-    const uint32_t v_rows = (uint32_t)a.nkv * a.page_size;
-    const int tiles = (part.k1 - part.k0 + TK - 1) / TK, mine = tile0 < tiles ? (tiles - tile0 + step - 1) / step : 0;
-    const int base_row = group * TK;
+    const int lane = threadIdx.x & 31, base_row = group * TK;
+    const SmCopy<HD, R> copy(a, part, tile0, step, base_row + wr * SM_WARP_KEYS, stages);
+    const float scale = a.scale_log2;
 #pragma unroll
     for (int b = 0; b < HD / 8; b++) { x.o[b][0] = x.o[b][1] = x.o[b][2] = x.o[b][3] = 0.0f; }
     x.m[0] = x.m[1] = -INFINITY;
     x.l[0] = x.l[1] = 0.0f;
-
-    // the row of the pool that holds key `lane % 16` of this warp's keys of the n-th tile; none: ~0
-    auto row_of = [&](int n) -> uint32_t {
-        const int key = part.k0 + (tile0 + n * step) * TK + wr * SM_WARP_KEYS + (lane & 15);
-        if (n >= mine || key >= part.k1) return 0xffffffffu;
-        const int block = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
-        const int page = part.table[block];
-        if ((uint32_t)page >= (uint32_t)a.pages) return 0xffffffffu;
-        return ((uint32_t)page * 2u * a.nkv + part.kvh) * a.page_size + (key - block * a.page_size);
-    };
-    auto issue = [&](int n, uint32_t rows) {
-        if (n < mine) {
-            const uint32_t stage = stages + (n % SM_STAGES) * SmSmem<HD>::STAGE;
-#pragma unroll
-            for (int i = 0; i < SM_WARP_KEYS * CH / 32; i++) {
-                const int c = i * 32 + lane, kl = c / CH, piece = c % CH;
-                const uint32_t row = __shfl_sync(0xffffffffu, rows, kl);
-                const bool there = row != 0xffffffffu;
-                const __nv_bfloat16* src = cache + (there ? (size_t)row * HD + piece * 8 : 0);
-                const uint32_t dst = stage + ((base_row + wr * SM_WARP_KEYS + kl) * CH + (piece ^ (kl & 7))) * 16;
-                sm_copy16(dst, src, there);
-                sm_copy16(dst + SmSmem<HD>::HALF, there ? src + (size_t)v_rows * HD : src, there);
-            }
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
-    issue(0, row_of(0));
-    issue(1, row_of(1));
-    uint32_t rows = row_of(2);
-    for (int n = 0; n < mine; n++) {
+    const int page0 = copy.page_of(0), page1 = copy.page_of(1);
+    int page = copy.page_of(2);
+    copy.issue(0, page0);
+    copy.issue(1, page1);
+    for (int n = 0; n < copy.mine; n++) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         if (R == 1) __syncwarp();
         else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(R * 32) : "memory");
-        issue(n + 2, rows);                                // into the stage of the tile before, which the whole group is past
-        rows = row_of(n + 3);
+        copy.issue(n + 2, page);                           // into the stage of the tile before, which the whole group is past
+        page = copy.page_of(n + 3);
         const uint32_t sk = stages + (n % SM_STAGES) * SmSmem<HD>::STAGE, sv = sk + SmSmem<HD>::HALF;
         const int key0 = part.k0 + (tile0 + n * step) * TK;
 #pragma unroll 1                                           // four copies of the body would not stay in the instruction cache
@@ -120,25 +172,27 @@ __device__ __forceinline__ void sm_walk(const SaArgs& a, const SaPart& part, int
                     sm_mma(s[nb], qf[ks], b[0], b[1]);
                     sm_mma(s[nb + 1], qf[ks], b[2], b[3]);
                 }
-            const bool edge = key0 + sub + SUB > part.k1;
-            float top[2] = {x.m[0], x.m[1]};
+            if (key0 + sub + SUB > part.k1) {
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
+                for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float v = s[nb][e] * a.scale_log2;
-                    if (edge && key0 + sub + nb * 8 + (lane & 3) * 2 + (e & 1) >= part.k1) v = -INFINITY;
-                    s[nb][e] = v;
-                    top[e >> 1] = fmaxf(top[e >> 1], v);
-                }
+                    for (int e = 0; e < 4; e++)
+                        if (key0 + sub + nb * 8 + (lane & 3) * 2 + (e & 1) >= part.k1) s[nb][e] = -INFINITY;
+            }
+            float top[2];
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+                top[r] = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
+#pragma unroll
+                for (int nb = 1; nb < NB; nb++) top[r] = fmaxf(top[r], fmaxf(s[nb][2 * r], s[nb][2 * r + 1]));
+                top[r] *= scale;
             }
-            if (__any_sync(0xffffffffu, top[0] > x.m[0] || top[1] > x.m[1])) {
+            if (__any_sync(0xffffffffu, top[0] > x.m[0] + SM_AHEAD || top[1] > x.m[1] + SM_AHEAD)) {
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
+                    top[r] = fmaxf(x.m[r], top[r]);
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
                     const float keep = top[r] == -INFINITY ? 0.0f : sa_ex2(x.m[r] - top[r]);
                     x.l[r] *= keep;
 #pragma unroll
@@ -152,11 +206,9 @@ __device__ __forceinline__ void sm_walk(const SaArgs& a, const SaPart& part, int
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    const float p0 = sa_ex2(s[nb][2 * r] - ref[r]), p1 = sa_ex2(s[nb][2 * r + 1] - ref[r]);
+                    const float p0 = sa_ex2(fmaf(s[nb][2 * r], scale, -ref[r])), p1 = sa_ex2(fmaf(s[nb][2 * r + 1], scale, -ref[r]));
                     x.l[r] += p0 + p1;
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-                    ph[nb >> 1][(nb & 1) * 2 + r] = *reinterpret_cast<const uint32_t*>(&h);
-                    pl[nb >> 1][(nb & 1) * 2 + r] = sm_pack(p0 - __bfloat162float(h.x), p1 - __bfloat162float(h.y));
+                    sm_split(p0, p1, ph[nb >> 1][(nb & 1) * 2 + r], pl[nb >> 1][(nb & 1) * 2 + r]);
                 }
 #pragma unroll
             for (int kk = 0; kk < NB / 2; kk++)
@@ -179,6 +231,98 @@ __device__ __forceinline__ void sm_walk(const SaArgs& a, const SaPart& part, int
     }
 }
 
+// The same for at most eight rows, with the keys as the 16 rows of the products: S^T = K Q^T, and O^T = V^T P^T with the weights turned over in registers
+// (movmatrix).  Half the products and half the exponentials.  Lane (gq, qd): rows 2 qd and 2 qd + 1, dims 16 b + gq and + 8; the sums over this lane's keys alone.
+template <int HD> struct SmFew {
+    float o[HD / 16][4], m[2], l[2];
+};
+template <int HD>
+__device__ __forceinline__ void sm_walk_few(const SaArgs& a, const SaPart& part, int tile0, int step, int warp, const uint32_t (&qb)[HD / 16][2], SmFew<HD>& x, uint32_t stages) {
+    constexpr int CH = HD / 8;
+    const int lane = threadIdx.x & 31, base_row = warp * SM_WARP_KEYS;
+    const SmCopy<HD, 1> copy(a, part, tile0, step, base_row, stages);
+    const float scale = a.scale_log2;
+#pragma unroll
+    for (int b = 0; b < HD / 16; b++) { x.o[b][0] = x.o[b][1] = x.o[b][2] = x.o[b][3] = 0.0f; }
+    x.m[0] = x.m[1] = -INFINITY;
+    x.l[0] = x.l[1] = 0.0f;
+    const uint32_t at_k = ((base_row + (lane & 15)) * CH) * 16, at_v = ((base_row + (lane & 7) + ((lane >> 4) << 3)) * CH) * 16;      // this lane's rows for ldmatrix
+    const int page0 = copy.page_of(0), page1 = copy.page_of(1);
+    int page = copy.page_of(2);
+    copy.issue(0, page0);
+    copy.issue(1, page1);
+    for (int n = 0; n < copy.mine; n++) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        copy.issue(n + 2, page);
+        page = copy.page_of(n + 3);
+        const uint32_t sk = stages + (n % SM_STAGES) * SmSmem<HD>::STAGE, sv = sk + SmSmem<HD>::HALF;
+        const int key0 = part.k0 + (tile0 + n * step) * SM_WARP_KEYS;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ks++) {
+            uint32_t k[4];
+            sm_ldsm4(k, sk + at_k + (((ks * 2 + (lane >> 4)) ^ (lane & 7)) << 4));
+            sm_mma(s, k, qb[ks][0], qb[ks][1]);
+        }
+        if (key0 + SM_WARP_KEYS > part.k1) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (key0 + (lane >> 2) + (e >> 1) * 8 >= part.k1) s[e] = -INFINITY;
+        }
+        float top[2] = {fmaxf(s[0], s[2]) * scale, fmaxf(s[1], s[3]) * scale};
+        if (__any_sync(0xffffffffu, top[0] > x.m[0] + SM_AHEAD || top[1] > x.m[1] + SM_AHEAD)) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                top[h] = fmaxf(x.m[h], top[h]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+                const float keep = top[h] == -INFINITY ? 0.0f : sa_ex2(x.m[h] - top[h]);
+                x.l[h] *= keep;
+#pragma unroll
+                for (int b = 0; b < HD / 16; b++) { x.o[b][h] *= keep; x.o[b][2 + h] *= keep; }
+                x.m[h] = top[h];
+            }
+        }
+        const float ref[2] = {x.m[0] == -INFINITY ? 0.0f : x.m[0], x.m[1] == -INFINITY ? 0.0f : x.m[1]};
+        uint32_t ph[2], pl[2];
+#pragma unroll
+        for (int half = 0; half < 2; half++) {             // keys gq and gq + 8
+            const float p0 = sa_ex2(fmaf(s[2 * half], scale, -ref[0])), p1 = sa_ex2(fmaf(s[2 * half + 1], scale, -ref[1]));
+            x.l[0] += p0;
+            x.l[1] += p1;
+            uint32_t hi, lo;
+            sm_split(p0, p1, hi, lo);
+            ph[half] = sm_turn(hi);                        // [key][rows 2 qd, 2 qd + 1] -> [row][keys 2 qd, 2 qd + 1]
+            pl[half] = sm_turn(lo);
+        }
+#pragma unroll
+        for (int b = 0; b < HD / 16; b++) {
+            uint32_t v[4];
+            sm_ldsm4_trans(v, sv + at_v + (((b * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+            sm_mma(x.o[b], v, ph[0], ph[1]);
+            sm_mma(x.o[b], v, pl[0], pl[1]);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) x.l[h] += __shfl_xor_sync(0xffffffffu, x.l[h], d);
+}
+
+// The queries of up to eight rows of a part as the 8-column operand: lane (gq, qd) has row gq, dims 2 qd, the next and + 8 of each k step.
+template <int HD>
+__device__ __forceinline__ void sm_queries_few(const SaArgs& a, const SaPlan& p, const SaPart& part, uint32_t (&qb)[HD / 16][2]) {
+    const int lane = threadIdx.x & 31, rows = (part.i1 - part.i0) * part.heads, row = lane >> 2, i = part.i0 + row / part.heads;
+    const bool on = row < rows && p.pos[min(i, SA_MAX_TOKENS - 1)] >= 0;
+    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (on ? ((size_t)p.tok[i] * a.nh + part.kvh * a.gq + part.h0 + row % part.heads) * HD : 0) + 2 * (lane & 3);
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ks++) {
+        qb[ks][0] = on ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
+        qb[ks][1] = on ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
+    }
+}
+
 // The queries of rows row0 + gq and row0 + gq + 8 of a part as the 16-row operand (zeros where there is no such row, or its member is not there).
 template <int HD>
 __device__ __forceinline__ void sm_queries(const SaArgs& a, const SaPlan& p, const SaPart& part, int row0, uint32_t (&qf)[HD / 16][4]) {
@@ -196,41 +340,16 @@ __device__ __forceinline__ void sm_queries(const SaArgs& a, const SaPlan& p, con
     }
 }
 
-// A block's part of a family's prefix: 8 / R groups of R warps; their outputs meet in shared memory and the part's rows are written.
+// The outputs that a block's groups of R warps left in shared memory ([8 warps][16][HD + 4], maxima and sums behind them) meet, and the part's rows are written.
 template <int HD, int R>
-__device__ __forceinline__ void sm_prefix(const SaArgs& a, const SaPlan& p, const SaPart& part, unsigned char* stages) {
+__device__ __forceinline__ void sm_meet(const SaArgs& a, const SaPart& part, const unsigned char* stages) {
     constexpr int GROUPS = (SA_THREADS / 32) / R, LD = HD + 4;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp / R, wr = warp % R;
+    const float* out = reinterpret_cast<const float*>(stages);
+    const float2 (*ml)[16] = reinterpret_cast<const float2 (*)[16]>(stages + SmSmem<HD>::OUT);
     const int rows = (part.i1 - part.i0) * part.heads;
-    uint32_t qf[HD / 16][4];
-    sm_queries<HD>(a, p, part, wr * 16, qf);
-    SmRows<HD> x;
-    sm_walk<HD, R>(a, part, group, GROUPS, group, wr, qf, x, sm_addr(stages));
-    if (GROUPS == 1) {
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int row = wr * 16 + (lane >> 2) + 8 * r;
-            if (row >= rows) continue;
-            const int at = part.row0 + row * part.stride;
-#pragma unroll
-            for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(a.part_o + (size_t)at * HD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
-            if ((lane & 3) == 0) a.part_ml[at] = make_float2(x.m[r], x.l[r]);
-        }
-        return;
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();                                       // every group is past its tiles
-    float* out = reinterpret_cast<float*>(stages);         // [8 warps][16][LD]
-    float2 (*ml)[16] = reinterpret_cast<float2 (*)[16]>(stages + SmSmem<HD>::OUT);
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int row = (lane >> 2) + 8 * r;
-#pragma unroll
-        for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(out + (warp * 16 + row) * LD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
-        if ((lane & 3) == 0) ml[warp][row] = make_float2(x.m[r], x.l[r]);
-    }
     __syncthreads();
-    for (int c = tid; c < rows * (HD / 4); c += SA_THREADS) {
+#pragma unroll 1
+    for (int c = threadIdx.x; c < rows * (HD / 4); c += SA_THREADS) {
         const int row = c / (HD / 4), d = c % (HD / 4) * 4, w0 = row / 16, rr = row % 16;
         float m = -INFINITY;
 #pragma unroll
@@ -252,6 +371,75 @@ __device__ __forceinline__ void sm_prefix(const SaArgs& a, const SaPlan& p, cons
     }
 }
 
+// A block's part of a family's prefix: 8 / R groups of R warps; their outputs meet in shared memory and the part's rows are written.
+template <int HD, int R>
+__device__ __forceinline__ void sm_prefix(const SaArgs& a, const SaPlan& p, const SaPart& part, unsigned char* stages) {
+    constexpr int GROUPS = (SA_THREADS / 32) / R, LD = HD + 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / R, wr = warp % R;
+    const int rows = (part.i1 - part.i0) * part.heads;
+    uint32_t qf[HD / 16][4];
+    sm_queries<HD>(a, p, part, wr * 16, qf);
+    SmRows<HD> x;
+    sm_walk<HD, R>(a, part, group, GROUPS, group, wr, qf, x, sm_addr(stages));
+    if (GROUPS == 1) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int row = wr * 16 + (lane >> 2) + 8 * r;
+            if (row >= rows) continue;
+            const int at = part.row0 + row * part.stride;
+#pragma unroll
+            for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(a.part_o + (size_t)at * HD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
+            if ((lane & 3) == 0) a.part_ml[at] = make_float2(x.m[r], x.l[r]);
+        }
+        return;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                                       // every group is past its tiles
+    float* out = reinterpret_cast<float*>(stages);
+    float2 (*ml)[16] = reinterpret_cast<float2 (*)[16]>(stages + SmSmem<HD>::OUT);
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int row = (lane >> 2) + 8 * r;
+#pragma unroll
+        for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(out + (warp * 16 + row) * LD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
+        if ((lane & 3) == 0) ml[warp][row] = make_float2(x.m[r], x.l[r]);
+    }
+    sm_meet<HD, R>(a, part, stages);
+}
+
+// The same of at most eight rows: every warp by itself.
+template <int HD>
+__device__ __forceinline__ void sm_prefix_few(const SaArgs& a, const SaPlan& p, const SaPart& part, unsigned char* stages) {
+    constexpr int LD = HD + 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t qb[HD / 16][2];
+    sm_queries_few<HD>(a, p, part, qb);
+    SmFew<HD> x;
+    sm_walk_few<HD>(a, part, warp, SA_THREADS / 32, warp, qb, x, sm_addr(stages));
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    float* out = reinterpret_cast<float*>(stages);
+    float2 (*ml)[16] = reinterpret_cast<float2 (*)[16]>(stages + SmSmem<HD>::OUT);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int row = 2 * (lane & 3) + h;
+#pragma unroll
+        for (int b = 0; b < HD / 16; b++) {
+            out[(warp * 16 + row) * LD + b * 16 + (lane >> 2)] = x.o[b][h];
+            out[(warp * 16 + row) * LD + b * 16 + (lane >> 2) + 8] = x.o[b][2 + h];
+        }
+        if (lane < 4) ml[warp][row] = make_float2(x.m[h], x.l[h]);
+    }
+    sm_meet<HD, 1>(a, part, stages);
+}
+
+// What a warp's walk of an own part leaves: the result where the unit needs nobody else, else the part's row.
+template <int HD>
+__device__ __forceinline__ void sm_leave(const SaArgs& a, const SaPlan& p, const SaPart& part, bool alone, int row, int d, float x, float y) {
+    if (alone) *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + ((size_t)p.tok[part.i0] * a.nh + part.kvh * a.gq + part.h0 + row) * HD + d) = sm_pack(x, y);
+    else *reinterpret_cast<float2*>(a.part_o + (size_t)(part.row0 + row * part.stride) * HD + d) = make_float2(x, y);
+}
+
 template <int HD>
 __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared_mma_kernel(const SaArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -262,59 +450,73 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
     dependency_wait();
     let_dependents_start();
     SaPart part;
-    int at = blockIdx.x * p.lp, end = min(at + p.lp, p.pbase[SA_MAX_TOKENS]);
+    const bool prefix = (int)blockIdx.x < p.prefix_blocks;
+    int at = blockIdx.x * p.lp, end = prefix ? min(at + p.lp, p.pbase[SA_MAX_TOKENS]) : 0;
     while (at < end) {
         if (!sa_prefix_part(a, p, at, end, blockIdx.x, part)) continue;
         const int rows = (part.i1 - part.i0) * part.heads;
-        if (rows <= 16) sm_prefix<HD, 1>(a, p, part, stages);
+        if (rows <= 8) sm_prefix_few<HD>(a, p, part, stages);
+        else if (rows <= 16) sm_prefix<HD, 1>(a, p, part, stages);
         else if (rows <= 32) sm_prefix<HD, 2>(a, p, part, stages);
         else if (rows <= 64) sm_prefix<HD, 4>(a, p, part, stages);
         else sm_prefix<HD, 8>(a, p, part, stages);
         __syncthreads();
     }
-    // from here on every warp is by itself: neighbouring parts of the own keys go to different multiprocessors, first to those without a part of a prefix
-    const int worker = warp * gridDim.x + gridDim.x - 1 - blockIdx.x;
+    // every warp by itself; neighbouring parts of the own keys go to different multiprocessors
+    const int worker = prefix ? 0 : warp * ((int)gridDim.x - p.prefix_blocks) + (int)blockIdx.x - p.prefix_blocks;
     at = worker * p.lo;
-    end = min(at + p.lo, p.obase[SA_MAX_TOKENS]);
+    end = prefix ? 0 : min(at + p.lo, p.obase[SA_MAX_TOKENS]);
     while (at < end) {
         int parts;
         if (!sa_own_part(a, p, at, end, worker, part, parts)) continue;
         const bool alone = parts == 1 && p.shared[part.g] == 0;      // the unit needs nobody else
-        uint32_t qf[HD / 16][4];
-        sm_queries<HD>(a, p, part, 0, qf);
-        SmRows<HD> x;
         __syncwarp();                                      // the lanes are past the tiles of the part before
-        sm_walk<HD, 1>(a, part, 0, 1, warp, 0, qf, x, sm_addr(stages));
+        if (part.heads <= 8) {
+            uint32_t qb[HD / 16][2];
+            sm_queries_few<HD>(a, p, part, qb);
+            SmFew<HD> x;
+            sm_walk_few<HD>(a, part, 0, 1, warp, qb, x, sm_addr(stages));
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int row = (lane >> 2) + 8 * r;
-            if (row >= part.heads) continue;
-            if (alone) {
-                __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + ((size_t)p.tok[part.i0] * a.nh + part.kvh * a.gq + part.h0 + row) * HD + 2 * (lane & 3);
-                const float w = 1.0f / x.l[r];
+            for (int h = 0; h < 2; h++) {
+                const int row = 2 * (lane & 3) + h, gq = lane >> 2;
+                const float w = alone ? 1.0f / x.l[h] : 1.0f;
 #pragma unroll
-                for (int b = 0; b < HD / 8; b++) *reinterpret_cast<uint32_t*>(out + b * 8) = sm_pack(x.o[b][2 * r] * w, x.o[b][2 * r + 1] * w);
-            } else {
-                const int to = part.row0 + row * part.stride;
+                for (int b = 0; b < HD / 16; b++) {        // neighbouring dims lie in neighbouring lanes' registers: even lanes take the lower eight, odd ones the upper
+                    const float lo = x.o[b][h] * w, up = x.o[b][2 + h] * w;
+                    const float got = __shfl_xor_sync(0xffffffffu, gq & 1 ? lo : up, 4);
+                    if (row < part.heads) sm_leave<HD>(a, p, part, alone, row, b * 16 + (gq & 1 ? 8 + gq - 1 : gq), gq & 1 ? got : lo, gq & 1 ? up : got);
+                }
+                if (!alone && lane < 4 && row < part.heads) a.part_ml[part.row0 + row * part.stride] = make_float2(x.m[h], x.l[h]);
+            }
+        } else {
+            uint32_t qf[HD / 16][4];
+            sm_queries<HD>(a, p, part, 0, qf);
+            SmRows<HD> x;
+            sm_walk<HD, 1>(a, part, 0, 1, warp, 0, qf, x, sm_addr(stages));
 #pragma unroll
-                for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(a.part_o + (size_t)to * HD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
-                if ((lane & 3) == 0) a.part_ml[to] = make_float2(x.m[r], x.l[r]);
+            for (int r = 0; r < 2; r++) {
+                const int row = (lane >> 2) + 8 * r;
+                if (row >= part.heads) continue;
+                const float w = alone ? 1.0f / x.l[r] : 1.0f;
+#pragma unroll
+                for (int b = 0; b < HD / 8; b++) sm_leave<HD>(a, p, part, alone, row, b * 8 + 2 * (lane & 3), x.o[b][2 * r] * w, x.o[b][2 * r + 1] * w);
+                if (!alone && (lane & 3) == 0) a.part_ml[part.row0 + row * part.stride] = make_float2(x.m[r], x.l[r]);
             }
         }
     }
     sa_write_rows(a, p);
 }
 
-// Rows of the pool are counted in 32 bits here.
+// Rows of the pool are counted in 32 bits here, and a row's largest score is that of its largest product.
 bool attention_shared_mma_takes(const SaArgs& a, int dtype) {
-    return dtype == 1 && (a.hd == 64 || a.hd == 128) && (long long)a.pages * 2 * a.nkv * a.page_size < 0x7fffffffLL;
+    return dtype == 1 && (a.hd == 64 || a.hd == 128) && a.scale_log2 > 0.0f && (long long)a.pages * 2 * a.nkv * a.page_size < 0x7fffffffLL;
 }
 
 int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream) {
     a.prefix_rows = SM_PREFIX_ROWS;
     const int blocks = multiprocessors * (a.hd == 64 ? 2 : 1);
-    a.prefix_workers = blocks;
-    a.own_workers = blocks * (SA_THREADS / 32);
+    a.blocks = blocks;
+    a.own_per_block = SA_THREADS / 32;
     a.min_prefix = 8;
     a.min_own = 4;
     a.prefix_cost = 16;

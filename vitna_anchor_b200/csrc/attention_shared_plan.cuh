@@ -7,10 +7,11 @@
 //            family's shared keys [0, P); P is at most the smallest position of its members, and 0 for a family of one
 //   own      one member's heads (up to OWN_ROWS of them) over the keys [P, position] that only it reads
 //
-// The prefix units, each as its tiles of 16 keys and a number of empty tiles that stands for what a unit costs besides its keys, lie one after
-// the other on a line; worker b walks the tiles [b lp, (b+1) lp) of it.  The own units lie on another line with workers and a length lo of their
-// own.  So every worker has the same to do whatever the families look like, a unit is cut into at most tiles / l + 2 parts, and a part's place among its
-// unit's parts is the worker's number minus that of the unit's first worker.  A part leaves an unnormalised output, a
+// The launch's blocks are divided between the two by what they have to do, so that a block walks one kind only: what limits the prefixes of large families (products) and what limits
+// the own keys (memory) is then busy at the same time, and where there is little to do neither waits for the other.  The prefix units, each as its tiles of 16 keys and a number of
+// empty tiles that stands for what a unit costs besides its keys, lie one after the other on a line; worker b walks the tiles [b lp, (b+1) lp) of it.  The own units lie on another
+// line with workers and a length lo of their own.  So every worker has the same to do whatever the families look like, a unit is cut into at most tiles / l + 2 parts, and a part's
+// place among its unit's parts is the worker's number minus that of the unit's first worker.  A part leaves an unnormalised output, a
 // maximum and a sum for each of its rows, and a second launch joins a row's parts.
 //
 // Lengths are read from the step's metadata on the device, so that a captured graph follows them.
@@ -36,7 +37,7 @@ struct SaArgs {
     float2* part_ml;               // [rows] maximum (base 2) and sum
     float* part_o;                 // [rows][hd]
     int n, families, tokens, segments, pages, nh, nkv, gq, hd, page_size, page_shift, max_blocks;
-    int prefix_rows, prefix_workers, own_workers, min_prefix, min_own, prefix_cost, own_cost;      // the last four in tiles of keys
+    int prefix_rows, blocks, own_per_block, min_prefix, min_own, prefix_cost, own_cost;      // own workers a block; the last four in tiles of keys
     float scale_log2;
 };
 
@@ -45,12 +46,14 @@ struct SaRow { int prefix_row, prefix_parts, own_row, own_parts; };
 
 struct SaPlan {
     int pbase[SA_MAX_TOKENS + 1], obase[SA_MAX_TOKENS + 1];            // where a family's, a member's units begin on their line, in tiles
-    int start[SA_MAX_TOKENS + 1], first[SA_MAX_TOKENS], shared[SA_MAX_TOKENS];
+    __align__(16) int start[SA_MAX_TOKENS + 4];
+    int begin[SA_MAX_TOKENS], width[SA_MAX_TOKENS], first[SA_MAX_TOKENS], shared[SA_MAX_TOKENS];      // of a family: its members, the first that is there, P; start: as given
     int prow[SA_MAX_TOKENS], orow[SA_MAX_TOKENS];                      // where their parts' rows begin
     int tok[SA_MAX_TOKENS], seg[SA_MAX_TOKENS], pos[SA_MAX_TOKENS], grp[SA_MAX_TOKENS];    // of a member; pos -1: not there
     int count[SA_MAX_TOKENS], least[SA_MAX_TOKENS];
-    int lp, lo, tile_members, own_tiles;
-    int scan[2][SA_THREADS / 32];
+    int lp, lo, prefix_blocks, tile_members, own_tiles;
+    float weight[SA_THREADS / 32];
+    int scan[2][2][SA_THREADS / 32];
 };
 
 constexpr int SA_TILE = 16;            // keys: a part's products are whole
@@ -58,7 +61,7 @@ __device__ __forceinline__ int sa_tiles(int keys) { return (keys + SA_TILE - 1) 
 // The most parts that a unit of `keys` keys is cut into.
 __device__ __forceinline__ int sa_parts(int keys, int length) { return (sa_tiles(keys) + length - 1) / length + 1; }
 
-// Exclusive scans of two numbers a thread over the block; both totals to every thread.
+// Exclusive scans of two numbers a thread over the block; both totals to every thread.  `warps` is this scan's own.  One barrier.
 __device__ __forceinline__ void sa_scan2(int (*warps)[SA_THREADS / 32], int& a, int& b, int& ta, int& tb) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int x = a, y = b;
@@ -67,16 +70,16 @@ __device__ __forceinline__ void sa_scan2(int (*warps)[SA_THREADS / 32], int& a, 
         const int u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
         if (lane >= o) { x += u; y += v; }
     }
-    __syncthreads();
     if (lane == 31) { warps[0][warp] = x; warps[1][warp] = y; }
     __syncthreads();
     int px = 0, py = 0;
     ta = tb = 0;
 #pragma unroll
     for (int w = 0; w < SA_THREADS / 32; w++) {
-        if (w < warp) { px += warps[0][w]; py += warps[1][w]; }
-        ta += warps[0][w];
-        tb += warps[1][w];
+        const int u = warps[0][w], v = warps[1][w];
+        if (w < warp) { px += u; py += v; }
+        ta += u;
+        tb += v;
     }
     a = px + x - a;
     b = py + y - b;
@@ -95,70 +98,81 @@ __device__ __forceinline__ int sa_find(const int* base, int n, int at) {
 // Filled by all SA_THREADS threads of a block.  Numbers that cannot be (a member beyond the batch, a negative position, starts
 // that go back) are taken as members that are not there and runs of no length: nothing is read or written for them.
 __device__ __forceinline__ void sa_make_plan(const SaArgs& a, SaPlan& p) {
-    const int i = threadIdx.x, lane = i & 31, warp = i >> 5;
-    // starts, made to ascend: a running maximum
-    int s = i < a.families ? min(max(a.starts[i], 0), a.n) : 0;
+    const int i = threadIdx.x, lane = i & 31;
     const int token = i < a.n ? a.members[i] : -1;
-    const int shared_i = i < a.families ? a.shared[i] : 0;
+    const int shared_i = i < a.families ? a.shared[i] : 0, start_i = i <= a.families ? a.starts[i] : 0;
     const bool there = token >= 0 && token < a.tokens;
-    const int seg = there ? a.token_seg[token] : -1;
-    int pos = there && seg >= 0 && seg < a.segments ? a.positions[token] : -1;
-    pos = (int)min((long long)pos, (long long)a.max_blocks * a.page_size - 1);
+    const int seg = there ? a.token_seg[token] : -1, at = there ? a.positions[token] : -1;
+    p.start[i] = start_i;                   // zeros behind the last, so that groups of four count no more
+    if (i < 4) p.start[SA_MAX_TOKENS + i] = a.families == SA_MAX_TOKENS && i == 0 ? a.starts[SA_MAX_TOKENS] : 0;
+    p.shared[i] = shared_i;
     p.tok[i] = token;
-    p.seg[i] = seg;
-    p.pos[i] = pos;
-    p.count[i] = 0;
-    p.first[i] = SA_MAX_TOKENS;
+    p.count[i] = p.width[i] = 0;
+    p.begin[i] = p.first[i] = SA_MAX_TOKENS;
     p.least[i] = 0x7fffffff;
-    int* tops = p.scan[0];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s = max(s, v);
-    }
-    if (lane == 31) tops[warp] = s;
-    __syncthreads();
-    for (int w = 0; w < warp; w++) s = max(s, tops[w]);
-    if (i < a.families) p.start[i] = s;
-    if (i == a.families - 1) p.start[a.families] = max(s, min(a.starts[a.families], a.n));
-    __syncthreads();
-    int g = -1;
-    if (pos >= 0 && i >= p.start[0] && i < p.start[a.families]) {        // the last family that begins at or before the member
-        int lo = 0, hi = a.families;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (p.start[mid] <= i) lo = mid; else hi = mid;
-        }
-        g = lo;
-        atomicAdd(&p.count[g], 1);
-        atomicMin(&p.first[g], i);
-        atomicMin(&p.least[g], pos);
-    }
-    p.grp[i] = g;
     if (i == 0) {
         p.tile_members = a.prefix_rows / a.gq;
         p.own_tiles = (a.gq + SA_OWN_ROWS - 1) / SA_OWN_ROWS;
     }
     __syncthreads();
-    const int P = i < a.families && p.count[i] > 1 ? max(0, min(shared_i, p.least[i])) : 0;
-    p.shared[i] = P;
-    const int width = i < a.families ? p.start[i + 1] - p.start[i] : 0;
-    const int tiles = (width + p.tile_members - 1) / p.tile_members;
+    // the member's family: as many as begin at or before it, the first aside (so families are runs of members even where starts go back); none: before the
+    // first or behind all
+    int before = 0, behind = 0;
+    if (i < a.n) {
+#pragma unroll 2
+        for (int k = 0; k <= a.families; k += 4) {
+            const int4 f = *reinterpret_cast<const int4*>(p.start + k);
+            behind |= (f.x > i) | (f.y > i) | (f.z > i) | (f.w > i);
+            before += (f.x <= i) + (f.y <= i) + (f.z <= i) + (f.w <= i);
+        }
+        before -= (a.families / 4 + 1) * 4 - (a.families + 1) + (p.start[a.families] <= i);      // without the zeros, and the end
+    }
+    const int g = i < a.n && p.start[0] <= i && behind ? before - 1 : -1;
+    const bool valid = g >= 0 && seg >= 0 && seg < a.segments && at >= 0;
+    const int pos = valid ? (int)min((long long)at, (long long)a.max_blocks * a.page_size - 1) : -1;
+    p.seg[i] = seg;
+    p.pos[i] = pos;
+    p.grp[i] = valid ? g : -1;
+    {   // a family's neighbours in the warp count together
+        const unsigned same = __match_any_sync(0xffffffffu, g), live = __ballot_sync(0xffffffffu, valid) & same;
+        const int least = __reduce_min_sync(same, valid ? pos : 0x7fffffff);
+        if (g >= 0 && lane == __ffs(same) - 1) {
+            atomicAdd(&p.width[g], __popc(same));
+            atomicMin(&p.begin[g], i);
+            if (live) {
+                atomicAdd(&p.count[g], __popc(live));
+                atomicMin(&p.first[g], i - lane + __ffs(live) - 1);
+                atomicMin(&p.least[g], least);
+            }
+        }
+    }
     __syncthreads();
-    const int own = g >= 0 ? pos + 1 - p.shared[g] : 0;
+    auto common = [&](int f) { return p.count[f] > 1 ? max(0, min(p.shared[f], p.least[f])) : 0; };
+    const int P = i < a.families ? common(i) : 0, width = p.width[i], tiles = (width + p.tile_members - 1) / p.tile_members;
+    const int own = valid ? pos + 1 - common(g) : 0;
     int wp = P > 0 ? (sa_tiles(P) + a.prefix_cost) * tiles * a.nkv : 0, wo = own > 0 ? (sa_tiles(own) + a.own_cost) * p.own_tiles * a.nkv : 0, tp, to;
-    sa_scan2(p.scan, wp, wo, tp, to);
+    // a prefix's tile costs a block as much as an own tile for every sixteen of its rows (1, 2, 4 or 8 warps share its keys)
+    const int unit_rows = min(width, p.tile_members) * a.gq;
+    const float weight = warp_sum((float)wp * (unit_rows <= 16 ? 1.0f : unit_rows <= 32 ? 2.0f : unit_rows <= 64 ? 4.0f : 8.0f));
+    if (lane == 0) p.weight[i >> 5] = weight;
+    sa_scan2(p.scan[0], wp, wo, tp, to);
+    p.shared[i] = P;                        // behind the barrier: until then it is what was claimed
     p.pbase[i] = wp;
     p.obase[i] = wo;
+    float all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < SA_THREADS / 32; w++) all += p.weight[w];
+    const int blocks = tp > 0 ? min(max((int)((float)a.blocks * all / (all + (float)to) + 0.5f), 1), a.blocks - 1) : 0, own_workers = (a.blocks - blocks) * a.own_per_block;
+    const int lp = max(blocks > 0 ? (tp + blocks - 1) / blocks : 1, a.min_prefix), lo = max((to + own_workers - 1) / own_workers, a.min_own);
     if (i == 0) {
         p.pbase[SA_MAX_TOKENS] = tp;
         p.obase[SA_MAX_TOKENS] = to;
-        p.lp = max((tp + a.prefix_workers - 1) / a.prefix_workers, a.min_prefix);
-        p.lo = max((to + a.own_workers - 1) / a.own_workers, a.min_own);
+        p.prefix_blocks = blocks;
+        p.lp = lp;
+        p.lo = lo;
     }
-    __syncthreads();
-    int rp = P > 0 ? width * a.nh * sa_parts(P, p.lp) : 0, ro = own > 0 ? a.nh * sa_parts(own, p.lo) : 0;
-    sa_scan2(p.scan, rp, ro, tp, to);
+    int rp = P > 0 ? width * a.nh * sa_parts(P, lp) : 0, ro = own > 0 ? a.nh * sa_parts(own, lo) : 0;
+    sa_scan2(p.scan[1], rp, ro, tp, to);
     p.prow[i] = rp;
     p.orow[i] = tp + ro;          // behind the prefix rows
     __syncthreads();
@@ -176,20 +190,20 @@ struct SaPart {
 // The part of a prefix unit at tile `at` of the line, for the worker that walks up to `end`; `at` moves behind it.  False: the unit's keys end before `at`.
 __device__ __forceinline__ bool sa_prefix_part(const SaArgs& a, const SaPlan& p, int& at, int end, int worker, SaPart& r) {
     r.g = sa_find(p.pbase, SA_MAX_TOKENS, at);
-    const int P = p.shared[r.g], width = p.start[r.g + 1] - p.start[r.g], full = sa_tiles(P), length = full + a.prefix_cost;
+    const int P = p.shared[r.g], width = p.width[r.g], full = sa_tiles(P), length = full + a.prefix_cost;
     const int tiles = (width + p.tile_members - 1) / p.tile_members;
     const int rel = at - p.pbase[r.g], u = rel / length, t = rel - u * length, off = at - t;
     at = min(end, off + length);
     if (t >= full) return false;
     r.kvh = u / tiles;
-    r.i0 = p.start[r.g] + (u - r.kvh * tiles) * p.tile_members;
-    r.i1 = min(r.i0 + p.tile_members, p.start[r.g + 1]);
+    r.i0 = p.begin[r.g] + (u - r.kvh * tiles) * p.tile_members;
+    r.i1 = min(r.i0 + p.tile_members, p.begin[r.g] + width);
     r.h0 = 0;
     r.heads = a.gq;
     r.k0 = t * SA_TILE;
     r.k1 = min(P, (at - off) * SA_TILE);
     r.stride = sa_parts(P, p.lp);
-    r.row0 = p.prow[r.g] + (r.kvh * width + r.i0 - p.start[r.g]) * a.gq * r.stride + (worker - off / p.lp);
+    r.row0 = p.prow[r.g] + (r.kvh * width + r.i0 - p.begin[r.g]) * a.gq * r.stride + (worker - off / p.lp);
     r.table = a.block_tables + (size_t)p.seg[p.first[r.g]] * a.max_blocks;
     return true;
 }
@@ -220,8 +234,8 @@ __device__ __forceinline__ bool sa_own_part(const SaArgs& a, const SaPlan& p, in
 __device__ __forceinline__ int sa_prefix_parts(const SaArgs& a, const SaPlan& p, int i, int kvh) {
     const int g = p.grp[i], P = p.shared[g];
     if (P == 0) return 0;
-    const int width = p.start[g + 1] - p.start[g], tiles = (width + p.tile_members - 1) / p.tile_members, full = sa_tiles(P);
-    const int off = p.pbase[g] + (kvh * tiles + (i - p.start[g]) / p.tile_members) * (full + a.prefix_cost);
+    const int width = p.width[g], tiles = (width + p.tile_members - 1) / p.tile_members, full = sa_tiles(P);
+    const int off = p.pbase[g] + (kvh * tiles + (i - p.begin[g]) / p.tile_members) * (full + a.prefix_cost);
     return (off + full - 1) / p.lp - off / p.lp + 1;
 }
 __device__ __forceinline__ int sa_own_parts(const SaArgs& a, const SaPlan& p, int i, int kvh, int tile) {
@@ -236,10 +250,10 @@ __device__ __forceinline__ void sa_write_rows(const SaArgs& a, const SaPlan& p) 
         const int i = r / a.nh, head = r - i * a.nh, kvh = head / a.gq, h = head - kvh * a.gq, g = p.grp[i];
         int4 row = make_int4(0, 0, 0, 0);
         if (g >= 0) {
-            const int P = p.shared[g], own = p.pos[i] + 1 - P, width = p.start[g + 1] - p.start[g];
+            const int P = p.shared[g], own = p.pos[i] + 1 - P, width = p.width[g];
             const int np = sa_prefix_parts(a, p, i, kvh), no = sa_own_parts(a, p, i, kvh, h / SA_OWN_ROWS);
             if (np > 0 || no > 1)
-                row = make_int4(np > 0 ? p.prow[g] + ((kvh * width + i - p.start[g]) * a.gq + h) * sa_parts(P, p.lp) : 0, np,
+                row = make_int4(np > 0 ? p.prow[g] + ((kvh * width + i - p.begin[g]) * a.gq + h) * sa_parts(P, p.lp) : 0, np,
                                 p.orow[i] + head * sa_parts(own, p.lo), no);
         }
         a.rows[r] = row;

@@ -11,6 +11,7 @@ from __future__ import annotations
 import array
 import ctypes
 import os
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -2270,6 +2271,10 @@ def _fit(t: torch.Tensor, name: str, dtype, dims: int, here: int) -> int:
 SHARED_MAX_TOKENS, SHARED_MAX_HEADS, SHARED_MAX_KV_HEADS = 256, 64, 128      # tokens a launch, query heads a key-value head, key-value heads
 
 
+# vk_attention_shared's arguments in one piece: a call with two dozen arguments of their own takes ctypes 3 us, this 1
+_SHARED_ARGS = struct.Struct("QQQQQQQQQQQiiiiiiiiiifi")
+
+
 def attention_shared_takes(dtype: torch.dtype, nh: int, nkv: int, hd: int, tokens: int = 1) -> bool:
     """Whether attention_shared takes these sizes (else the members' tables are read one by one, by attention_decode or attention_rows)."""
     return (dtype in (torch.float32, torch.bfloat16) and 0 < hd <= 256 and hd % (4 if dtype == torch.float32 else 8) == 0 and 0 < nkv <= SHARED_MAX_KV_HEADS
@@ -2302,17 +2307,15 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
     n, families = members.shape[0], shared.shape[0]
     pages, two, kv_heads, page_size, dim = cache_layer.shape
     segments, max_blocks = block_tables.shape
-    if not attention_shared_takes(dtype, nh, nkv, hd, n):
-        raise KernelError(f"attention_shared: {n} tokens of {nh} heads over {nkv} of {hd} in {dtype} are not taken")
-    if width != nh * hd or out.shape != q.shape or two != 2 or kv_heads != nkv or dim != hd:
-        raise KernelError("attention_shared: shapes do not fit the head counts")
+    if width != nh * hd or out.shape != q.shape or two != 2 or kv_heads != nkv or dim != hd or not attention_shared_takes(dtype, nh, nkv, hd, n):
+        raise KernelError(f"attention_shared: shapes do not fit the head counts, or {n} tokens of {nh} heads over {nkv} of {hd} in {dtype} are not taken")
     if token_seg.shape[0] != T or positions.shape[0] != T:
         raise KernelError("attention_shared: per-token arrays differ in length")
     if starts.shape[0] != families + 1 or families > SHARED_MAX_TOKENS:
         raise KernelError("attention_shared: starts is not one longer than shared, or there are more than 256 families")
-    fn = _entry("vk_attention_shared", "ppppppppppziiiiiiiiiifip")
-    _check(fn(pq, pc, pt, ps, pp, pm, pst, psh, po, _fit(scratch, "scratch", torch.uint8, 1, here), scratch.numel(), T, segments, n, families, pages, nh, nkv, hd,
-              page_size, max_blocks, scale, 0 if dtype == torch.float32 else 1, torch._C._cuda_getCurrentRawStream(here)), "attention_shared")
+    args = _SHARED_ARGS.pack(pq, pc, pt, ps, pp, pm, pst, psh, po, _fit(scratch, "scratch", torch.uint8, 1, here), scratch.numel(), T, segments, n, families, pages, nh, nkv,
+                             hd, page_size, max_blocks, scale, dtype is torch.bfloat16)
+    _check(_entry("vk_attention_shared", "pp")(args, torch._C._cuda_getCurrentRawStream(here)), "attention_shared")
     add_launches(1)                       # the walk, and the launch that joins the rows' parts
     return out
 
