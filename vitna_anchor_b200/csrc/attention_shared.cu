@@ -6,104 +6,223 @@
 // the keys they share, which are read once, and the keys that a member has alone are walked by themselves; the two meet by their maxima
 // and sums, which stay in float32 like everything between the scores and the output's rounding.  How the walks are cut: attention_shared_plan.cuh.
 //
-// This file has the entry point and the kernel that takes every size and both types: a part at a time by a block of eight warps, 32 keys
-// and values at a time in shared memory as float32, a warp's lanes 32 keys of a score and then 32 dims of the output.
+// This file has the entry point, the launch that joins the parts, and the kernel that takes every size and both types, on the float32 units.
 // attention_shared_mma.cu has bfloat16 heads of 64 and 128 on the tensor cores.
+//
+// The float32 kernel: a warp holds up to eight rows against 32 keys.  Lane j has key j's scores of all the rows (a piece of its key is read once for the eight, the queries come as
+// broadcasts), the weights go through shared memory, and then the lane has dims j, j + 32, ... of the rows' outputs (a value once for the eight, the weights as broadcasts of four keys).
+// Shared memory then serves 32 products with 12 reads of 16 bytes and its bandwidth and the float32 units' are about even; with a row at a time it was one for one, and 7.5 times slower.
+// R = 1, 2, 4 or 8 warps that cover a prefix's rows share the tiles of their keys; own keys are walked by single warps.
 #include "attention_shared_plan.cuh"
 
 #include <atomic>
 
 namespace vk {
 
-constexpr int SG_KEYS = 32, SG_PREFIX_ROWS = 64, SG_ROWS = SG_PREFIX_ROWS / (SA_THREADS / 32);      // rows a block, rows a warp
+constexpr int SG_KEYS = 32, SG_ROWS = 8, SG_WARPS = SA_THREADS / 32, SG_PREFIX_ROWS = SG_ROWS * SG_WARPS;      // of a warp's tile; rows a block
+constexpr size_t SG_ROOM = 150 * 1024;                                                                          // for the tiles' keys and values
 
-// Shared memory: the plan, then the rows' queries [64][hd] and the keys' and values' tiles [32][hd + 4].
+// Tiles of keys and values that a block holds: one for each warp where there is room.
+__host__ __device__ inline int sg_slots(int hd) {
+    const size_t one = (size_t)2 * SG_KEYS * (hd + 4) * 4;
+    return SG_ROOM / one >= 8 ? 8 : SG_ROOM / one >= 4 ? 4 : 2;
+}
+// Shared memory: the plan; the rows' queries [64][hd], where the groups' outputs meet later, and their maxima and sums [64]; the warps' weights [8][8][32]; the slots' keys and values [32][hd + 4].
 __host__ __device__ inline size_t sg_plan_bytes() { return (sizeof(SaPlan) + 15) / 16 * 16; }
-static size_t sg_smem(int hd) { return sg_plan_bytes() + (size_t)(SG_PREFIX_ROWS * hd + 2 * SG_KEYS * (hd + 4)) * 4; }
+static size_t sg_smem(int hd) {
+    return sg_plan_bytes() + (size_t)SG_PREFIX_ROWS * (hd * 4 + 8) + (size_t)SG_WARPS * SG_ROWS * SG_KEYS * 4 + (size_t)sg_slots(hd) * 2 * SG_KEYS * (hd + 4) * 4;
+}
 
-// A block walks a part and leaves its rows; `alone`: they are all there is of the unit, and the result is written.
-template <typename T, int DIMS>
-__device__ __forceinline__ void sg_walk(const SaArgs& a, const SaPlan& p, const SaPart& r, bool alone, float* sq, float* sk, float* sv) {
+struct SgRows {
+    float *q, *weights, *k, *v;      // the warp's queries [8][hd], weights [8][32], and its group's tile
+    int warps, place;                // of the group, and this warp's place in it
+    int barrier;                     // the group's, where it has more warps than one
+};
+
+// A row's reference maximum is moved only when a score is more than 8 (in base 2) above it, see attention_shared_mma.cu.
+constexpr float SG_AHEAD = 8.0f;
+
+// A group of warps walks tiles tile0, tile0 + step, ... of 32 keys of a part; this warp for its NR rows, whose queries are in w.q.
+template <typename T, int DIMS, int NR>
+__device__ __forceinline__ void sg_walk(const SaArgs& a, const SaPart& part, int tile0, int step, const SgRows& w, float (&m)[NR], float (&l)[NR], float (&o)[NR][DIMS]) {
     constexpr int N = Vec16<T>::N;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = a.hd, ld = hd + 4, vec = hd / N;
-    const int rows = (r.i1 - r.i0) * r.heads;
-    __syncthreads();                                    // the part before is done with the tiles
-    for (int c = threadIdx.x; c < rows * vec; c += SA_THREADS) {
-        const int row = c / vec, d = c % vec * N, i = r.i0 + row / r.heads;
-        float f[N];
-        if (p.pos[i] >= 0) load16<T>(static_cast<const T*>(a.q) + ((size_t)p.tok[i] * a.nh + r.kvh * a.gq + r.h0 + row % r.heads) * hd + d, f);
-        else for (int e = 0; e < N; e++) f[e] = 0.0f;
+    const int lane = threadIdx.x & 31, hd = a.hd, ld = hd + 4, vec = hd / N;
+    auto meet = [&]() {
+        if (w.warps == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(w.barrier), "r"(w.warps * 32) : "memory");
+    };
 #pragma unroll
-        for (int e = 0; e < N; e++) sq[row * hd + d + e] = f[e] * a.scale_log2;
+    for (int r = 0; r < NR; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DIMS; d++) o[r][d] = 0.0f;
     }
-    float m[SG_ROWS], l[SG_ROWS], o[SG_ROWS][DIMS];
-#pragma unroll
-    for (int x = 0; x < SG_ROWS; x++) {
-        m[x] = -INFINITY;
-        l[x] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DIMS; d++) o[x][d] = 0.0f;
-    }
-    for (int kb = r.k0; kb < r.k1; kb += SG_KEYS) {
-        __syncthreads();
-        for (int c = threadIdx.x; c < SG_KEYS * vec; c += SA_THREADS) {
+    for (int kb = part.k0 + tile0 * SG_KEYS; kb < part.k1; kb += step * SG_KEYS) {
+        meet();                                             // the group is past the tile before
+#pragma unroll 4
+        for (int c = w.place * 32 + lane; c < SG_KEYS * vec; c += w.warps * 32) {
             const int kl = c / vec, d = c % vec * N, key = kb + kl;
-            float fk[N], fv[N];
+            const T* src = nullptr;
+            if (key < part.k1) {
+                const int block = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size, page = part.table[block];
+                if (page >= 0 && page < a.pages) src = static_cast<const T*>(a.cache) + (((size_t)page * 2 * a.nkv + part.kvh) * a.page_size + key - block * a.page_size) * hd + d;
+            }
+            const size_t to_value = (size_t)a.nkv * a.page_size * hd;
+            if (sizeof(T) == 4) {                           // no key: nothing of it may be read, not even a NaN
+                copy16_or_zero(w.k + kl * ld + d, reinterpret_cast<const float*>(src ? src : static_cast<const T*>(a.cache)), src != nullptr);
+                copy16_or_zero(w.v + kl * ld + d, reinterpret_cast<const float*>(src ? src + to_value : static_cast<const T*>(a.cache)), src != nullptr);
+            } else {
+                float fk[N], fv[N];
 #pragma unroll
-            for (int e = 0; e < N; e++) fk[e] = fv[e] = 0.0f;       // no key: nothing of it may be read, not even a NaN
-            if (key < r.k1) {
-                const int block = key / a.page_size, page = r.table[block];
-                if (page >= 0 && page < a.pages) {
-                    const T* src = static_cast<const T*>(a.cache) + (((size_t)page * 2 * a.nkv + r.kvh) * a.page_size + key - block * a.page_size) * hd + d;
+                for (int e = 0; e < N; e++) fk[e] = fv[e] = 0.0f;
+                if (src) {
                     load16<T>(src, fk);
-                    load16<T>(src + (size_t)a.nkv * a.page_size * hd, fv);
+                    load16<T>(src + to_value, fv);
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < N; e++) { sk[kl * ld + d + e] = fk[e]; sv[kl * ld + d + e] = fv[e]; }
+                for (int e = 0; e < N; e++) { w.k[kl * ld + d + e] = fk[e]; w.v[kl * ld + d + e] = fv[e]; }
+            }
         }
-        __syncthreads();
-        const int keys = min(SG_KEYS, r.k1 - kb);
+        if (sizeof(T) == 4) asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+        meet();
+        float s[NR];
 #pragma unroll
-        for (int x = 0; x < SG_ROWS; x++) {
-            const int row = warp + x * (SA_THREADS / 32);
-            if (row >= rows) continue;
-            float s = 0.0f;
-            for (int d = 0; d < hd; d += 4) {
-                const float4 u = *reinterpret_cast<const float4*>(sq + row * hd + d), v = *reinterpret_cast<const float4*>(sk + lane * ld + d);
-                s += u.x * v.x + u.y * v.y + u.z * v.z + u.w * v.w;
+        for (int r = 0; r < NR; r++) s[r] = 0.0f;
+#pragma unroll 2
+        for (int d = 0; d < hd; d += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(w.k + lane * ld + d);
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const float4 q = *reinterpret_cast<const float4*>(w.q + r * hd + d);
+                s[r] += q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
             }
-            if (lane >= keys) s = -INFINITY;
-            const float top = fmaxf(m[x], warp_max(s)), ref = top == -INFINITY ? 0.0f : top;
-            const float keep = exp2f(m[x] - ref), w = exp2f(s - ref);
-            m[x] = top;
-            l[x] = l[x] * keep + warp_sum(w);
+        }
+        bool ahead = false;
 #pragma unroll
-            for (int d = 0; d < DIMS; d++) o[x][d] *= keep;
-            for (int k = 0; k < keys; k++) {
-                const float wk = __shfl_sync(0xffffffffu, w, k);
+        for (int r = 0; r < NR; r++) {
+            if (kb + lane >= part.k1) s[r] = -INFINITY;
+            ahead |= s[r] > m[r] + SG_AHEAD;
+        }
+        if (__any_sync(0xffffffffu, ahead)) {
 #pragma unroll
-                for (int d = 0; d < DIMS; d++)
-                    if (lane + 32 * d < hd) o[x][d] += wk * sv[k * ld + lane + 32 * d];
+            for (int r = 0; r < NR; r++) {
+                const float top = fmaxf(m[r], warp_max(s[r])), keep = top == -INFINITY ? 0.0f : exp2f(m[r] - top);
+                m[r] = top;
+                l[r] *= keep;
+#pragma unroll
+                for (int d = 0; d < DIMS; d++) o[r][d] *= keep;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            const float p = exp2f(s[r] - (m[r] == -INFINITY ? 0.0f : m[r]));       // no score above -inf so far: nothing
+            l[r] += p;
+            w.weights[r * SG_KEYS + lane] = p;
+        }
+        __syncwarp();
+        const int keys = min(SG_KEYS, part.k1 - kb);
+        for (int k = 0; k < keys; k += 4) {                 // behind the last key weights and values are zeros
+            float v[4][DIMS];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int d = 0; d < DIMS; d++) v[e][d] = lane + 32 * d < hd ? w.v[(k + e) * ld + lane + 32 * d] : 0.0f;
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                const float4 p = *reinterpret_cast<const float4*>(w.weights + r * SG_KEYS + k);
+#pragma unroll
+                for (int d = 0; d < DIMS; d++) o[r][d] += p.x * v[0][d] + p.y * v[1][d] + p.z * v[2][d] + p.w * v[3][d];
             }
         }
     }
 #pragma unroll
-    for (int x = 0; x < SG_ROWS; x++) {
-        const int row = warp + x * (SA_THREADS / 32), i = r.i0 + row / r.heads;
-        if (row >= rows || p.pos[i] < 0) continue;
-        if (alone) {
-            T* out = static_cast<T*>(a.out) + ((size_t)p.tok[i] * a.nh + r.kvh * a.gq + r.h0 + row % r.heads) * hd;
+    for (int r = 0; r < NR; r++) l[r] = warp_sum(l[r]);
+}
+
+// The warp's rows' queries, scaled, into w.q; zeros where there is no such row, or its member is not there.
+template <typename T> __device__ __forceinline__ void sg_queries(const SaArgs& a, const SaPlan& p, const SaPart& part, int row0, int rows, const SgRows& w) {
+    constexpr int N = Vec16<T>::N;
+    const int vec = a.hd / N;
+    for (int c = threadIdx.x & 31; c < SG_ROWS * vec; c += 32) {
+        const int r = c / vec, d = c % vec * N, row = row0 + r, i = part.i0 + row / part.heads;
+        float f[N];
+        if (row < rows && p.pos[i] >= 0) load16<T>(static_cast<const T*>(a.q) + ((size_t)p.tok[i] * a.nh + part.kvh * a.gq + part.h0 + row % part.heads) * a.hd + d, f);
+        else
+#pragma unroll
+            for (int e = 0; e < N; e++) f[e] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; e++) w.q[r * a.hd + d + e] = f[e] * a.scale_log2;
+    }
+    __syncwarp();
+}
+
+// A block's part of a prefix: groups of R warps, 8 rows a warp; the groups' outputs meet over the queries.
+template <typename T, int DIMS, int NR>
+__device__ __forceinline__ void sg_prefix(const SaArgs& a, const SaPlan& p, const SaPart& part, float* sq, float2* ml, const SgRows& mine) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = a.hd, rows = (part.i1 - part.i0) * part.heads;
+    const int R = rows <= SG_ROWS ? 1 : rows <= 2 * SG_ROWS ? 2 : rows <= 4 * SG_ROWS ? 4 : 8, groups = min(SG_WARPS / R, sg_slots(hd)), group = warp / R, place = warp % R;
+    SgRows w = mine;
+    w.warps = R;
+    w.place = place;
+    w.barrier = 1 + group;
+    float m[NR], l[NR], o[NR][DIMS];
+    __syncthreads();                                        // everybody is past the part before
+    if (group < groups) {
+        w.k = mine.k + (size_t)group * 2 * SG_KEYS * (hd + 4);
+        w.v = w.k + SG_KEYS * (hd + 4);
+        sg_queries<T>(a, p, part, place * SG_ROWS, rows, w);
+        sg_walk<T, DIMS, NR>(a, part, group, groups, w, m, l, o);
+    }
+    __syncthreads();                                        // and past the queries
+    if (group < groups) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
 #pragma unroll
             for (int d = 0; d < DIMS; d++)
-                if (lane + 32 * d < hd) out[lane + 32 * d] = from_f32<T>(o[x][d] / l[x]);
-        } else {
-            const int at = r.row0 + ((i - r.i0) * a.gq + row % r.heads) * r.stride;
-#pragma unroll
-            for (int d = 0; d < DIMS; d++)
-                if (lane + 32 * d < hd) a.part_o[(size_t)at * hd + lane + 32 * d] = o[x][d];
-            if (lane == 0) a.part_ml[at] = make_float2(m[x], l[x]);
+                if (lane + 32 * d < hd) sq[(warp * SG_ROWS + r) * hd + lane + 32 * d] = o[r][d];
+            if (lane == 0) ml[warp * SG_ROWS + r] = make_float2(m[r], l[r]);
         }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < rows * hd; c += SA_THREADS) {
+        const int row = c / hd, d = c - row * hd, i = part.i0 + row / part.heads;
+        if (p.pos[i] < 0) continue;
+        float top = -INFINITY, sum = 0.0f, out = 0.0f;
+        for (int g = 0; g < groups; g++) top = fmaxf(top, ml[g * R * SG_ROWS + row].x);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        for (int g = 0; g < groups; g++) {
+            const float2 s = ml[g * R * SG_ROWS + row];
+            const float e = exp2f(s.x - ref);
+            sum += s.y * e;
+            out += sq[(g * R * SG_ROWS + row) * hd + d] * e;
+        }
+        const int at = part.row0 + ((i - part.i0) * a.gq + row % part.heads) * part.stride;
+        a.part_o[(size_t)at * hd + d] = out;
+        if (d == 0) a.part_ml[at] = make_float2(top, sum);
+    }
+}
+
+// A warp's part of own keys; `alone`: it is all there is of the unit, and the result is written.
+template <typename T, int DIMS, int NR>
+__device__ __forceinline__ void sg_own(const SaArgs& a, const SaPlan& p, const SaPart& part, bool alone, const SgRows& w) {
+    const int lane = threadIdx.x & 31, hd = a.hd;
+    float m[NR], l[NR], o[NR][DIMS];
+    __syncwarp();
+    sg_queries<T>(a, p, part, 0, part.heads, w);
+    sg_walk<T, DIMS, NR>(a, part, 0, 1, w, m, l, o);
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        if (r >= part.heads) break;
+        T* out = static_cast<T*>(a.out) + ((size_t)p.tok[part.i0] * a.nh + part.kvh * a.gq + part.h0 + r) * hd;
+        const int at = part.row0 + r * part.stride;
+#pragma unroll
+        for (int d = 0; d < DIMS; d++)
+            if (lane + 32 * d < hd) {
+                if (alone) out[lane + 32 * d] = from_f32<T>(o[r][d] / l[r]);
+                else a.part_o[(size_t)at * hd + lane + 32 * d] = o[r][d];
+            }
+        if (!alone && lane == 0) a.part_ml[at] = make_float2(m[r], l[r]);
     }
 }
 
@@ -112,25 +231,43 @@ __global__ void __launch_bounds__(SA_THREADS) attention_shared_kernel(const SaAr
     extern __shared__ __align__(16) unsigned char smem[];
     SaPlan& p = *reinterpret_cast<SaPlan*>(smem);
     float* sq = reinterpret_cast<float*>(smem + sg_plan_bytes());
-    float* sk = sq + SG_PREFIX_ROWS * a.hd;
-    float* sv = sk + SG_KEYS * (a.hd + 4);
+    float2* ml = reinterpret_cast<float2*>(sq + SG_PREFIX_ROWS * a.hd);
+    float* weights = reinterpret_cast<float*>(ml + SG_PREFIX_ROWS);
+    const int warp = threadIdx.x >> 5;
+    SgRows w;
+    w.q = sq + warp * SG_ROWS * a.hd;
+    w.weights = weights + warp * SG_ROWS * SG_KEYS;
+    w.k = weights + SG_WARPS * SG_ROWS * SG_KEYS;
+    w.v = nullptr;
+    w.warps = 1;
+    w.place = w.barrier = 0;
     sa_make_plan(a, p);                       // from the step's metadata, which no kernel writes
     dependency_wait();
     let_dependents_start();
     SaPart r;
     const bool prefix = (int)blockIdx.x < p.prefix_blocks;
-    const int worker = (int)blockIdx.x - (prefix ? 0 : p.prefix_blocks);
-    int at = worker * p.lp, end = prefix ? min(at + p.lp, p.pbase[SA_MAX_TOKENS]) : 0;
+    int at = blockIdx.x * p.lp, end = prefix ? min(at + p.lp, p.pbase[SA_MAX_TOKENS]) : 0;
     while (at < end) {
-        if (!sa_prefix_part(a, p, at, end, worker, r)) continue;
-        sg_walk<T, DIMS>(a, p, r, false, sq, sk, sv);
+        if (!sa_prefix_part(a, p, at, end, blockIdx.x, r)) continue;
+        const int rows = (r.i1 - r.i0) * r.heads;
+        if (rows <= 2) sg_prefix<T, DIMS, 2>(a, p, r, sq, ml, w);
+        else if (rows <= 4) sg_prefix<T, DIMS, 4>(a, p, r, sq, ml, w);
+        else sg_prefix<T, DIMS, 8>(a, p, r, sq, ml, w);
     }
-    at = worker * p.lo;
-    end = prefix ? 0 : min(at + p.lo, p.obase[SA_MAX_TOKENS]);
-    while (at < end) {
-        int parts;
-        if (!sa_own_part(a, p, at, end, worker, r, parts)) continue;
-        sg_walk<T, DIMS>(a, p, r, parts == 1 && p.shared[r.g] == 0, sq, sk, sv);      // a unit that needs nobody else writes its result
+    if (!prefix && warp < a.own_per_block) {
+        const int worker = warp * ((int)gridDim.x - p.prefix_blocks) + (int)blockIdx.x - p.prefix_blocks;
+        w.k += (size_t)warp * 2 * SG_KEYS * (a.hd + 4);
+        w.v = w.k + SG_KEYS * (a.hd + 4);
+        at = worker * p.lo;
+        end = min(at + p.lo, p.obase[SA_MAX_TOKENS]);
+        while (at < end) {
+            int parts;
+            if (!sa_own_part(a, p, at, end, worker, r, parts)) continue;
+            const bool alone = parts == 1 && p.shared[r.g] == 0;      // a unit that needs nobody else
+            if (r.heads == 1) sg_own<T, DIMS, 1>(a, p, r, alone, w);
+            else if (r.heads <= 4) sg_own<T, DIMS, 4>(a, p, r, alone, w);
+            else sg_own<T, DIMS, 8>(a, p, r, alone, w);
+        }
     }
     sa_write_rows(a, p);
 }
@@ -271,7 +408,7 @@ static int sa_multiprocessors() {
 // Rows of parts that a launch can need: a unit of so many tiles of keys and up to R rows leaves at most R (tiles / L + 2), L is at least the line's
 // length / workers, and the units' rows are n nh together.  R is 128 for prefixes here and the workers a multiprocessor's blocks (2) and warps (16), which covers
 // both kernels.
-static size_t sa_part_rows(int tokens, int nh) { return (size_t)(128 * 2 + SA_OWN_ROWS * 16) * SA_MAX_MULTIPROCESSORS + 4 * (size_t)tokens * nh; }
+static size_t sa_part_rows(int tokens, int nh) { return (size_t)(128 * 2 + SA_MAX_OWN_ROWS * 16) * SA_MAX_MULTIPROCESSORS + 4 * (size_t)tokens * nh; }
 
 }  // namespace vk
 
@@ -324,8 +461,9 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
         return status != VK_OK ? status : launch_join(a, dtype, stream);
     }
     a.prefix_rows = SG_PREFIX_ROWS;
+    a.own_rows = SG_ROWS;
     a.blocks = sms;
-    a.own_per_block = 1;
+    a.own_per_block = sg_slots(hd);
     a.min_prefix = a.min_own = 4;
     a.prefix_cost = a.own_cost = 4;
     const size_t smem = sg_smem(hd);

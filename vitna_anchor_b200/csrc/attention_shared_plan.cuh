@@ -5,7 +5,7 @@
 //
 //   prefix   a tile of up to prefix_rows rows (members x the heads that read one key-value head) of one family over the
 //            family's shared keys [0, P); P is at most the smallest position of its members, and 0 for a family of one
-//   own      one member's heads (up to OWN_ROWS of them) over the keys [P, position] that only it reads
+//   own      one member's heads (up to own_rows of them) over the keys [P, position] that only it reads
 //
 // The launch's blocks are divided between the two by what they have to do, so that a block walks one kind only: what limits the prefixes of large families (products) and what limits
 // the own keys (memory) is then busy at the same time, and where there is little to do neither waits for the other.  The prefix units, each as its tiles of 16 keys and a number of
@@ -21,7 +21,7 @@
 
 namespace vk {
 
-constexpr int SA_MAX_TOKENS = 256, SA_THREADS = 256, SA_MAX_HEADS = 64, SA_OWN_ROWS = 16, SA_MAX_KV_HEADS = 128;
+constexpr int SA_MAX_TOKENS = 256, SA_THREADS = 256, SA_MAX_HEADS = 64, SA_MAX_OWN_ROWS = 16, SA_MAX_KV_HEADS = 128;
 
 struct SaArgs {
     const void* q;                 // [tokens][nh][hd]
@@ -37,7 +37,7 @@ struct SaArgs {
     float2* part_ml;               // [rows] maximum (base 2) and sum
     float* part_o;                 // [rows][hd]
     int n, families, tokens, segments, pages, nh, nkv, gq, hd, page_size, page_shift, max_blocks;
-    int prefix_rows, blocks, own_per_block, min_prefix, min_own, prefix_cost, own_cost;      // own workers a block; the last four in tiles of keys
+    int prefix_rows, own_rows, blocks, own_per_block, min_prefix, min_own, prefix_cost, own_cost;      // own workers a block; the last four in tiles of keys
     float scale_log2;
 };
 
@@ -112,7 +112,7 @@ __device__ __forceinline__ void sa_make_plan(const SaArgs& a, SaPlan& p) {
     p.least[i] = 0x7fffffff;
     if (i == 0) {
         p.tile_members = a.prefix_rows / a.gq;
-        p.own_tiles = (a.gq + SA_OWN_ROWS - 1) / SA_OWN_ROWS;
+        p.own_tiles = (a.gq + a.own_rows - 1) / a.own_rows;
     }
     __syncthreads();
     // the member's family: as many as begin at or before it, the first aside (so families are runs of members even where starts go back); none: before the
@@ -218,8 +218,8 @@ __device__ __forceinline__ bool sa_own_part(const SaArgs& a, const SaPlan& p, in
     at = min(end, off + length);
     if (t >= full) return false;
     r.kvh = u / p.own_tiles;
-    r.h0 = (u - r.kvh * p.own_tiles) * SA_OWN_ROWS;
-    r.heads = min(SA_OWN_ROWS, a.gq - r.h0);
+    r.h0 = (u - r.kvh * p.own_tiles) * a.own_rows;
+    r.heads = min(a.own_rows, a.gq - r.h0);
     r.k0 = P + t * SA_TILE;
     r.k1 = P + min(own, (at - off) * SA_TILE);
     r.stride = sa_parts(own, p.lo);
@@ -251,7 +251,7 @@ __device__ __forceinline__ void sa_write_rows(const SaArgs& a, const SaPlan& p) 
         int4 row = make_int4(0, 0, 0, 0);
         if (g >= 0) {
             const int P = p.shared[g], own = p.pos[i] + 1 - P, width = p.width[g];
-            const int np = sa_prefix_parts(a, p, i, kvh), no = sa_own_parts(a, p, i, kvh, h / SA_OWN_ROWS);
+            const int np = sa_prefix_parts(a, p, i, kvh), no = sa_own_parts(a, p, i, kvh, h / a.own_rows);
             if (np > 0 || no > 1)
                 row = make_int4(np > 0 ? p.prow[g] + ((kvh * width + i - p.begin[g]) * a.gq + h) * sa_parts(P, p.lp) : 0, np,
                                 p.orow[i] + head * sa_parts(own, p.lo), no);
