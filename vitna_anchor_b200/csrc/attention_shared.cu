@@ -20,13 +20,10 @@
 namespace vk {
 
 constexpr int SG_KEYS = 32, SG_ROWS = 8, SG_WARPS = SA_THREADS / 32, SG_PREFIX_ROWS = SG_ROWS * SG_WARPS;      // of a warp's tile; rows a block
-constexpr size_t SG_ROOM = 150 * 1024;                                                                          // for the tiles' keys and values
 
-// Tiles of keys and values that a block holds: one for each warp where there is room.
-__host__ __device__ inline int sg_slots(int hd) {
-    const size_t one = (size_t)2 * SG_KEYS * (hd + 4) * 4;
-    return SG_ROOM / one >= 8 ? 8 : SG_ROOM / one >= 4 ? 4 : 2;
-}
+// Tiles of keys and values that a block holds, for as many warps that walk keys of their own: heads of up to 64 leave room for two blocks a multiprocessor with four each.
+__host__ __device__ inline int sg_slots(int hd) { return hd <= 128 ? 4 : 2; }
+static int sg_blocks(int hd) { return hd <= 64 ? 2 : 1; }
 // Shared memory: the plan; the rows' queries [64][hd], where the groups' outputs meet later, and their maxima and sums [64]; the warps' weights [8][8][32]; the slots' keys and values [32][hd + 4].
 __host__ __device__ inline size_t sg_plan_bytes() { return (sizeof(SaPlan) + 15) / 16 * 16; }
 static size_t sg_smem(int hd) {
@@ -227,7 +224,7 @@ __device__ __forceinline__ void sg_own(const SaArgs& a, const SaPlan& p, const S
 }
 
 template <typename T, int DIMS>
-__global__ void __launch_bounds__(SA_THREADS) attention_shared_kernel(const SaArgs a) {
+__global__ void __launch_bounds__(SA_THREADS, DIMS == 2 ? 2 : 1) attention_shared_kernel(const SaArgs a) {
     extern __shared__ __align__(16) unsigned char smem[];
     SaPlan& p = *reinterpret_cast<SaPlan*>(smem);
     float* sq = reinterpret_cast<float*>(smem + sg_plan_bytes());
@@ -462,7 +459,8 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
     }
     a.prefix_rows = SG_PREFIX_ROWS;
     a.own_rows = SG_ROWS;
-    a.blocks = sms;
+    a.row_unit = 16.0f;
+    a.blocks = sms * sg_blocks(hd);
     a.own_per_block = sg_slots(hd);
     a.min_prefix = a.min_own = 4;
     a.prefix_cost = a.own_cost = 4;
@@ -472,7 +470,7 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
         auto kern = attention_shared_kernel<T, DIMS>;                                                                                   \
         const int e = sa_allow_smem(kern, smem);                                                                                        \
         if (e != VK_OK) return e;                                                                                                       \
-        const int status = launch_dependent(kern, dim3(sms), dim3(SA_THREADS), smem, stream, a);                                        \
+        const int status = launch_dependent(kern, dim3(a.blocks), dim3(SA_THREADS), smem, stream, a);                                        \
         return status != VK_OK ? status : launch_join(a, dtype, stream);                                                                \
     } while (0)
     if (dtype == 0) {

@@ -515,6 +515,7 @@ bool attention_shared_mma_takes(const SaArgs& a, int dtype) {
 int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream) {
     a.prefix_rows = SM_PREFIX_ROWS;
     a.own_rows = 16;
+    a.row_unit = 16.0f;
     const int blocks = multiprocessors * (a.hd == 64 ? 2 : 1);
     a.blocks = blocks;
     a.own_per_block = SA_THREADS / 32;

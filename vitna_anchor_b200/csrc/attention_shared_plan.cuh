@@ -38,7 +38,7 @@ struct SaArgs {
     float* part_o;                 // [rows][hd]
     int n, families, tokens, segments, pages, nh, nkv, gq, hd, page_size, page_shift, max_blocks;
     int prefix_rows, own_rows, blocks, own_per_block, min_prefix, min_own, prefix_cost, own_cost;      // own workers a block; the last four in tiles of keys
-    float scale_log2;
+    float scale_log2, row_unit;    // row_unit: the rows of a prefix's tile that cost as much as an own tile
 };
 
 // A row's parts: prefix_parts from prefix_row on and own_parts from own_row on; none: the row was written when it was walked, or its member is not there.
@@ -151,9 +151,7 @@ __device__ __forceinline__ void sa_make_plan(const SaArgs& a, SaPlan& p) {
     const int P = i < a.families ? common(i) : 0, width = p.width[i], tiles = (width + p.tile_members - 1) / p.tile_members;
     const int own = valid ? pos + 1 - common(g) : 0;
     int wp = P > 0 ? (sa_tiles(P) + a.prefix_cost) * tiles * a.nkv : 0, wo = own > 0 ? (sa_tiles(own) + a.own_cost) * p.own_tiles * a.nkv : 0, tp, to;
-    // a prefix's tile costs a block as much as an own tile for every sixteen of its rows (1, 2, 4 or 8 warps share its keys)
-    const int unit_rows = min(width, p.tile_members) * a.gq;
-    const float weight = warp_sum((float)wp * (unit_rows <= 16 ? 1.0f : unit_rows <= 32 ? 2.0f : unit_rows <= 64 ? 4.0f : 8.0f));
+    const float weight = warp_sum((float)wp * fmaxf(1.0f, (float)(min(width, p.tile_members) * a.gq) / a.row_unit));
     if (lane == 0) p.weight[i >> 5] = weight;
     sa_scan2(p.scan[0], wp, wo, tp, to);
     p.shared[i] = P;                        // behind the barrier: until then it is what was claimed
