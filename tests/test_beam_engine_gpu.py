@@ -21,7 +21,7 @@ def dirs(tmp_path_factory):
     root = tmp_path_factory.mktemp("beam")
     made = {name: write_tiny(str(root / name), tiny, std=0.15) for name, tiny in TINIES.items()}
     for kv, hd in [(2, 64), (1, 128)]:
-        cfg = dict(TINIES["tinyA"]["config"], hidden_size=256, num_attention_heads=6, num_key_value_heads=kv, head_dim=hd, vocab_size=500, max_position_embeddings=512)
+        cfg = dict(TINIES["tinyA"]["config"], hidden_size=256, num_attention_heads=6, num_key_value_heads=kv, head_dim=hd, vocab_size=500, max_position_embeddings=8192)
         made[f"heads{hd}"] = write_tiny(str(root / f"heads{hd}"), dict(TINIES["tinyA"], config=cfg), std=0.1)
     import importlib
     for name in OTHERS:
@@ -29,6 +29,15 @@ def dirs(tmp_path_factory):
         made[name] = str(root / name.replace("/", "_"))
         importlib.import_module(f"{arch}_models").make_model(made[name], which)
     return made
+
+
+@pytest.fixture(params=[1, 2])
+def shared_mode(request):
+    """Every step that shares goes through the attention that reads common pages once, or those of the rule (on these small models none)."""
+    from vitna_anchor_b200 import ops
+    before = ops.set_attention_shared(request.param)
+    yield request.param
+    ops.set_attention_shared(before)
 
 
 def _engine(path, dtype, **kw):
@@ -91,10 +100,12 @@ def test_search_matches_one_that_starts_over(name, dirs):
 
 @pytest.mark.parametrize("graphs", [True, False])
 @pytest.mark.parametrize("name", ["tinyB", "heads64", "heads128", "lupanex/looped", "lirutar/all"])
-def test_sums_are_those_of_the_sequences(name, graphs, dirs):
+def test_sums_are_those_of_the_sequences(name, graphs, dirs, shared_mode):
     """bfloat16: every result's sum of log probabilities is that of its sequence run from its start, as near as two ways of cutting one request come
     (8e-2 of the logits' scale at a position; the mean over a sequence is held to that)."""
-    eng = _engine(dirs[name], "bfloat16", kv_block=16 if name.startswith("heads") else 4, cuda_graphs=graphs)
+    # heads64 and heads128: tables so wide that the common keys are walked once, not every member by itself
+    wide = dict(kv_block=16, ctx=8192, num_pages=200) if name.startswith("heads") else {}
+    eng = _engine(dirs[name], "bfloat16", cuda_graphs=graphs, **wide)
     rng = np.random.default_rng(3)
     prompt = [int(t) for t in rng.integers(0, eng.model.vocab_size, 150 if name.startswith("heads") else 40)]
     got = eng.beam_search(prompt, beams=6, max_new=40)
@@ -106,10 +117,11 @@ def test_sums_are_those_of_the_sequences(name, graphs, dirs):
         lp = _log_probs(eng, prompt + r.ids[:-1])[len(prompt) - 1:]
         assert abs(lp[np.arange(40), r.ids].sum() - r.log_prob) <= 40 * 8e-2 * scale
     eng.runner.cache.check()
+    assert {k[2] for k in eng.runner._decode_graphs} == ({shared_mode == 1} if graphs else set())
 
 
 @pytest.mark.parametrize("name,tol", [("heads64", 3e-2), ("heads128", 3e-2), ("tinyB", 3e-2)])
-def test_forked_requests_give_the_logits_of_separate_ones(name, tol, dirs):
+def test_forked_requests_give_the_logits_of_separate_ones(name, tol, dirs, shared_mode):
     """Six requests forked from one, decoding beside a stranger through the graph that reads common pages once, against the same tokens in
     requests of their own through the ordinary graph (bfloat16; both see the same keys)."""
     from vitna_anchor_b200.engine.loading import load_model
@@ -120,7 +132,7 @@ def test_forked_requests_give_the_logits_of_separate_ones(name, tol, dirs):
     prompt, stranger = ([int(t) for t in rng.integers(0, V, n)] for n in (203, 30))
 
     def play(fork):
-        r = ModelRunner(model, page_size=16, max_requests=8, max_batch_tokens=512, max_model_len=256)
+        r = ModelRunner(model, page_size=16, max_requests=8, max_batch_tokens=512, num_pages=200)
         r.open("s")
         r.step([StepEntry("s", stranger, [])])
         for i in range(6):
@@ -135,7 +147,7 @@ def test_forked_requests_give_the_logits_of_separate_ones(name, tol, dirs):
         for row in tokens:
             out.append(r.step([StepEntry(rid, [int(t)], [0]) for rid, t in zip(order, row)]).clone())
         r.check()
-        assert {k[2] for k in r._decode_graphs} == {fork} and r.graph_replays > 5
+        assert {k[2] for k in r._decode_graphs} == {fork and shared_mode == 1} and r.graph_replays > 5
         r.cache.check()
         return torch.stack(out)
 

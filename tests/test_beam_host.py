@@ -117,6 +117,13 @@ def test_forks_and_adoptions_keep_everybodys_positions(seed):
         except CacheError as e:
             assert what == "truncate", e                      # behind a window, or inside a page that others hold
         m.check()
+        for f in t.families(list(m.history)):
+            rids = [list(m.history)[i] for i in f]
+            blocks = [t.get(r).tables[0].blocks for r in rids]
+            same = 0
+            while all(same < len(b) for b in blocks) and len({b[same] for b in blocks}) == 1:
+                same += 1
+            assert t.common_blocks(rids, 0) == same
     for rid in list(m.history):
         t.close(rid)
     assert [p.free_pages for p in t.pools] == [60, 60]
@@ -179,6 +186,18 @@ def test_who_takes_over_whom():
         for r, p in zip(requests, parents):
             assert r is None or source.get(r, r) == live[p]
         assert (None in requests) <= (not left)
+
+
+def test_when_common_pages_are_read_once():
+    """The rule's two sides (positions of 32 heads of 64: 8 KB; of 3: 0.75 KB), and the switch."""
+    pays = ops.attention_shared_pays
+    assert not pays(4, 4 * 576, 3 * 512, 32, 64) and pays(8, 8 * 576, 7 * 512, 32, 64)
+    assert not pays(64, 64 * 576, 63 * 512, 3, 64) and pays(64, 64 * 2112, 63 * 2048, 3, 64)
+    assert not pays(8, 8 * 2000, 7 * 512, 32, 64) and not pays(8, 8 * 576, 0, 32, 64)
+    for mode, taken in [(0, False), (1, True)]:
+        assert ops.set_attention_shared(mode) == 2
+        assert pays(2, 20, 8, 1, 16) == taken and not pays(2, 20, 0, 1, 16)
+        assert ops.set_attention_shared(2) == mode
 
 
 def test_scores():

@@ -63,8 +63,11 @@ class Batch:
                 self.cache[page, :, :, at % ps] = mine
         self.maxb = max(max(len(t) for t in self.tables), 1) + 2
 
-    def device(self):
+    def device(self, wide=True):
+        """wide: block tables so wide that the call does not walk every member by itself (where it can)."""
         i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
+        if wide:
+            self.maxb = max(self.maxb, (256 << 20) // (max(1, len(self.members)) * self.ps * self.nkv * self.hd * 4) + 1)
         self.d = dict(q=self.q.cuda(), cache=self.cache.cuda(), tables=i([t + [0x7fffffff] * (self.maxb - len(t)) for t in self.tables]), seg=i(list(range(len(self.pos)))),
                       pos=i(self.pos), members=i(self.members).reshape(-1), starts=i(self.starts), shared=i(self.shared))
         self.d["out"] = torch.full_like(self.d["q"], 7.0)
@@ -126,20 +129,20 @@ SHAPES = [
 ]
 
 
-@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dtype,wide", [(BF16, True), (BF16, False), (F32, True)])
 @pytest.mark.parametrize("n", range(len(SHAPES)))
-def test_attention_shared(ops, dtype, n):
+def test_attention_shared(ops, dtype, wide, n):
     families, nh, nkv, hd, ps = SHAPES[n]
     if not families:
-        b = Batch([(16, [3])], nh, nkv, hd, ps, dtype, outside=2).device()
+        b = Batch([(16, [3])], nh, nkv, hd, ps, dtype, outside=2).device(wide)
         b.d["members"], b.d["starts"], b.d["shared"] = b.d["members"][:0], b.d["starts"][:1], b.d["shared"][:0]
         assert bool((b.run(ops) == 7).all())                               # no family: nothing is written
         return
-    Batch(families, nh, nkv, hd, ps, dtype, seed=n).device().check(ops)
+    Batch(families, nh, nkv, hd, ps, dtype, seed=n).device(wide).check(ops)
 
 
-@pytest.mark.parametrize("dtype,hd", [(BF16, 64), (BF16, 128), (F32, 64)])
-def test_attention_shared_random_families(ops, dtype, hd):
+@pytest.mark.parametrize("dtype,hd,wide", [(BF16, 64, True), (BF16, 128, True), (BF16, 64, False), (BF16, 128, False), (F32, 64, True)])
+def test_attention_shared_random_families(ops, dtype, hd, wide):
     """Many layouts through ONE scratch of exactly the bytes of the largest, with guards around it."""
     rng = random.Random(11)
     most = ops.attention_shared_scratch_bytes(128, 8, 8, hd)
@@ -150,14 +153,15 @@ def test_attention_shared_random_families(ops, dtype, hd):
         nkv = rng.choice([1, 2, 8])
         nh = nkv * rng.choice([1, 2, 3, 8] if nkv == 1 else [1])
         fams = [(rng.choice([0, rng.randint(1, 900)]), [rng.randint(1, 90) for _ in range(rng.randint(1, 12))]) for _ in range(rng.randint(1, 9))]
-        Batch(fams, nh, nkv, hd, rng.choice([16, 8, 13]), dtype, seed=n, outside=rng.randint(0, 3)).device().check(ops, scratch)
+        Batch(fams, nh, nkv, hd, rng.choice([16, 8, 13]), dtype, seed=n, outside=rng.randint(0, 3)).device(wide).check(ops, scratch)
     assert bool((guarded[:2048] == 0x5A).all()) and bool((guarded[2048 + most:] == 0x5A).all())
 
 
-def test_attention_shared_claims_that_do_not_fit(ops):
+@pytest.mark.parametrize("wide", [True, False])
+def test_attention_shared_claims_that_do_not_fit(ops, wide):
     """shared beyond the smallest position is cut there; an empty family, tokens that are not there, starts that go back and starts beyond
     the list are nothing."""
-    b = Batch([(64, [5, 9])], 4, 2, 64, 16, BF16, outside=3).device()
+    b = Batch([(64, [5, 9])], 4, 2, 64, 16, BF16, outside=3).device(wide)
     want, tol = b.want()
     i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")          # noqa: E731
     m = b.members
@@ -168,7 +172,7 @@ def test_attention_shared_claims_that_do_not_fit(ops):
         b.d["out"].fill_(7.0)
         got = b.run(ops, torch.zeros(ops.attention_shared_scratch_bytes(8, 4, 2, 64), dtype=torch.uint8, device="cuda")).double().cpu()
         assert float(((got - want).abs() - tol).max()) <= 0
-    same = Batch([(0, [40, 40])], 4, 2, 64, 16, BF16).device()               # two names for one request: all it has is common, but for the token's own key
+    same = Batch([(0, [40, 40])], 4, 2, 64, 16, BF16).device(wide)               # two names for one request: all it has is common, but for the token's own key
     t = same.members
     same.d["tables"][t[1]] = same.d["tables"][t[0]]
     same.d["q"][t[1]] = same.d["q"][t[0]]
@@ -177,25 +181,27 @@ def test_attention_shared_claims_that_do_not_fit(ops):
     same.check(ops)
 
 
-def test_attention_shared_bad_blocks_count_as_zeros(ops):
+@pytest.mark.parametrize("wide", [True, False])
+def test_attention_shared_bad_blocks_count_as_zeros(ops, wide):
     b = Batch([(64, [20, 9])], 4, 2, 64, 16, BF16)
     b.cache[b.tables[b.members[0]][1]] = 0
     b.cache[b.tables[b.members[1]][4]] = 0
-    b.device()
+    b.device(wide)
     b.d["tables"][b.members[0], 1] = b.pages
     b.d["tables"][b.members[1], 1] = b.pages
     b.d["tables"][b.members[1], 4] = -7
     b.check(ops)
 
 
-def test_attention_shared_of_scores_without_a_number(ops):
+@pytest.mark.parametrize("wide", [True, False])
+def test_attention_shared_of_scores_without_a_number(ops, wide):
     """Scores of -inf weigh nothing; a token all of whose scores are -inf, or one of them NaN, has no number, and the others keep theirs."""
     b = Batch([(128, [40, 9, 30])], 4, 2, 64, 16, BF16)
     b.q.abs_()
     own = b.tables[b.members[0]][8:]
     b.cache[b.tables[b.members[0]][2], 0, :, 3] = -math.inf       # one shared key
     b.cache[own[1], 0, 0, 5] = float("nan")                       # one key of the first member, the first key-value head
-    got = b.device().run(ops).double().cpu().view(-1, 4, 64)
+    got = b.device(wide).run(ops).double().cpu().view(-1, 4, 64)
     want, tol = (x.view(-1, 4, 64) for x in b.want())
     assert bool(torch.isnan(got[b.members[0], :2]).all()) and bool(torch.isnan(want[b.members[0], :2]).all())
     tol = torch.where(torch.isfinite(tol), tol, torch.tensor(2.0 ** -6).double())      # the bound's sums are over infinite keys
@@ -215,8 +221,9 @@ def test_attention_shared_far_in_a_large_pool(ops):
     b.check(ops)
 
 
-def test_attention_shared_replayed_and_on_another_stream(ops):
-    b = Batch([(200, [5, 60, 17]), (0, [9])], 6, 2, 64, 16, BF16, seed=3).device()
+@pytest.mark.parametrize("wide", [True, False])
+def test_attention_shared_replayed_and_on_another_stream(ops, wide):
+    b = Batch([(200, [5, 60, 17]), (0, [9])], 6, 2, 64, 16, BF16, seed=3).device(wide)
     scratch = torch.zeros(ops.attention_shared_scratch_bytes(4, 6, 2, 64), dtype=torch.uint8, device="cuda")
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

@@ -152,6 +152,7 @@ class RequestCache:
     length: int = 0                # positions whose keys and values are in the cache (committed)
     reserved: int = 0              # positions reserved beyond `length` for the step in flight
     family: Hashable = None        # the request this one's pages began with: its own id, or that of the request it was forked from
+    common: int = 1 << 30          # at least so many leading blocks it has in common with all of its family (no limit while it is alone)
     tables: Dict[int, GroupTable] = field(default_factory=dict)   # group index -> table
 
 
@@ -215,6 +216,8 @@ class PageTables:
                 else:
                     mine.blocks.append(UNMAPPED)
         rc.length, rc.reserved, rc.family = source.length, 0, source.family
+        source.common = min(source.common, full)
+        rc.common = source.common
         return copies
 
     def fork(self, source_id: Hashable, request_id: Hashable) -> List[tuple]:
@@ -359,7 +362,25 @@ class PageTables:
                 if page != UNMAPPED and self.pools[g].is_shared(page):
                     raise CacheError(f"position {length} of request {request_id!r} lies inside a page that others hold too")
         rc.length = length
+        rc.common = min(rc.common, length // self.page_size)
         self._trim(rc, length)
+
+    def families(self, request_ids: Sequence[Hashable]) -> List[List[int]]:
+        """The requests' places in the sequence, family by family (requests that were forked from one another)."""
+        found: Dict[Hashable, List[int]] = {}
+        for i, rid in enumerate(request_ids):
+            found.setdefault(self.get(rid).family, []).append(i)
+        return list(found.values())
+
+    def common_blocks(self, request_ids: Sequence[Hashable], g: int) -> int:
+        """How many leading blocks requests of one family have alike in group g."""
+        rcs = [self.get(r) for r in request_ids]
+        blocks = [rc.tables[g].blocks for rc in rcs]
+        n, most = min(rc.common for rc in rcs), min(len(b) for b in blocks)
+        n = min(n, most)
+        while n < most and all(b[n] == blocks[0][n] for b in blocks[1:]):
+            n += 1
+        return n
 
     def _trim(self, rc: RequestCache, length: int) -> None:
         keep = -(-length // self.page_size)

@@ -454,6 +454,7 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
     for (int b = 0; b < 30; b++) if ((1 << b) == page_size) a.page_shift = b;
     a.scale_log2 = scale * 1.4426950408889634f;
     if (attention_shared_mma_takes(a, dtype)) {
+        if (attention_each_takes(a)) return launch_attention_each_mma(a, sms, stream);
         const int status = launch_attention_shared_mma(a, sms, stream);
         return status != VK_OK ? status : launch_join(a, dtype, stream);
     }

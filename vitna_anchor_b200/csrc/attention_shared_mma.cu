@@ -310,35 +310,45 @@ __device__ __forceinline__ void sm_walk_few(const SaArgs& a, const SaPart& part,
         for (int d = 4; d < 32; d <<= 1) x.l[h] += __shfl_xor_sync(0xffffffffu, x.l[h], d);
 }
 
-// The queries of up to eight rows of a part as the 8-column operand: lane (gq, qd) has row gq, dims 2 qd, the next and + 8 of each k step.
-template <int HD>
-__device__ __forceinline__ void sm_queries_few(const SaArgs& a, const SaPlan& p, const SaPart& part, uint32_t (&qb)[HD / 16][2]) {
-    const int lane = threadIdx.x & 31, rows = (part.i1 - part.i0) * part.heads, row = lane >> 2, i = part.i0 + row / part.heads;
-    const bool on = row < rows && p.pos[min(i, SA_MAX_TOKENS - 1)] >= 0;
-    const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (on ? ((size_t)p.tok[i] * a.nh + part.kvh * a.gq + part.h0 + row % part.heads) * HD : 0) + 2 * (lane & 3);
+// The queries of up to eight rows as the 8-column operand: lane (gq, qd) has row gq, dims 2 qd, the next and + 8 of each k step.  at(row): where its query lies, null for none (zeros).
+template <int HD, typename At>
+__device__ __forceinline__ void sm_queries_few(const At& at, uint32_t (&qb)[HD / 16][2]) {
+    const int lane = threadIdx.x & 31;
+    const __nv_bfloat16* q = at(lane >> 2);
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ks++) {
-        qb[ks][0] = on ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
-        qb[ks][1] = on ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
+        qb[ks][0] = q ? *reinterpret_cast<const uint32_t*>(q + 2 * (lane & 3) + ks * 16) : 0u;
+        qb[ks][1] = q ? *reinterpret_cast<const uint32_t*>(q + 2 * (lane & 3) + ks * 16 + 8) : 0u;
     }
 }
 
-// The queries of rows row0 + gq and row0 + gq + 8 of a part as the 16-row operand (zeros where there is no such row, or its member is not there).
-template <int HD>
-__device__ __forceinline__ void sm_queries(const SaArgs& a, const SaPlan& p, const SaPart& part, int row0, uint32_t (&qf)[HD / 16][4]) {
-    const int lane = threadIdx.x & 31, rows = (part.i1 - part.i0) * part.heads;
+// The same of rows row0 + gq and row0 + gq + 8 as the 16-row operand.
+template <int HD, typename At>
+__device__ __forceinline__ void sm_queries(const At& at, int row0, uint32_t (&qf)[HD / 16][4]) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-        const int row = row0 + (lane >> 2) + 8 * r, i = part.i0 + row / part.heads;
-        const bool on = row < rows && p.pos[min(i, SA_MAX_TOKENS - 1)] >= 0;
-        const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (on ? ((size_t)p.tok[i] * a.nh + part.kvh * a.gq + part.h0 + row % part.heads) * HD : 0) + 2 * (lane & 3);
+        const __nv_bfloat16* q = at(row0 + (lane >> 2) + 8 * r);
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ks++) {
-            qf[ks][r] = on ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
-            qf[ks][r + 2] = on ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
+            qf[ks][r] = q ? *reinterpret_cast<const uint32_t*>(q + 2 * (lane & 3) + ks * 16) : 0u;
+            qf[ks][r + 2] = q ? *reinterpret_cast<const uint32_t*>(q + 2 * (lane & 3) + ks * 16 + 8) : 0u;
         }
     }
 }
+
+// Where the query of a part's row lies; null: no such row, or its member is not there.
+struct SmQueryOf {
+    const SaArgs& a;
+    const SaPlan& p;
+    const SaPart& part;
+    int hd;
+    __device__ __forceinline__ const __nv_bfloat16* operator()(int row) const {
+        const int i = part.i0 + row / part.heads;
+        if (row >= (part.i1 - part.i0) * part.heads || p.pos[i] < 0) return nullptr;
+        return static_cast<const __nv_bfloat16*>(a.q) + ((size_t)p.tok[i] * a.nh + part.kvh * a.gq + part.h0 + row % part.heads) * hd;
+    }
+};
 
 // The outputs that a block's groups of R warps left in shared memory ([8 warps][16][HD + 4], maxima and sums behind them) meet, and the part's rows are written.
 template <int HD, int R>
@@ -378,7 +388,7 @@ __device__ __forceinline__ void sm_prefix(const SaArgs& a, const SaPlan& p, cons
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / R, wr = warp % R;
     const int rows = (part.i1 - part.i0) * part.heads;
     uint32_t qf[HD / 16][4];
-    sm_queries<HD>(a, p, part, wr * 16, qf);
+    sm_queries<HD>(SmQueryOf{a, p, part, HD}, wr * 16, qf);
     SmRows<HD> x;
     sm_walk<HD, R>(a, part, group, GROUPS, group, wr, qf, x, sm_addr(stages));
     if (GROUPS == 1) {
@@ -413,7 +423,7 @@ __device__ __forceinline__ void sm_prefix_few(const SaArgs& a, const SaPlan& p, 
     constexpr int LD = HD + 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t qb[HD / 16][2];
-    sm_queries_few<HD>(a, p, part, qb);
+    sm_queries_few<HD>(SmQueryOf{a, p, part, HD}, qb);
     SmFew<HD> x;
     sm_walk_few<HD>(a, part, warp, SA_THREADS / 32, warp, qb, x, sm_addr(stages));
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -473,7 +483,7 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
         __syncwarp();                                      // the lanes are past the tiles of the part before
         if (part.heads <= 8) {
             uint32_t qb[HD / 16][2];
-            sm_queries_few<HD>(a, p, part, qb);
+            sm_queries_few<HD>(SmQueryOf{a, p, part, HD}, qb);
             SmFew<HD> x;
             sm_walk_few<HD>(a, part, 0, 1, warp, qb, x, sm_addr(stages));
 #pragma unroll
@@ -490,7 +500,7 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
             }
         } else {
             uint32_t qf[HD / 16][4];
-            sm_queries<HD>(a, p, part, 0, qf);
+            sm_queries<HD>(SmQueryOf{a, p, part, HD}, 0, qf);
             SmRows<HD> x;
             sm_walk<HD, 1>(a, part, 0, 1, warp, 0, qf, x, sm_addr(stages));
 #pragma unroll
@@ -507,9 +517,166 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
     sa_write_rows(a, p);
 }
 
+// ---- every member by itself ---------------------------------------------------------------------------------------------------------------
+//
+// Where the members' tables are short and few, reading common keys once is worth less than what it takes to find out who has which in common and to bring the two kinds of parts
+// together: a cluster of blocks walks a member's whole table for one tile of heads, a run of its keys a block, its eight warps in turn, and the blocks' outputs meet through
+// each other's shared memory.  One launch, nothing in scratch memory.
+
+__device__ __forceinline__ uint32_t sm_of_rank(const void* p, int rank) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(sm_addr(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float sm_remote(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sm_cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int HD>
+__global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_each_mma_kernel(const SaArgs a) {
+    extern __shared__ __align__(128) unsigned char stages[];
+    constexpr int LD = HD + 4;
+    __shared__ float row_m[16], row_l[16];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = blockIdx.z, rank = blockIdx.x, ranks = gridDim.x;      // a cluster is a row of the grid
+    // from the step's metadata, which no kernel writes; the whole cluster has the same member
+    const int token = a.members[i];
+    const bool there = token >= 0 && token < a.tokens;
+    const int seg = there ? a.token_seg[token] : -1, at = there ? a.positions[token] : -1;
+    const bool behind = tid < a.families && a.starts[tid + 1] > i;
+    if (!__syncthreads_or(behind) || a.starts[0] > i || seg < 0 || seg >= a.segments || at < 0) return;
+    const int keys = (int)min((long long)at, (long long)a.max_blocks * a.page_size - 1) + 1;
+    const int own_tiles = (a.gq + 15) / 16, run = (sa_tiles(keys) + ranks - 1) / ranks * SA_TILE;
+    SaPart part;
+    part.kvh = blockIdx.y / own_tiles;
+    part.h0 = (blockIdx.y - part.kvh * own_tiles) * 16;
+    part.heads = min(16, a.gq - part.h0);
+    part.k0 = min(rank * run, keys);
+    part.k1 = min(part.k0 + run, keys);
+    part.table = a.block_tables + (size_t)seg * a.max_blocks;
+    const __nv_bfloat16* queries = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * HD;
+    auto query_of = [&](int row) -> const __nv_bfloat16* { return row < part.heads ? queries + row * HD : nullptr; };
+    float* out = reinterpret_cast<float*>(stages);                                        // the warps' outputs, over the stages: [8][16][LD]
+    float2 (*ml)[16] = reinterpret_cast<float2 (*)[16]>(stages + SmSmem<HD>::OUT);
+    float* whole = reinterpret_cast<float*>(stages + SmSmem<HD>::OUT + SmSmem<HD>::ML);      // and the block's: [16][HD]
+    static_assert(SmSmem<HD>::OUT + SmSmem<HD>::ML + 16 * HD * 4 <= SM_STAGES * SmSmem<HD>::STAGE, "the block's output lies behind the warps'");
+    dependency_wait();
+    let_dependents_start();
+    if (part.heads <= 8) {
+        uint32_t qb[HD / 16][2];
+        sm_queries_few<HD>(query_of, qb);
+        SmFew<HD> x;
+        sm_walk_few<HD>(a, part, warp, SA_THREADS / 32, warp, qb, x, sm_addr(stages));
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int row = 2 * (lane & 3) + h;
+#pragma unroll
+            for (int b = 0; b < HD / 16; b++) {
+                out[(warp * 16 + row) * LD + b * 16 + (lane >> 2)] = x.o[b][h];
+                out[(warp * 16 + row) * LD + b * 16 + (lane >> 2) + 8] = x.o[b][2 + h];
+            }
+            if (lane < 4) ml[warp][row] = make_float2(x.m[h], x.l[h]);
+        }
+    } else {
+        uint32_t qf[HD / 16][4];
+        sm_queries<HD>(query_of, 0, qf);
+        SmRows<HD> x;
+        sm_walk<HD, 1>(a, part, warp, SA_THREADS / 32, warp, 0, qf, x, sm_addr(stages));
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int row = (lane >> 2) + 8 * r;
+#pragma unroll
+            for (int b = 0; b < HD / 8; b++) *reinterpret_cast<float2*>(out + (warp * 16 + row) * LD + b * 8 + 2 * (lane & 3)) = make_float2(x.o[b][2 * r], x.o[b][2 * r + 1]);
+            if ((lane & 3) == 0) ml[warp][row] = make_float2(x.m[r], x.l[r]);
+        }
+    }
+    __syncthreads();
+    // the warps' outputs meet: against the block's largest reference
+    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * HD;
+#pragma unroll 1
+    for (int c = tid; c < part.heads * HD; c += SA_THREADS) {
+        const int row = c / HD, d = c % HD;
+        float m = -INFINITY, l = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < SA_THREADS / 32; w++) m = fmaxf(m, ml[w][row].x);
+        const float ref = m == -INFINITY ? 0.0f : m;      // no score above -inf: every weight is 0
+#pragma unroll
+        for (int w = 0; w < SA_THREADS / 32; w++) {
+            const float e = sa_ex2(ml[w][row].x - ref);
+            l += ml[w][row].y * e;
+            o += out[(w * 16 + row) * LD + d] * e;
+        }
+        if (ranks == 1) {
+            to[c] = __float2bfloat16_rn(o / l);
+        } else {
+            whole[c] = o;
+            if (d == 0) {
+                row_m[row] = m;
+                row_l[row] = l;
+            }
+        }
+    }
+    if (ranks == 1) return;
+    sm_cluster_meet();
+    // and the blocks': every block joins a share of the values
+#pragma unroll 1
+    for (int c = rank * SA_THREADS + tid; c < part.heads * HD; c += ranks * SA_THREADS) {
+        const int row = c / HD;
+        float m = -INFINITY, l = 0.0f, o = 0.0f, rm[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            rm[r] = r < ranks ? sm_remote(sm_of_rank(&row_m[row], r)) : -INFINITY;
+            m = fmaxf(m, rm[r]);
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            if (r >= ranks) break;
+            const float e = sa_ex2(rm[r] - ref);
+            l += sm_remote(sm_of_rank(&row_l[row], r)) * e;
+            o += sm_remote(sm_of_rank(&whole[c], r)) * e;
+        }
+        to[c] = __float2bfloat16_rn(o / l);
+    }
+    sm_cluster_meet();                                        // nobody leaves while another reads its shared memory
+}
+
 // Rows of the pool are counted in 32 bits here, and a row's largest score is that of its largest product.
 bool attention_shared_mma_takes(const SaArgs& a, int dtype) {
     return dtype == 1 && (a.hd == 64 || a.hd == 128) && a.scale_log2 > 0.0f && (long long)a.pages * 2 * a.nkv * a.page_size < 0x7fffffffLL;
+}
+
+// Every member by itself, where all tables at their full width are few bytes (what the members really have is on the device).  Measured on families of 2 to 64 members with up to 64
+// positions of their own, this way against the other: 2 x 2,048 positions (1.7B sizes, 35 MB) 10.0 us against 9.6, 4 x 512 (20 MB) 8.8 / 9.9, 8 x 512 (40 MB) 12.8 / 10.0, 16 x 128 (29 MB)
+// 8.1 / 12.2; 64 x 512 (135M sizes, 30 MB) 10.9 / 13.8, 4 x 512 (2 MB) 4.0 / 8.2; 64 x 512 (360M sizes, 50 MB) 14.7 / 14.9, 4 x 8,000 (41 MB) 15.2 / 10.6; 16 x 2,048 (16 heads of 128 over
+// 2, 35 MB) 17.1 / 14.5.  The other way costs more the more members there are.
+bool attention_each_takes(const SaArgs& a) {
+    return (long long)a.n * a.max_blocks * a.page_size * a.nkv * a.hd * 4 <= SA_EACH_BYTES + a.n * SA_EACH_MEMBER_BYTES;
+}
+// A block for every 256 keys of a table, but no more blocks than run at once, and clusters of at most eight (four where a block fills a multiprocessor).
+int launch_attention_each_mma(const SaArgs& a, int multiprocessors, cudaStream_t stream) {
+    const int units = a.nkv * ((a.gq + 15) / 16) * a.n, room = multiprocessors * (a.hd == 64 ? 2 : 1), most = a.hd == 64 ? 8 : 4;
+    int ranks = 1;
+    while (ranks < most && ranks * 256 < (long long)a.max_blocks * a.page_size && 2 * ranks * units <= room) ranks *= 2;
+    const dim3 grid(ranks, a.nkv * ((a.gq + 15) / 16), a.n);
+#define GO(HD)                                                                                                                                  \
+    do {                                                                                                                                        \
+        const int e = sa_allow_smem(attention_each_mma_kernel<HD>, SM_STAGES * SmSmem<HD>::STAGE);                                              \
+        if (e != VK_OK) return e;                                                                                                               \
+        return launch_dependent_cluster(attention_each_mma_kernel<HD>, grid, dim3(SA_THREADS), ranks, SM_STAGES * SmSmem<HD>::STAGE, stream, a); \
+    } while (0)
+    if (a.hd == 64) GO(64);
+    GO(128);
+#undef GO
 }
 
 int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream) {

@@ -15,6 +15,7 @@ from typing import Hashable, List, Optional, Sequence, Tuple
 import numpy as np
 import torch
 
+from .. import ops
 from ..cache.manager import CacheManager
 from ..cache.pages import UNMAPPED
 from ..parts.base import GroupMeta, StepContext, Workspace
@@ -174,15 +175,24 @@ class ContextBuilder:
         return ctx, (dev[s_rows] if R else None)
 
     # -- single tokens, padded to a fixed number of segments -----------------------------------------------
-    def families(self, requests: Sequence[Hashable]) -> Optional[List[List[int]]]:
-        """The requests' places in the batch, family by family (requests that were forked from one another); None where nobody shares."""
-        by_family = {}
-        for i, rid in enumerate(requests):
-            by_family.setdefault(self.cache.tables.get(rid).family, []).append(i)
-        return list(by_family.values()) if len(by_family) < len(requests) else None
+    def families(self, requests: Sequence[Hashable]) -> Optional[List[Tuple[List[int], List[int]]]]:
+        """What requests of a batch of single tokens hold in common: for every family its places in the batch and the positions it shares in each page
+        group (0 in groups with a window).  None where reading those once is not worth it (ops.attention_shared_pays)."""
+        tables, ps = self.cache.tables, self.page_size
+        by_family = tables.families(requests)
+        if len(by_family) == len(requests):
+            return None
+        out = [(f, [tables.common_blocks([requests[i] for i in f], g) * ps if len(f) > 1 and group.window == 0 else 0 for g, group in enumerate(self.cache.groups)])
+               for f in by_family]
+        positions = sum(tables.get(rid).length + 1 for rid in requests)
+        for g, group in enumerate(self.cache.groups):
+            saved = sum((len(f) - 1) * shared[g] for f, shared in out)
+            if ops.attention_shared_pays(len(requests), positions, saved, group.num_kv_heads, group.head_dim):
+                return out
+        return None
 
     def build_decode(self, requests: Sequence[Hashable], tokens: Sequence[int], B: int, views: bool = True, reach: int = 0,
-                     families: Optional[List[List[int]]] = None):
+                     families: Optional[List[Tuple[List[int], List[int]]]] = None):
         """The context of a batch of single tokens, padded to B segments, at offsets that depend on B alone, so
         that a captured graph finds every array where it was at capture.  A padding segment has one token at
         position 0 that writes nothing (slot mapping -1, state slot -1) and reads page 0.  views=False: only fill the buffer.
@@ -225,17 +235,12 @@ class ContextBuilder:
                 bt[i, :len(row)] = row
             if families:
                 o = o_families + g * (3 * B + 1)
-                order = [i for f in families for i in f] + list(range(S, B))
-                sizes = [len(f) for f in families] + [1] * (B - S)
+                order = [i for f, _ in families for i in f] + list(range(S, B))
+                sizes = [len(f) for f, _ in families] + [1] * (B - S)
                 buf[o:o + B] = order
                 buf[o + B + 1:o + B + 1 + len(sizes)] = np.cumsum(sizes)
                 buf[o + B + 1 + len(sizes):o + 2 * B + 1] = B
-                if self.cache.groups[g].window == 0:
-                    for k, f in enumerate(families):
-                        if len(f) > 1:
-                            n = min(len(rcs[i].tables[g].blocks) for i in f)
-                            apart = (bt[f[1:], :n] != bt[f[0], :n]).any(0)
-                            buf[o + 2 * B + 1 + k] = (int(apart.argmax()) if apart.any() else n) * ps
+                buf[o + 2 * B + 1:o + 2 * B + 1 + len(families)] = [shared[g] for _, shared in families]
         self._send(st, total)
         if not views:               # a replay needs the arrays in place, not their description
             return None, None

@@ -325,7 +325,7 @@ class ModelRunner:
         # bucket runs eagerly and is then captured (a stall of about two steps, once per bucket).
         longest = max(self.cache.tables.get(e.request_id).length for e in entries) + 1
         reach = self.context_bucket(longest, self.max_model_len)
-        # Requests that hold pages in common (and are not alone in their family) take the attention that reads those once: a graph of its own.
+        # Requests that hold enough in common take the attention that reads it once: a graph of its own.
         requests = [e.request_id for e in entries]
         families = self.builder.families(requests)
         key = (B, reach, families is not None)
