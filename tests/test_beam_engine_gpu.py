@@ -21,7 +21,7 @@ def dirs(tmp_path_factory):
     root = tmp_path_factory.mktemp("beam")
     made = {name: write_tiny(str(root / name), tiny, std=0.15) for name, tiny in TINIES.items()}
     for kv, hd in [(2, 64), (1, 128)]:
-        cfg = dict(TINIES["tinyA"]["config"], hidden_size=256, num_attention_heads=6, num_key_value_heads=kv, head_dim=hd, vocab_size=500, max_position_embeddings=8192)
+        cfg = dict(TINIES["tinyA"]["config"], hidden_size=256, num_attention_heads=6, num_key_value_heads=kv, head_dim=hd, vocab_size=500, max_position_embeddings=131072)
         made[f"heads{hd}"] = write_tiny(str(root / f"heads{hd}"), dict(TINIES["tinyA"], config=cfg), std=0.1)
     import importlib
     for name in OTHERS:
@@ -103,8 +103,8 @@ def test_search_matches_one_that_starts_over(name, dirs):
 def test_sums_are_those_of_the_sequences(name, graphs, dirs, shared_mode):
     """bfloat16: every result's sum of log probabilities is that of its sequence run from its start, as near as two ways of cutting one request come
     (8e-2 of the logits' scale at a position; the mean over a sequence is held to that)."""
-    # heads64 and heads128: tables so wide that the common keys are walked once, not every member by itself
-    wide = dict(kv_block=16, ctx=8192, num_pages=200) if name.startswith("heads") else {}
+    # heads64 and heads128: tables so wide that the common keys are walked once, not every member by itself (a search of six, heads of 64: 96 MB and more)
+    wide = dict(kv_block=16, ctx=65536, num_pages=200) if name.startswith("heads") else {}
     eng = _engine(dirs[name], "bfloat16", cuda_graphs=graphs, **wide)
     rng = np.random.default_rng(3)
     prompt = [int(t) for t in rng.integers(0, eng.model.vocab_size, 150 if name.startswith("heads") else 40)]
@@ -132,7 +132,7 @@ def test_forked_requests_give_the_logits_of_separate_ones(name, tol, dirs, share
     prompt, stranger = ([int(t) for t in rng.integers(0, V, n)] for n in (203, 30))
 
     def play(fork):
-        r = ModelRunner(model, page_size=16, max_requests=8, max_batch_tokens=512, num_pages=200)
+        r = ModelRunner(model, page_size=16, max_requests=8, max_batch_tokens=512, max_model_len=131072, num_pages=200)
         r.open("s")
         r.step([StepEntry("s", stranger, [])])
         for i in range(6):

@@ -67,7 +67,7 @@ class Batch:
         """wide: block tables so wide that the call does not walk every member by itself (where it can)."""
         i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
         if wide:
-            self.maxb = max(self.maxb, (256 << 20) // (max(1, len(self.members)) * self.ps * self.nkv * self.hd * 4) + 1)
+            self.maxb = max(self.maxb, (260 << 20) // (max(1, len(self.members)) * self.ps * self.nkv * self.hd * 4) + 1)
         self.d = dict(q=self.q.cuda(), cache=self.cache.cuda(), tables=i([t + [0x7fffffff] * (self.maxb - len(t)) for t in self.tables]), seg=i(list(range(len(self.pos)))),
                       pos=i(self.pos), members=i(self.members).reshape(-1), starts=i(self.starts), shared=i(self.shared))
         self.d["out"] = torch.full_like(self.d["q"], 7.0)

@@ -655,12 +655,13 @@ bool attention_shared_mma_takes(const SaArgs& a, int dtype) {
     return dtype == 1 && (a.hd == 64 || a.hd == 128) && a.scale_log2 > 0.0f && (long long)a.pages * 2 * a.nkv * a.page_size < 0x7fffffffLL;
 }
 
-// Every member by itself, where all tables at their full width are few bytes (what the members really have is on the device).  Measured on families of 2 to 64 members with up to 64
-// positions of their own, this way against the other: 2 x 2,048 positions (1.7B sizes, 35 MB) 10.0 us against 9.6, 4 x 512 (20 MB) 8.8 / 9.9, 8 x 512 (40 MB) 12.8 / 10.0, 16 x 128 (29 MB)
-// 8.1 / 12.2; 64 x 512 (135M sizes, 30 MB) 10.9 / 13.8, 4 x 512 (2 MB) 4.0 / 8.2; 64 x 512 (360M sizes, 50 MB) 14.7 / 14.9, 4 x 8,000 (41 MB) 15.2 / 10.6; 16 x 2,048 (16 heads of 128 over
-// 2, 35 MB) 17.1 / 14.5.  The other way costs more the more members there are.
+// Every member by itself, where all tables at their full width are few bytes (what the members really have is on the device).  Measured on families of 2 to 64 members, this way
+// against the other (bytes of the whole tables in brackets).  Heads of 64: 64 members of 512 common and up to 64 own positions, 5 key-value heads (48 MB), 8.9 us against 14.8;
+// 32 of 2,048, 5 heads (87 MB), 12.7 / 14.4; 8 of 2,048, 5 heads (44 MB), 6.6 / 9.8; 4 of 2,048, 32 heads (70 MB), 8.8 / 10.6; 16 of 512, 32 heads (78 MB), 10.3 / 11.3; 16 of 8,000, 3 heads
+// (99 MB), 13.8 / 12.7; 64 of 128, 32 heads (109 MB), 20.4 / 15.6; 8 of 2,048, 32 heads (139 MB), 12.7 / 11.4; 64 of 512, 32 heads (310 MB), 34 / 17.  Heads of 128 (2 of them, 8 queries
+// each): 16 of 8,000 (132 MB) 14.8 / 19.5, 64 of 2,048 (139 MB) 13.6 / 21.8, 32 of 8,000 (265 MB) 23.5 / 23.3, 64 of 8,000 (530 MB) 40 / 35.
 bool attention_each_takes(const SaArgs& a) {
-    return (long long)a.n * a.max_blocks * a.page_size * a.nkv * a.hd * 4 <= SA_EACH_BYTES + a.n * SA_EACH_MEMBER_BYTES;
+    return (long long)a.n * a.max_blocks * a.page_size * a.nkv * a.hd * 4 <= (a.hd == 64 ? 96ll << 20 : 240ll << 20);
 }
 // A block for every 256 keys of a table, but no more blocks than run at once, and clusters of at most eight (four where a block fills a multiprocessor).
 int launch_attention_each_mma(const SaArgs& a, int multiprocessors, cudaStream_t stream) {

@@ -287,7 +287,6 @@ template <typename... Args> inline int sa_allow_smem(void (*kernel)(Args...), si
 // attention_shared_mma.cu
 bool attention_shared_mma_takes(const SaArgs& a, int dtype);
 int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream);
-constexpr long long SA_EACH_BYTES = 20ll << 20, SA_EACH_MEMBER_BYTES = 600ll << 10;
 bool attention_each_takes(const SaArgs& a);
 int launch_attention_each_mma(const SaArgs& a, int multiprocessors, cudaStream_t stream);
 
