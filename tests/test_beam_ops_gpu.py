@@ -129,7 +129,7 @@ SHAPES = [
 ]
 
 
-@pytest.mark.parametrize("dtype,wide", [(BF16, True), (BF16, False), (F32, True)])
+@pytest.mark.parametrize("dtype,wide", [(BF16, True), (BF16, False), (F32, True), (F32, False)])
 @pytest.mark.parametrize("n", range(len(SHAPES)))
 def test_attention_shared(ops, dtype, wide, n):
     families, nh, nkv, hd, ps = SHAPES[n]
@@ -141,7 +141,7 @@ def test_attention_shared(ops, dtype, wide, n):
     Batch(families, nh, nkv, hd, ps, dtype, seed=n).device(wide).check(ops)
 
 
-@pytest.mark.parametrize("dtype,hd,wide", [(BF16, 64, True), (BF16, 128, True), (BF16, 64, False), (BF16, 128, False), (F32, 64, True)])
+@pytest.mark.parametrize("dtype,hd,wide", [(BF16, 64, True), (BF16, 128, True), (BF16, 64, False), (BF16, 128, False), (F32, 64, True), (F32, 64, False)])
 def test_attention_shared_random_families(ops, dtype, hd, wide):
     """Many layouts through ONE scratch of exactly the bytes of the largest, with guards around it."""
     rng = random.Random(11)

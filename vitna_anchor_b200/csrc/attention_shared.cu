@@ -269,6 +269,77 @@ __global__ void __launch_bounds__(SA_THREADS, DIMS == 2 ? 2 : 1) attention_share
     sa_write_rows(a, p);
 }
 
+// ---- every member by itself, see attention_shared_mma.cu: a block of four warps, eight heads, a run of its keys ------------------------------------------------------
+
+constexpr int SE_WARPS = 4;
+// Shared memory: the queries [8][hd], the warps' weights [4][8][32], the warps' keys and values [32][hd + 4] (the warps' outputs [4][8][hd] later), the block's output [8][hd].
+__host__ __device__ inline int se_walkers(int hd) { return hd <= 128 ? 4 : 2; }
+static size_t se_smem(int hd) { return (size_t)2 * SG_ROWS * hd * 4 + SE_WARPS * SG_ROWS * SG_KEYS * 4 + (size_t)se_walkers(hd) * 2 * SG_KEYS * (hd + 4) * 4; }
+
+template <typename T, int DIMS, int NR>
+__device__ __forceinline__ void se_walk(const SaArgs& a, const SaPart& part, const SgRows& w, float* out, float2* ml) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, walkers = se_walkers(a.hd);
+    float m[NR], l[NR], o[NR][DIMS];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DIMS; d++) o[r][d] = 0.0f;
+    }
+    if (warp < walkers) sg_walk<T, DIMS, NR>(a, part, warp, walkers, w, m, l, o);
+    __syncthreads();                                        // everybody is past the keys and values
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+#pragma unroll
+        for (int d = 0; d < DIMS; d++)
+            if (lane + 32 * d < a.hd) out[(warp * SG_ROWS + r) * a.hd + lane + 32 * d] = o[r][d];
+        if (lane == 0) ml[warp * SG_ROWS + r] = make_float2(m[r], l[r]);
+    }
+    __syncthreads();
+}
+
+template <typename T, int DIMS>
+__global__ void __launch_bounds__(SE_WARPS * 32) attention_each_kernel(const SaArgs a) {
+    constexpr int N = Vec16<T>::N;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float row_m[SG_ROWS], row_l[SG_ROWS];
+    __shared__ float2 ml[SE_WARPS * SG_ROWS];
+    float* sq = reinterpret_cast<float*>(smem);
+    float* whole = sq + SG_ROWS * a.hd;
+    float* weights = whole + SG_ROWS * a.hd;
+    float* tiles = weights + SE_WARPS * SG_ROWS * SG_KEYS;
+    const int warp = threadIdx.x >> 5, vec = a.hd / N;
+    SaPart part;
+    int token;
+    if (!sa_each_part(a, SG_ROWS, part, token)) return;
+    dependency_wait();
+    let_dependents_start();
+    const T* q = static_cast<const T*>(a.q) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * a.hd;
+    for (int c = threadIdx.x; c < SG_ROWS * vec; c += SE_WARPS * 32) {
+        const int r = c / vec, d = c % vec * N;
+        float f[N];
+        if (r < part.heads) load16<T>(q + r * a.hd + d, f);
+        else
+#pragma unroll
+            for (int e = 0; e < N; e++) f[e] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; e++) sq[r * a.hd + d + e] = f[e] * a.scale_log2;
+    }
+    __syncthreads();
+    SgRows w;
+    w.q = sq;
+    w.weights = weights + warp * SG_ROWS * SG_KEYS;
+    w.k = tiles + (size_t)min(warp, se_walkers(a.hd) - 1) * 2 * SG_KEYS * (a.hd + 4);
+    w.v = w.k + SG_KEYS * (a.hd + 4);
+    w.warps = 1;
+    w.place = w.barrier = 0;
+    if (part.heads == 1) se_walk<T, DIMS, 1>(a, part, w, tiles, ml);
+    else if (part.heads <= 4) se_walk<T, DIMS, 4>(a, part, w, tiles, ml);
+    else se_walk<T, DIMS, 8>(a, part, w, tiles, ml);
+    sa_each_join<T, SE_WARPS>(a, part, token, SG_ROWS, a.hd, tiles, ml, whole, row_m, row_l);
+}
+
 // A row's parts meet: weights 2^(own maximum - row maximum), sums in the parts' order within a lane, then over the lanes, then over the warps, the same in every launch of
 // the same lengths.  WARPS warps a row: one where the rows alone fill the machine, four where few rows have many parts.  A part's row is read as 16-byte pieces by
 // L = 2, 4 .. 32 neighbouring lanes, 32 / L parts at once and four of those in flight.
@@ -391,6 +462,37 @@ static int launch_join(const SaArgs& a, int dtype, cudaStream_t stream) {
 #undef GO
 }
 
+// Where: tables of up to 64 MB together at their full width, none longer than 256 positions a block of the largest cluster.  Measured in float32, this way against the other: 8 members of 512
+// common and up to 64 own positions at 3 key-value heads of 64 (7 MB) 9.7 us against 16.6, 64 of 512 (58 MB) 29.8 / 30.7, 24 of 512 and up to 600 (42 MB) 24.0 / 25.9, 64 of 512 at 5 heads
+// (97 MB) 55 / 37; 8 of 512 at 32 heads (78 MB) 25 / 27, 24 of 512 (233 MB) 72 / 37; 2 of 2,048 at 3 heads (6 MB) 16.3 / 14.4, of 8,000 (25 MB) 41 / 17; 8 of 512 at 2 heads of 128, eight queries
+// each (10 MB), 23 / 38, of 2,048 (35 MB) 52 / 39.
+static int each_most(const SaArgs& a) { return a.hd <= 64 ? 8 : 4; }
+static bool each_takes(const SaArgs& a, int dtype) {
+    const long long reach = (long long)a.max_blocks * a.page_size;
+    return reach <= 256 * each_most(a) && a.n * reach * a.nkv * a.hd * 2 * (dtype == 0 ? 4 : 2) <= 64ll << 20;
+}
+static int launch_each(const SaArgs& a, int dtype, int multiprocessors, cudaStream_t stream) {
+    const int tiles = a.nkv * ((a.gq + SG_ROWS - 1) / SG_ROWS), room = multiprocessors * (a.hd <= 64 ? 2 : 1);
+    int ranks = 1;
+    while (ranks < each_most(a) && ranks * 128 < (long long)a.max_blocks * a.page_size && 2 * ranks * tiles * a.n <= room) ranks *= 2;
+    const size_t smem = se_smem(a.hd);
+#define GO(T, DIMS)                                                                                                                      \
+    do {                                                                                                                                 \
+        const int e = sa_allow_smem(attention_each_kernel<T, DIMS>, smem);                                                               \
+        if (e != VK_OK) return e;                                                                                                        \
+        return launch_dependent_cluster(attention_each_kernel<T, DIMS>, dim3(ranks, tiles, a.n), dim3(SE_WARPS * 32), ranks, smem, stream, a); \
+    } while (0)
+    if (dtype == 0) {
+        if (a.hd <= 64) GO(float, 2);
+        if (a.hd <= 128) GO(float, 4);
+        GO(float, 8);
+    }
+    if (a.hd <= 64) GO(__nv_bfloat16, 2);
+    if (a.hd <= 128) GO(__nv_bfloat16, 4);
+    GO(__nv_bfloat16, 8);
+#undef GO
+}
+
 // The current device's multiprocessors, asked for once a device.
 static int sa_multiprocessors() {
     static std::atomic<int> known[64];
@@ -454,10 +556,11 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
     for (int b = 0; b < 30; b++) if ((1 << b) == page_size) a.page_shift = b;
     a.scale_log2 = scale * 1.4426950408889634f;
     if (attention_shared_mma_takes(a, dtype)) {
-        if (attention_each_takes(a)) return launch_attention_each_mma(a, sms, stream);
+        if (attention_each_mma_takes(a)) return launch_attention_each_mma(a, sms, stream);
         const int status = launch_attention_shared_mma(a, sms, stream);
         return status != VK_OK ? status : launch_join(a, dtype, stream);
     }
+    if (each_takes(a, dtype)) return launch_each(a, dtype, sms, stream);
     a.prefix_rows = SG_PREFIX_ROWS;
     a.own_rows = SG_ROWS;
     a.row_unit = 16.0f;

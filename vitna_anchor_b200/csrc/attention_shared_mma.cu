@@ -523,42 +523,15 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
 // together: a cluster of blocks walks a member's whole table for one tile of heads, a run of its keys a block, its eight warps in turn, and the blocks' outputs meet through
 // each other's shared memory.  One launch, nothing in scratch memory.
 
-__device__ __forceinline__ uint32_t sm_of_rank(const void* p, int rank) {
-    uint32_t at;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(sm_addr(p)), "r"(rank));
-    return at;
-}
-__device__ __forceinline__ float sm_remote(uint32_t at) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ void sm_cluster_meet() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 template <int HD>
 __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_each_mma_kernel(const SaArgs a) {
     extern __shared__ __align__(128) unsigned char stages[];
     constexpr int LD = HD + 4;
     __shared__ float row_m[16], row_l[16];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = blockIdx.z, rank = blockIdx.x, ranks = gridDim.x;      // a cluster is a row of the grid
-    // from the step's metadata, which no kernel writes; the whole cluster has the same member
-    const int token = a.members[i];
-    const bool there = token >= 0 && token < a.tokens;
-    const int seg = there ? a.token_seg[token] : -1, at = there ? a.positions[token] : -1;
-    const bool behind = tid < a.families && a.starts[tid + 1] > i;
-    if (!__syncthreads_or(behind) || a.starts[0] > i || seg < 0 || seg >= a.segments || at < 0) return;
-    const int keys = (int)min((long long)at, (long long)a.max_blocks * a.page_size - 1) + 1;
-    const int own_tiles = (a.gq + 15) / 16, run = (sa_tiles(keys) + ranks - 1) / ranks * SA_TILE;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     SaPart part;
-    part.kvh = blockIdx.y / own_tiles;
-    part.h0 = (blockIdx.y - part.kvh * own_tiles) * 16;
-    part.heads = min(16, a.gq - part.h0);
-    part.k0 = min(rank * run, keys);
-    part.k1 = min(part.k0 + run, keys);
-    part.table = a.block_tables + (size_t)seg * a.max_blocks;
+    int token;
+    if (!sa_each_part(a, 16, part, token)) return;                                        // from the step's metadata, which no kernel writes
     const __nv_bfloat16* queries = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * HD;
     auto query_of = [&](int row) -> const __nv_bfloat16* { return row < part.heads ? queries + row * HD : nullptr; };
     float* out = reinterpret_cast<float*>(stages);                                        // the warps' outputs, over the stages: [8][16][LD]
@@ -600,54 +573,7 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_each_m
         }
     }
     __syncthreads();
-    // the warps' outputs meet: against the block's largest reference
-    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(a.out) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * HD;
-#pragma unroll 1
-    for (int c = tid; c < part.heads * HD; c += SA_THREADS) {
-        const int row = c / HD, d = c % HD;
-        float m = -INFINITY, l = 0.0f, o = 0.0f;
-#pragma unroll
-        for (int w = 0; w < SA_THREADS / 32; w++) m = fmaxf(m, ml[w][row].x);
-        const float ref = m == -INFINITY ? 0.0f : m;      // no score above -inf: every weight is 0
-#pragma unroll
-        for (int w = 0; w < SA_THREADS / 32; w++) {
-            const float e = sa_ex2(ml[w][row].x - ref);
-            l += ml[w][row].y * e;
-            o += out[(w * 16 + row) * LD + d] * e;
-        }
-        if (ranks == 1) {
-            to[c] = __float2bfloat16_rn(o / l);
-        } else {
-            whole[c] = o;
-            if (d == 0) {
-                row_m[row] = m;
-                row_l[row] = l;
-            }
-        }
-    }
-    if (ranks == 1) return;
-    sm_cluster_meet();
-    // and the blocks': every block joins a share of the values
-#pragma unroll 1
-    for (int c = rank * SA_THREADS + tid; c < part.heads * HD; c += ranks * SA_THREADS) {
-        const int row = c / HD;
-        float m = -INFINITY, l = 0.0f, o = 0.0f, rm[8];
-#pragma unroll
-        for (int r = 0; r < 8; r++) {
-            rm[r] = r < ranks ? sm_remote(sm_of_rank(&row_m[row], r)) : -INFINITY;
-            m = fmaxf(m, rm[r]);
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int r = 0; r < 8; r++) {
-            if (r >= ranks) break;
-            const float e = sa_ex2(rm[r] - ref);
-            l += sm_remote(sm_of_rank(&row_l[row], r)) * e;
-            o += sm_remote(sm_of_rank(&whole[c], r)) * e;
-        }
-        to[c] = __float2bfloat16_rn(o / l);
-    }
-    sm_cluster_meet();                                        // nobody leaves while another reads its shared memory
+    sa_each_join<__nv_bfloat16, SA_THREADS / 32>(a, part, token, 16, LD, out, &ml[0][0], whole, row_m, row_l);
 }
 
 // Rows of the pool are counted in 32 bits here, and a row's largest score is that of its largest product.
@@ -660,7 +586,7 @@ bool attention_shared_mma_takes(const SaArgs& a, int dtype) {
 // 32 of 2,048, 5 heads (87 MB), 12.7 / 14.4; 8 of 2,048, 5 heads (44 MB), 6.6 / 9.8; 4 of 2,048, 32 heads (70 MB), 8.8 / 10.6; 16 of 512, 32 heads (78 MB), 10.3 / 11.3; 16 of 8,000, 3 heads
 // (99 MB), 13.8 / 12.7; 64 of 128, 32 heads (109 MB), 20.4 / 15.6; 8 of 2,048, 32 heads (139 MB), 12.7 / 11.4; 64 of 512, 32 heads (310 MB), 34 / 17.  Heads of 128 (2 of them, 8 queries
 // each): 16 of 8,000 (132 MB) 14.8 / 19.5, 64 of 2,048 (139 MB) 13.6 / 21.8, 32 of 8,000 (265 MB) 23.5 / 23.3, 64 of 8,000 (530 MB) 40 / 35.
-bool attention_each_takes(const SaArgs& a) {
+bool attention_each_mma_takes(const SaArgs& a) {
     return (long long)a.n * a.max_blocks * a.page_size * a.nkv * a.hd * 4 <= (a.hd == 64 ? 96ll << 20 : 240ll << 20);
 }
 // A block for every 256 keys of a table, but no more blocks than run at once, and clusters of at most eight (four where a block fills a multiprocessor).

@@ -264,6 +264,96 @@ __device__ __forceinline__ float sa_ex2(float x) {
     return y;
 }
 
+// For the launches that walk every member by itself, in clusters: what another block of the cluster has in its shared memory.
+__device__ __forceinline__ uint32_t sa_of_rank(const void* p, int rank) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float sa_remote(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sa_cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The member, tile of `rows` heads and run of keys of a block of such a launch (grid: blocks of a cluster, tiles of heads of every key-value head, members); false: nothing of it is there, for the
+// whole cluster alike.
+__device__ __forceinline__ bool sa_each_part(const SaArgs& a, int rows, SaPart& part, int& token) {
+    const int i = blockIdx.z, tid = threadIdx.x, ranks = gridDim.x;
+    token = a.members[i];
+    const bool there = token >= 0 && token < a.tokens;
+    const int seg = there ? a.token_seg[token] : -1, at = there ? a.positions[token] : -1;
+    bool behind = false;
+    for (int f = tid; f < a.families; f += blockDim.x) behind |= a.starts[f + 1] > i;
+    if (!__syncthreads_or(behind) || a.starts[0] > i || seg < 0 || seg >= a.segments || at < 0) return false;
+    const int keys = (int)min((long long)at, (long long)a.max_blocks * a.page_size - 1) + 1;
+    const int tiles = (a.gq + rows - 1) / rows, run = (sa_tiles(keys) + ranks - 1) / ranks * SA_TILE;
+    part.kvh = blockIdx.y / tiles;
+    part.h0 = (blockIdx.y - part.kvh * tiles) * rows;
+    part.heads = min(rows, a.gq - part.h0);
+    part.k0 = min((int)blockIdx.x * run, keys);
+    part.k1 = min(part.k0 + run, keys);
+    part.table = a.block_tables + (size_t)seg * a.max_blocks;
+    return true;
+}
+
+// The outputs of a block's warps ([warps][rows][ld], maxima and sums [warps][rows]) meet, and then the cluster's blocks': `whole` [rows][hd], row_m and row_l [rows] are this block's for the others.
+// No score above -inf anywhere: every weight is 0, and the result no number.
+template <typename T, int WARPS>
+__device__ __forceinline__ void sa_each_join(const SaArgs& a, const SaPart& part, int token, int rows, int ld, const float* out, const float2* ml, float* whole, float* row_m, float* row_l) {
+    const int tid = threadIdx.x, ranks = gridDim.x, hd = a.hd, values = part.heads * hd;
+    T* to = static_cast<T*>(a.out) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * hd;
+#pragma unroll 1
+    for (int c = tid; c < values; c += WARPS * 32) {
+        const int row = c / hd, d = c - row * hd;
+        float m = -INFINITY, l = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) m = fmaxf(m, ml[w * rows + row].x);
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const float e = sa_ex2(ml[w * rows + row].x - ref);
+            l += ml[w * rows + row].y * e;
+            o += out[(w * rows + row) * ld + d] * e;
+        }
+        if (ranks == 1) {
+            to[c] = from_f32<T>(o / l);
+        } else {
+            whole[c] = o;
+            if (d == 0) {
+                row_m[row] = m;
+                row_l[row] = l;
+            }
+        }
+    }
+    if (ranks == 1) return;
+    sa_cluster_meet();
+#pragma unroll 1
+    for (int c = blockIdx.x * WARPS * 32 + tid; c < values; c += ranks * WARPS * 32) {      // every block a share of the values
+        const int row = c / hd;
+        float m = -INFINITY, l = 0.0f, o = 0.0f, rm[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            rm[r] = r < ranks ? sa_remote(sa_of_rank(&row_m[row], r)) : -INFINITY;
+            m = fmaxf(m, rm[r]);
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            if (r >= ranks) break;
+            const float e = sa_ex2(rm[r] - ref);
+            l += sa_remote(sa_of_rank(&row_l[row], r)) * e;
+            o += sa_remote(sa_of_rank(&whole[c], r)) * e;
+        }
+        to[c] = from_f32<T>(o / l);
+    }
+    sa_cluster_meet();                                        // nobody leaves while another reads its shared memory
+}
+
 constexpr int SA_MAX_MULTIPROCESSORS = 160;         // of the sm_100a parts; the scratch is laid out for this many
 
 // Allows a kernel more than 48 KB of shared memory on the current device, asked for again only where a launch needs more than was allowed before.
@@ -287,7 +377,7 @@ template <typename... Args> inline int sa_allow_smem(void (*kernel)(Args...), si
 // attention_shared_mma.cu
 bool attention_shared_mma_takes(const SaArgs& a, int dtype);
 int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream);
-bool attention_each_takes(const SaArgs& a);
+bool attention_each_mma_takes(const SaArgs& a);
 int launch_attention_each_mma(const SaArgs& a, int multiprocessors, cudaStream_t stream);
 
 }  // namespace vk
