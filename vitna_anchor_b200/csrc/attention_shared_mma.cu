@@ -3,15 +3,23 @@
 // The mathematics and the cut into parts are attention_shared.cu's and attention_shared_plan.cuh's.  A part's rows (a family's members times the heads
 // that read one key-value head) are the 16-row operands of m16n8k16 products, 16 rows a warp; R = 1, 2, 4 or 8 warps that cover a part's rows
 // make a group that works through the same keys, and the block's 8 / R groups take turns at the tiles of 16 R keys.  So a block holds up to 128 rows
-// against keys that are read once, and with few rows all eight warps still read keys of their own.
+// against keys that are read once, and with few rows all eight warps still read keys of their own.  Up to eight rows turn the products over: the keys are the 16 rows and
+// the rows the eight columns, half the products and half the exponentials.
 //
-//   copy      three stages of 128 keys and values a block by cp.async, each warp asks for 16 keys of its group's tile and the group meets once a tile;
-//             16-byte pieces are stored at piece ^ (key & 7), so that ldmatrix meets no bank twice
+//   copy      three stages of 128 keys and values a block by cp.async, each warp asks for 16 keys of its group's tile and the group meets once a tile; the page of the tile after
+//             next is asked for a tile before its number is used.  16-byte pieces are stored at piece ^ (key & 7), so that ldmatrix meets no bank twice
 //   scores    S = Q K^T, the queries in registers
-//   softmax   a running maximum and sum a row, float32, in base 2; the output is scaled only when a row's maximum rose
-//   p v       the probabilities go from the score registers into the 16-row operand as a high and a low bfloat16 part (p to 2^-17)
+//   softmax   against a reference maximum that follows only when a score is 2^8 above it, sums in float32
+//   p v       the weights go from the score registers into the next product's operand as a high and a low bfloat16 part (p to 2^-17): one part alone would double the error
+//             that the output's own rounding makes
 //
-// A member's own keys are walked by single warps with the same routine (R = 1): up to 16 rows of heads.
+// A member's own keys are walked by single warps with the same routines (R = 1): up to 16 rows of heads.
+//
+// What bounds it.  64 requests behind 6,000 positions with up to 700 of their own, 32 heads of 64 (214 MB): 49 us, 4.4 TB/s; the common keys' blocks do 64 rows a key, 16,000 cycles of the tensor
+// cores' legacy path, and take 37,000 (a group's warps do scores, softmax and p v in step, 4 warps a scheduler), while the own keys' blocks beside them wait for memory.  One kind after the
+// other in every block: 57 us.  16 requests behind 32,000 positions, 16 heads of 128 over 2 (36 MB): 36 us; 128 rows a key are 21,000 cycles of products at best and take 39,000 with two warps a
+// scheduler (that many outputs fill the registers).  Eight beams of 2,048 positions, 32 heads of 64 (20 MB): 11.6 us, of which finding the parts is 2 (it runs before the wait for the kernel
+// before) and joining them 3.
 #include "attention_shared_plan.cuh"
 
 namespace vk {
@@ -521,7 +529,8 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
 //
 // Where the members' tables are short and few, reading common keys once is worth less than what it takes to find out who has which in common and to bring the two kinds of parts
 // together: a cluster of blocks walks a member's whole table for one tile of heads, a run of its keys a block, its eight warps in turn, and the blocks' outputs meet through
-// each other's shared memory.  One launch, nothing in scratch memory.
+// each other's shared memory.  One launch, nothing in scratch memory.  Four beams of 512 positions, 9 heads over 3 of 64: 4.0 us (8.2 the other way); the launch, five dependent trips to
+// memory and the cluster's two meetings are all of it.
 
 template <int HD>
 __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_each_mma_kernel(const SaArgs a) {

@@ -3,7 +3,8 @@
 // What a beam search does to the cache between two steps: a page pool's layers get a copy of the page that two beams would go on writing into, the slots of a
 // recurrent model the state of the beam that was chosen.  No row is both read and written, which the caller sees to, so the
 // blocks need no order.  Reads and writes of the moved bytes are all there is: a block moves 16 KB, four 16-byte pieces a thread asked for before
-// the first is stored.  The moves are arguments of the launch (up to 128 at a time): nothing is copied to the device for them.
+// the first is stored.  The moves are arguments of the launch (up to 128 at a time): nothing is copied to the device for them.  Seven states of 1 MB in
+// twelve layers (176 MB read and written): 22.5 us, 7.8 TB/s (the second-level cache holds part of them); three pages of 12 KB in thirty layers: 1.2 us, and the host's call 7.
 #include "common.cuh"
 
 namespace vk {
