@@ -191,12 +191,10 @@ def test_who_takes_over_whom():
 def test_when_common_pages_are_read_once():
     """The rule's two sides (positions of 32 heads of 64: 8 KB; of 3: 0.75 KB), and the switch."""
     pays = ops.attention_shared_pays
-    assert not pays(4, 4 * 576, 3 * 512, 32, 64) and pays(8, 8 * 576, 7 * 512, 32, 64)
-    assert not pays(64, 64 * 576, 63 * 512, 3, 64) and pays(64, 64 * 2112, 63 * 2048, 3, 64)
-    assert not pays(8, 8 * 2000, 7 * 512, 32, 64) and not pays(8, 8 * 576, 0, 32, 64)
+    assert not pays(3 * 2000, 32, 64) and pays(7 * 2000, 32, 64) and not pays(63 * 500, 3, 64) and pays(63 * 4000, 3, 64) and not pays(0, 32, 64)
     for mode, taken in [(0, False), (1, True)]:
         assert ops.set_attention_shared(mode) == 2
-        assert pays(2, 20, 8, 1, 16) == taken and not pays(2, 20, 0, 1, 16)
+        assert pays(8, 1, 16) == taken and not pays(0, 1, 16)
         assert ops.set_attention_shared(2) == mode
 
 

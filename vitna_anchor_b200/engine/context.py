@@ -184,10 +184,9 @@ class ContextBuilder:
             return None
         out = [(f, [tables.common_blocks([requests[i] for i in f], g) * ps if len(f) > 1 and group.window == 0 else 0 for g, group in enumerate(self.cache.groups)])
                for f in by_family]
-        positions = sum(tables.get(rid).length + 1 for rid in requests)
         for g, group in enumerate(self.cache.groups):
             saved = sum((len(f) - 1) * shared[g] for f, shared in out)
-            if ops.attention_shared_pays(len(requests), positions, saved, group.num_kv_heads, group.head_dim):
+            if ops.attention_shared_pays(saved, group.num_kv_heads, group.head_dim):
                 return out
         return None
 

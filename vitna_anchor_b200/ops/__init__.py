@@ -2292,14 +2292,14 @@ def set_attention_shared(mode: int) -> int:
     return before
 
 
-def attention_shared_pays(requests: int, positions: int, saved: int, nkv: int, hd: int) -> bool:
-    """Whether a step's requests, `positions` cached positions together of which `saved` would be read again and again, go through attention_shared rather than
-    attention_decode: where the whole is more than 20 MB and 0.6 MB a request (in bfloat16; below, the split-key kernel was measured to be the faster one: 8.9 us against 9.9 for 4 requests of
-    576 positions at 32 heads of 64, 12.7 against 10.0 for 8 of them; 10.9 / 13.8 for 64 of 576 at 3 heads) and a quarter of it is saved."""
+def attention_shared_pays(saved: int, nkv: int, hd: int) -> bool:
+    """Whether a decode step whose requests would read `saved` cached positions again and again goes through attention_shared rather than attention_decode: from 64 MB of
+    them on (bfloat16).  Whole steps of a beam search, this way against the other: 8 beams of 2,000 positions, 32 heads of 64 over 24 layers (115 MB), 1.70 ms against 1.84, 64 of 8,000
+    (4.1 GB) 4.5 / 16.0; 16 of 4,000, 5 heads, 32 layers (77 MB) 1.68 / 1.72; 4 of 2,000, 32 heads (49 MB) 1.61 / 1.49, 16 of 500 (61 MB) 1.77 / 1.71; 32 of 500, 3 heads, 30 layers
+    (12 MB) 1.38 / 1.20.  Below, at 3 and 5 heads and 4,000 positions and more, up to 0.2 ms of 1.4 are left."""
     if _shared_mode != 2:
         return _shared_mode == 1 and saved > 0
-    each = nkv * hd * 4
-    return 4 * saved >= positions and positions * each > (20 << 20) + requests * (600 << 10)
+    return saved * nkv * hd * 4 >= 64 << 20
 
 
 def attention_shared_scratch_bytes(tokens: int, nh: int, nkv: int, hd: int) -> int:
