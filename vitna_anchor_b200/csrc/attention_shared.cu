@@ -312,7 +312,10 @@ __global__ void __launch_bounds__(SE_WARPS * 32) attention_each_kernel(const SaA
     const int warp = threadIdx.x >> 5, vec = a.hd / N;
     SaPart part;
     int token;
-    if (!sa_each_part(a, SG_ROWS, part, token)) return;
+    if (!sa_each_part(a, SG_ROWS, part, token)) {
+        dependency_wait();                                  // (the kernel after this one may take it that the one before has finished)
+        return;
+    }
     dependency_wait();
     let_dependents_start();
     const T* q = static_cast<const T*>(a.q) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * a.hd;

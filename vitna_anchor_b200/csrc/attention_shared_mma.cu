@@ -540,7 +540,10 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_each_m
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     SaPart part;
     int token;
-    if (!sa_each_part(a, 16, part, token)) return;                                        // from the step's metadata, which no kernel writes
+    if (!sa_each_part(a, 16, part, token)) {                                              // from the step's metadata, which no kernel writes
+        dependency_wait();                                                                // (the kernel after this one may take it that the one before has finished)
+        return;
+    }
     const __nv_bfloat16* queries = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * HD;
     auto query_of = [&](int row) -> const __nv_bfloat16* { return row < part.heads ? queries + row * HD : nullptr; };
     float* out = reinterpret_cast<float*>(stages);                                        // the warps' outputs, over the stages: [8][16][LD]
