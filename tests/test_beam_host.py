@@ -129,6 +129,22 @@ def test_forks_and_adoptions_keep_everybodys_positions(seed):
     assert [p.free_pages for p in t.pools] == [60, 60]
 
 
+def test_a_name_that_is_used_again_begins_a_family_of_its_own():
+    t = PageTables([PageGroup((0,), 1, 8, 0)], 2, [20], 4)
+    t.open("a")
+    t.reserve("a", 6)
+    t.commit("a")
+    t.fork("a", "b")
+    assert t.families(["a", "b"]) == [[0, 1]] and t.common_blocks(["a", "b"], 0) == 3
+    t.close("a")
+    t.open("a")
+    t.reserve("a", 6)
+    t.commit("a")
+    assert not set(t.get("a").tables[0].blocks) & set(t.get("b").tables[0].blocks)
+    assert t.families(["a", "b"]) == [[0], [1]]
+    t.check()
+
+
 def test_what_fork_and_adopt_refuse():
     t = PageTables([PageGroup((0,), 1, 8, 0)], 4, [5], 3)
     t.open("a")

@@ -19,6 +19,7 @@ all-ones).  The paging here is this engine's own.
 """
 from __future__ import annotations
 
+import itertools
 from dataclasses import dataclass, field
 from typing import Dict, Hashable, List, Optional, Sequence
 
@@ -151,7 +152,7 @@ class RequestCache:
     slot: int
     length: int = 0                # positions whose keys and values are in the cache (committed)
     reserved: int = 0              # positions reserved beyond `length` for the step in flight
-    family: Hashable = None        # the request this one's pages began with: its own id, or that of the request it was forked from
+    family: int = 0                # a number of its own, or that of the request it goes on from (ids may be used again, families are not)
     common: int = 1 << 30          # at least so many leading blocks it has in common with all of its family (no limit while it is alone)
     tables: Dict[int, GroupTable] = field(default_factory=dict)   # group index -> table
 
@@ -178,6 +179,7 @@ class PageTables:
         self.pools = [PagePool(n) for n in pages_per_group]
         self.slots = SlotPool(max_requests)
         self.requests: Dict[Hashable, RequestCache] = {}
+        self._families = itertools.count()
 
     # -- requests ---------------------------------------------------------------------------
     def open(self, request_id: Hashable) -> RequestCache:
@@ -185,7 +187,7 @@ class PageTables:
             raise CacheError(f"request {request_id!r} is already open")
         rc = RequestCache(request_id, self.slots.acquire(request_id))
         rc.tables = {g: GroupTable() for g in range(len(self.groups))}
-        rc.family = request_id
+        rc.family = next(self._families)
         self.requests[request_id] = rc
         return rc
 
@@ -367,7 +369,7 @@ class PageTables:
 
     def families(self, request_ids: Sequence[Hashable]) -> List[List[int]]:
         """The requests' places in the sequence, family by family (requests that were forked from one another)."""
-        found: Dict[Hashable, List[int]] = {}
+        found: Dict[int, List[int]] = {}
         for i, rid in enumerate(request_ids):
             found.setdefault(self.get(rid).family, []).append(i)
         return list(found.values())
