@@ -235,6 +235,11 @@ def test_entries_refuse_before_anything_runs():
                dict(hd=6, dtype=0), dict(scratch=ctypes.c_void_p(72)), dict(room=1 << 20)]:
         assert attention(**kw) < 0, kw
 
+    # tiles of 16 keys and rows of outputs are counted in 31 bits; attention_shared_takes says so before, and a decode step then goes the other way
+    for n, nh, nkv, hd, reach in [(256, 64, 1, 64, 1 << 21), (256, 64, 64, 64, (1 << 31) - 16), (1, 64, 64, 256, (1 << 31) - 16), (256, 8192, 128, 256, 16)]:
+        assert attention(n=n, nh=nh, nkv=nkv, hd=hd, maxb=reach // 16, room=1 << 20) in (-3, -4)
+        assert (attention(n=n, nh=nh, nkv=nkv, hd=hd, maxb=reach // 16, room=1 << 20) == -3) == (not ops.attention_shared_takes(torch.bfloat16, nh, nkv, hd, n, reach)), (n, nh, reach)
+
     def select(rows=8, beams=4, vocab=100, ld=100, keep=8, scratch=some, room=1 << 40):
         return lib.vk_beam_select(some, some, some, some, some, scratch, SIZE(room), rows, beams, vocab, LL(ld), keep, null)
 

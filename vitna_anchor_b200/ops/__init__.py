@@ -752,7 +752,8 @@ def attention(q: torch.Tensor, pages: torch.Tensor, meta, ctx, out: torch.Tensor
               and not (q.dtype == torch.float32 and _float32_exact))
     pre_ok = (bool(ctx.num_pre) and q.dtype == torch.bfloat16 and hd in PREFILL_HEAD_SIZES and ctx.pre_tiles is not None
               and q.data_ptr() % 16 == 0)
-    if dec_ok and meta.members is not None and window == 0 and attention_shared_takes(q.dtype, nh, nkv, hd, ctx.num_tokens) and q.data_ptr() % 16 == 0:
+    if dec_ok and meta.members is not None and window == 0 and attention_shared_takes(q.dtype, nh, nkv, hd, ctx.num_tokens, meta.block_tables.shape[1] * pages.shape[3]) \
+            and q.data_ptr() % 16 == 0:
         ws = ctx.workspace
         scratch = ws.flat(f"att.shared/{nh}/{hd}", attention_shared_scratch_bytes(min(ws.max_segments, SHARED_MAX_TOKENS), nh, nkv, hd), torch.uint8)
         attention_shared(q, pages, meta.block_tables, ctx.token_seg, ctx.positions, meta.members, meta.starts, meta.shared, out, scratch, nh, nkv, hd, scale)
@@ -2275,10 +2276,11 @@ SHARED_MAX_TOKENS, SHARED_MAX_HEADS, SHARED_MAX_KV_HEADS = 256, 64, 128      # t
 _SHARED_ARGS = struct.Struct("QQQQQQQQQQQiiiiiiiiiifi")
 
 
-def attention_shared_takes(dtype: torch.dtype, nh: int, nkv: int, hd: int, tokens: int = 1) -> bool:
-    """Whether attention_shared takes these sizes (else the members' tables are read one by one, by attention_decode or attention_rows)."""
+def attention_shared_takes(dtype: torch.dtype, nh: int, nkv: int, hd: int, tokens: int = 1, reach: int = 1) -> bool:
+    """Whether attention_shared takes these sizes, `reach` positions a block table (else the members' tables are read one by one, by attention_decode or attention_rows)."""
     return (dtype in (torch.float32, torch.bfloat16) and 0 < hd <= 256 and hd % (4 if dtype == torch.float32 else 8) == 0 and 0 < nkv <= SHARED_MAX_KV_HEADS
-            and nh % nkv == 0 and 0 < nh // nkv <= SHARED_MAX_HEADS and tokens <= SHARED_MAX_TOKENS)
+            and nh % nkv == 0 and 0 < nh // nkv <= SHARED_MAX_HEADS and tokens <= SHARED_MAX_TOKENS
+            and (reach // 16 + 64) * tokens * nh < 1 << 31 and tokens * nh * hd * 4 < 1 << 31)      # the kernels count tiles of 16 keys and rows of outputs in 31 bits
 
 
 _shared_mode = 2
@@ -2318,6 +2320,7 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
     agree on the first shared[f] positions (any number: what lies at or behind the smallest of the members' positions is not counted).  A family
     may have one member or none.  Every token reads the positions 0 .. positions[t] of its own request, as in attention_decode; rows of `out` whose token
     is in no family are left as they were.  Block numbers outside the pool are not followed (their keys and values count as zeros).
+    A value that is infinite or no number where it counts makes its dim of the output no number.
     scratch: a byte buffer of attention_shared_scratch_bytes(members, ...) or more, whatever it holds, for launches of one stream at a time.  The lists and
     lengths are read while the kernel before this one in the stream may still run: that must not be a kernel of this library which writes them."""
     here, dtype, i32 = torch._C._cuda_getDevice(), q.dtype, torch.int32
@@ -2328,8 +2331,8 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
     n, families = members.shape[0], shared.shape[0]
     pages, two, kv_heads, page_size, dim = cache_layer.shape
     segments, max_blocks = block_tables.shape
-    if width != nh * hd or out.shape != q.shape or two != 2 or kv_heads != nkv or dim != hd or not attention_shared_takes(dtype, nh, nkv, hd, n):
-        raise KernelError(f"attention_shared: shapes do not fit the head counts, or {n} tokens of {nh} heads over {nkv} of {hd} in {dtype} are not taken")
+    if width != nh * hd or out.shape != q.shape or two != 2 or kv_heads != nkv or dim != hd or not attention_shared_takes(dtype, nh, nkv, hd, n, max_blocks * page_size):
+        raise KernelError(f"attention_shared: shapes do not fit the head counts, or {n} tokens of {nh} heads over {nkv} of {hd} in {dtype}, {max_blocks * page_size} positions each, are not taken")
     if token_seg.shape[0] != T or positions.shape[0] != T:
         raise KernelError("attention_shared: per-token arrays differ in length")
     if starts.shape[0] != families + 1 or families > SHARED_MAX_TOKENS:
