@@ -11,7 +11,7 @@
 //
 // The float32 kernel: a warp holds up to eight rows against 32 keys.  Lane j has key j's scores of all the rows (a piece of its key is read once for the eight, the queries come as
 // broadcasts), the weights go through shared memory, and then the lane has dims j, j + 32, ... of the rows' outputs (a value once for the eight, the weights as broadcasts of four keys).
-// Shared memory then serves 32 products with 12 reads of 16 bytes and its bandwidth and the float32 units' are about even; with a row at a time it was one for one, and 7.5 times slower.
+// Of the scores 9 reads of 16 bytes from shared memory then serve 32 multiply-adds a lane; a row at a time takes 2 for 4.
 // R = 1, 2, 4 or 8 warps that cover a prefix's rows share the tiles of their keys; own keys are walked by single warps.
 #include "attention_shared_plan.cuh"
 
