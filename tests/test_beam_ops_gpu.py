@@ -209,6 +209,36 @@ def test_attention_shared_of_scores_without_a_number(ops, wide):
         assert float(((got[t, heads] - want[t, heads]).abs() - tol[t, heads]).max()) <= 0
 
 
+@pytest.mark.parametrize("dtype,wide", [(BF16, True), (BF16, False), (F32, True), (F32, False)])
+def test_attention_shared_of_a_token_named_twice(ops, dtype, wide):
+    """In one family and in two: the token has its one result."""
+    for members, starts, shared in [([0, 1, 0], [0, 3], [96]), ([0, 1, 1, 0], [0, 2, 4], [96, 48])]:
+        b = Batch([(96, [20, 9])], 6, 2, 64, 16, dtype, seed=4)
+        place = b.members
+        b.members = [place[m] for m in members]
+        b.device(wide)
+        b.d["starts"], b.d["shared"] = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in (starts, shared))
+        b.check(ops)
+
+
+def test_attention_shared_two_graphs_through_one_scratch(ops):
+    """Captured apart, replayed in turns on one stream."""
+    a, b = Batch([(400, [5, 60, 17])], 6, 2, 64, 16, BF16, seed=1).device(), Batch([(64, [9, 30]), (128, [70, 3])], 6, 2, 64, 16, BF16, seed=2).device()
+    scratch = torch.full((ops.attention_shared_scratch_bytes(4, 6, 2, 64),), 0x7F, dtype=torch.uint8, device="cuda")
+    graphs = []
+    for x in (a, b):
+        x.run(ops, scratch)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            x.run(ops, scratch)
+        x.d["out"].fill_(7.0)
+    for n in (0, 1, 0, 1, 1, 0):
+        graphs[n].replay()
+    for x in (a, b):
+        want, tol = x.want()
+        assert float(((x.d["out"].double().cpu() - want).abs() - tol).max()) <= 0
+
+
 def test_attention_shared_far_in_a_large_pool(ops):
     """Element offsets beyond 2^31."""
     b = Batch([(96, [5, 40])], 32, 32, 64, 16, BF16)
@@ -355,6 +385,31 @@ def test_beam_select_values_laid_out_against_the_groups(ops, keep):
     up = torch.linspace(-5, 5, V, device="cuda").repeat(2, 1)
     check_choice(ops, up, torch.tensor([0.0, -1e-3], device="cuda"), 2, keep)
     check_choice(ops, up.flip(1).contiguous(), torch.tensor([0.0, -1e-3], device="cuda"), 2, keep)
+
+
+@pytest.mark.parametrize("size", [1e-6, 1e3, 3e4, 1e30])
+def test_beam_select_of_small_and_large_logits(ops, size):
+    """Beyond what the bounds' 16 bits tell apart.  The scores' gap of 1.5 is far beyond the error of a row's sum, or far below a step of its logits."""
+    x = torch.randn((4, 30000), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda") * size
+    for beams, keep in [(1, 3), (1, 128), (2, 9)]:
+        got = select(ops, x, torch.tensor([0.0, -1.5] * 2, device="cuda"), beams, keep)
+        best, parent, token = choose(x, torch.tensor([0.0, -1.5] * 2), beams, keep)
+        if beams == 1 or size > 1:
+            assert np.array_equal(got[1].cpu().numpy(), parent) and np.array_equal(got[2].cpu().numpy(), token)
+        b = got[0].cpu().numpy().astype(np.float64)
+        assert np.all(np.abs(b - best) <= 2.0 ** -24 * np.abs(best) + 40 * 2.0 ** -23)
+
+
+def test_beam_select_scores_in_place(ops):
+    """A step's sums over the last step's: the scores are read before any of them is written."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    logits = torch.randn((24, 9000), generator=g, device="cuda") * 3
+    scores = -torch.rand(24, generator=g, device="cuda")
+    best, parent, token = choose(logits, scores, 8, 8)
+    out = (scores.view(3, 8), torch.empty((3, 8), dtype=torch.int32, device="cuda"), torch.empty((3, 8), dtype=torch.int32, device="cuda"))
+    ops.beam_select(logits, scores, 8, 8, out, torch.zeros(ops.beam_select_scratch_bytes(24, 9000, 8), dtype=torch.uint8, device="cuda"))
+    assert np.array_equal(out[1].cpu().numpy(), parent) and np.array_equal(out[2].cpu().numpy(), token)
+    assert np.all(np.abs(scores.view(3, 8).cpu().numpy() - best) <= 2.0 ** -24 * np.abs(best) + 40 * 2.0 ** -23)
 
 
 def test_beam_select_one_strong_row(ops):
