@@ -225,14 +225,14 @@ def test_entries_refuse_before_anything_runs():
     some = ctypes.c_void_p(64)
     LL, SIZE = ctypes.c_longlong, ctypes.c_size_t
 
-    def attention(n=4, families=1, nh=4, nkv=2, hd=64, ps=16, maxb=8, dtype=1, scratch=some, room=1 << 40):
+    def attention(n=4, families=1, nh=4, nkv=2, hd=64, ps=16, maxb=8, dtype=1, scratch=some, room=1 << 40, error=64):
         at = lambda p: p.value or 0      # noqa: E731
-        args = ctypes.create_string_buffer(ops._SHARED_ARGS.pack(*[at(some)] * 9, at(scratch), room, 4, 4, n, families, 10, nh, nkv, hd, ps, maxb, 0.1, dtype))
+        args = ctypes.create_string_buffer(ops._SHARED_ARGS.pack(*[at(some)] * 9, at(scratch), room, 4, 4, n, families, 10, nh, nkv, hd, ps, maxb, 0.1, dtype, error))
         return lib.vk_attention_shared(args, null)
 
     assert attention(n=0) == 0 and attention(families=0) == 0
     for kw in [dict(n=257), dict(families=257), dict(hd=264), dict(nkv=129, nh=129), dict(hd=12), dict(nh=5), dict(nh=130), dict(ps=0), dict(maxb=0), dict(maxb=1 << 28),
-               dict(hd=6, dtype=0), dict(scratch=ctypes.c_void_p(72)), dict(room=1 << 20)]:
+               dict(hd=6, dtype=0), dict(error=0), dict(scratch=ctypes.c_void_p(72)), dict(room=1 << 20)]:
         assert attention(**kw) < 0, kw
 
     # tiles of 16 keys and rows of outputs are counted in 31 bits; attention_shared_takes says so before, and a decode step then goes the other way

@@ -209,6 +209,83 @@ def test_attention_shared_of_scores_without_a_number(ops, wide):
         assert float(((got[t, heads] - want[t, heads]).abs() - tol[t, heads]).max()) <= 0
 
 
+MANY = [  # families whose rows fill a tile of 128 or most of it, heads of 128: families, heads, kv heads, page
+    ([(64, [3] * 5)], 16, 1, 16),                                          # one tile of keys
+    ([(65, [3] * 5)], 16, 1, 16), ([(128, [1] * 8)], 16, 1, 64),
+    ([(1000, [2, 70, 9, 1, 33])], 14, 1, 16),                              # 70 rows
+    ([(4097, [5] * 16)], 16, 2, 16),                                       # 128 rows
+    ([(777, list(range(1, 30)))], 8, 1, 13),                               # 232 rows, a last tile of few, pages of an odd size
+    ([(300, [4] * 9), (1200, [8] * 12), (17, [40] * 3), (0, [9])], 16, 2, 8),
+    ([(2000, [3] * 80), (500, [7] * 100)], 2, 2, 16),                      # 80 and 100 members of one head
+]
+
+
+@pytest.mark.parametrize("n", range(len(MANY)))
+def test_attention_shared_of_many_rows(ops, n):
+    families, nh, nkv, ps = MANY[n]
+    Batch(families, nh, nkv, 128, ps, BF16, seed=40 + n).device().check(ops)
+
+
+def test_attention_shared_of_many_rows_far_in_a_large_pool(ops):
+    """Element offsets beyond 2^31."""
+    b = Batch([(200, [5] * 9)], 32, 4, 128, 16, BF16)
+    b.device()
+    pages = 140000
+    big = torch.empty((pages, 2, 4, 16, 128), dtype=BF16, device="cuda")
+    big[pages - b.pages:] = b.d["cache"]
+    b.d["cache"] = big
+    b.d["tables"] = torch.where(b.d["tables"] < b.pages, b.d["tables"] + (pages - b.pages), b.d["tables"])
+    b.check(ops)
+
+
+def test_attention_shared_of_many_rows_whose_maxima_rise(ops):
+    """Every tile's scores are far above the ones before, for some rows, and below for others; one tile weighs nothing at all."""
+    b = Batch([(1024, [20] * 8)], 16, 1, 128, 16, BF16, seed=7)
+    first = b.tables[b.members[0]][:64]
+    along = b.q[b.members[0], :128].float()
+    along /= along.norm()
+    for i, page in enumerate(first):
+        b.cache[page, 0] = (b.cache[page, 0].float() + along * (i - 20)).to(BF16)
+    b.cache[first[8:12], 0] = -math.inf
+    b.q.abs_()
+    got = b.device().run(ops).double().cpu()
+    want, tol = b.want()
+    tol = torch.where(torch.isfinite(tol), tol, torch.tensor(2.0 ** -6).double())      # the bound's sums are over infinite keys
+    assert float(((got - want).abs() - tol).max()) <= 0
+
+
+def test_attention_shared_of_many_rows_bad_blocks_and_no_number(ops):
+    b = Batch([(640, [20, 9, 3, 3, 3, 3])], 16, 1, 128, 16, BF16)
+    b.cache[b.tables[b.members[0]][3]] = 0
+    b.device()
+    for t, bad in zip(b.members, (-1, b.pages, 1 << 30, -(1 << 31), b.pages, -7)):
+        b.d["tables"][t, 3] = bad
+    b.check(ops)
+    b = Batch([(640, [20, 9, 3, 3, 3, 3])], 16, 1, 128, 16, BF16)
+    b.cache[b.tables[b.members[0]][3], 0, 0, 2] = float("nan")             # a common key: nobody has a number
+    got = b.device().run(ops)
+    assert bool(torch.isnan(got[b.members]).all())
+
+
+@pytest.mark.parametrize("tile,shared", [(0, 4000), (1, 30000)])      # of 4,000 keys a group of warps has one tile at most, of 30,000 (over at most 148 blocks) three or more
+def test_attention_shared_gives_up_a_wait_and_says_so(ops, tile, shared):
+    """A tile of keys whose scores are never told of (a hook for this test; nothing faults): the waits run out after the 5 ms set here, the kernel returns by itself with its
+    tensor memory freed, the error word is set, and the next launch is right."""
+    b = Batch([(shared, [5] * 16)], 16, 2, 128, 16, BF16, seed=2).device()
+    ops.set_wait_limit_ms(5.0)
+    try:
+        ops.skip_stage_once("attention_shared", tile)
+        b.run(ops)
+        torch.cuda.synchronize()
+        assert ops.device_error_code() == 81
+        with pytest.raises(ops.KernelGaveUp):
+            ops.check_device_errors()
+    finally:
+        ops.set_wait_limit_ms(0)
+    b.check(ops)
+    ops.check_device_errors()
+
+
 @pytest.mark.parametrize("dtype,wide", [(BF16, True), (BF16, False), (F32, True), (F32, False)])
 def test_attention_shared_of_a_token_named_twice(ops, dtype, wide):
     """In one family and in two: the token has its one result."""

@@ -529,15 +529,16 @@ struct VkAttentionShared {
     int32_t tokens, segments, n, families, pages, nh, nkv, hd, page_size, max_blocks;
     float scale;
     int32_t dtype;
+    int* error;                    // set where a wait inside the kernel runs out
 };
 
 VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t stream) {
     const auto [q, cache, block_tables, token_seg, positions, members, starts, shared, out, scratch, scratch_bytes, tokens, segments, n, families, pages, nh, nkv, hd, page_size,
-                max_blocks, scale, dtype] = *args;
+                max_blocks, scale, dtype, error] = *args;
     if (n <= 0 || families <= 0) return VK_OK;
     if (n > SA_MAX_TOKENS || families > SA_MAX_TOKENS || nkv > SA_MAX_KV_HEADS || hd > 256) return VK_TOO_LARGE;
     const int vec = dtype == 0 ? 4 : 8;
-    if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > SA_MAX_HEADS || hd <= 0 || hd % vec || page_size <= 0 || max_blocks <= 0 || pages <= 0) return VK_BAD_SHAPE;
+    if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > SA_MAX_HEADS || hd <= 0 || hd % vec || page_size <= 0 || max_blocks <= 0 || pages <= 0 || !error) return VK_BAD_SHAPE;
     if ((long long)max_blocks * page_size > 0x7fffffffLL) return VK_TOO_LARGE;
     // the lines' tiles and the parts' rows are counted in 31 bits
     const long long tiles = (long long)max_blocks * page_size / SA_TILE + 64, units = (long long)n * nh;
@@ -560,13 +561,15 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
     a.scale_log2 = scale * 1.4426950408889634f;
     if (attention_shared_mma_takes(a, dtype)) {
         if (attention_each_mma_takes(a)) return launch_attention_each_mma(a, sms, stream);
-        const int status = launch_attention_shared_mma(a, sms, stream);
+        const int status = launch_attention_shared_mma(a, sms, error, stream);
         return status != VK_OK ? status : launch_join(a, dtype, stream);
     }
     if (each_takes(a, dtype)) return launch_each(a, dtype, sms, stream);
     a.prefix_rows = SG_PREFIX_ROWS;
     a.own_rows = SG_ROWS;
     a.row_unit = 16.0f;
+    a.tensor_rows = 0x7fffffff;
+    a.tensor_unit = 1.0f;
     a.blocks = sms * sg_blocks(hd);
     a.own_per_block = sg_slots(hd);
     a.min_prefix = a.min_own = 4;

@@ -2,7 +2,7 @@
 //
 // The mathematics and the cut into parts are attention_shared.cu's and attention_shared_plan.cuh's.  A part's rows (a family's members times the heads
 // that read one key-value head) are the 16-row operands of m16n8k16 products, 16 rows a warp; R = 1, 2, 4 or 8 warps that cover a part's rows
-// make a group that works through the same keys, and the block's 8 / R groups take turns at the tiles of 16 R keys.  So a block holds up to 128 rows
+// make a group that works through the same keys, and the block's 8 / R groups take turns at the tiles of 16 R keys (heads of 128: R up to 4, more rows go to tcgen05, see below).  So a block holds up to 128 rows
 // against keys that are read once, and with few rows all eight warps still read keys of their own.  Up to eight rows turn the products over: the keys are the 16 rows and
 // the rows the eight columns, half the products and half the exponentials.
 //
@@ -17,10 +17,10 @@
 //
 // What bounds it.  64 requests behind 6,000 positions with up to 700 of their own, 32 heads of 64 (214 MB): 49 us, 4.4 TB/s; the common keys' blocks do 64 rows a key, 16,000 cycles of the tensor
 // cores' legacy path, and take 37,000 (a group's warps do scores, softmax and p v in step, 4 warps a scheduler), while the own keys' blocks beside them wait for memory.  One kind after the
-// other in every block: 57 us.  16 requests behind 32,000 positions, 16 heads of 128 over 2 (36 MB): 36 us; 128 rows a key are 21,000 cycles of products at best and take 39,000 with two warps a
-// scheduler (that many outputs fill the registers).  Eight beams of 2,048 positions, 32 heads of 64 (20 MB): 11.6 us, of which finding the parts is 2 (it runs before the wait for the kernel
+// other in every block: 57 us.  Eight beams of 2,048 positions, 32 heads of 64 (20 MB): 11.6 us, of which finding the parts is 2 (it runs before the wait for the kernel
 // before) and joining them 3.
 #include "attention_shared_plan.cuh"
+#include "tcgen05_common.cuh"
 
 namespace vk {
 
@@ -451,6 +451,234 @@ __device__ __forceinline__ void sm_prefix_few(const SaArgs& a, const SaPlan& p, 
     sm_meet<HD, 1>(a, part, stages);
 }
 
+// ---- prefixes of many rows, on the fifth-generation tensor cores ---------------------------------------------------------------------------------
+//
+// The part's rows (up to 128) are the lanes of tensor memory.  Two groups of four warps walk tiles of 64 keys in turn, each by itself: scores S[128 x 64] = Q K^T out of shared memory, a
+// thread a row takes them out, and puts the weights back in their place as high and low parts (32 keys in 16 + 16 columns); O[128 x HD] += P V has them from there and stays in
+// tensor memory.  Keys and values come by cp.async into rows of 128 bytes, 16-byte pieces at piece ^ (key & 7) (the 128-byte swizzle): keys two tiles ahead, values one, each into the
+// stage that the product before is known to have read.  While one group's weights are worked out the other's products run.
+//
+// Where: heads of 128 and 65 rows or more.  16 members of 16 heads over 2 of 128 (128 rows) behind 32,000 positions 28.0 us against 36.1 with mma.sync, behind 8,000 19.3 / 20.0; 32 members behind
+// 4,000 18.2 / 18.4.  With fewer rows the lanes that stand for none cost as much as the others (40 rows behind 16,000: 19.9 / 19.4; 64 behind 8,000, 8 key-value heads: 24.3 / 22.7), and heads of
+// 64 have half the products for the same exponentials: 64 rows behind 2,000, 32 heads, 27.7 / 24.3; 96 rows behind 4,000, 5 heads, 17.0 / 15.6.
+//
+// What bounds it.  A tile takes its group 2,800 cycles (S 220 from its issue, a thread's 64 weights 1,500, P V 700 until the next S may begin), two groups beside one another; four tiles a
+// group in the first of these cases.  Before them are the plan, 5,000, the queries, pages and first keys, behind them the groups' meeting, 4,000, and the launch that joins the parts.
+constexpr int SM_TENSOR_ROWS = 65;
+
+template <int HD> struct SmTc {
+    static constexpr int KEYS = 64, ROWS = 128, PANELS = HD / 64, PANEL = KEYS * 128, TILE = PANELS * PANEL, Q_PANEL = ROWS * 128, Q = PANELS * Q_PANEL;      // panels of 64 dims
+    static constexpr int GROUP = 4 * TILE;                                            // a group's keys, two stages, and values, two
+    static constexpr int OUT = 2 * ROWS * (HD + 4) * 4, ML = 2 * ROWS * 8;            // where the groups' outputs meet
+    static constexpr uint32_t O_COL = 2 * KEYS, TMEM = 512;                           // columns: the groups' scores, their outputs
+    static_assert(1024 + Q + 2 * GROUP <= SM_STAGES * SmSmem<HD>::STAGE && OUT + ML <= SM_STAGES * SmSmem<HD>::STAGE && O_COL + 2 * HD <= TMEM, "it lies over the stages");
+};
+
+// Of a block: the tensor memory, the groups' barriers (scores done, output done) and their phases, and whether a wait has run out.
+struct SmTcBlock {
+    uint32_t tmem;
+    uint64_t* bars;
+    int phase;
+    bool lost;
+};
+
+// The product with the first operand in tensor memory (128 lanes, two bfloat16 values a column).
+__device__ __forceinline__ void sm_umma_ts(uint32_t d, uint32_t at, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+        ::"r"(d), "r"(at), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(UMMA_DESC_HI_SW128));
+}
+__device__ __forceinline__ void sm_tmem_st16(uint32_t at, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+
+template <int HD>
+__device__ __forceinline__ void sm_prefix_tc(const SaArgs& a, const SaPlan& p, const SaPart& part, unsigned char* stages, SmTcBlock& block, const WaitCtl& wc, int* failed) {
+    typedef SmTc<HD> S;
+    constexpr int CH = HD / 8, AT_ONCE = 128 / CH, PIECES = S::KEYS / AT_ONCE, RW = 32 / CH, LD = HD + 4;      // 16-byte pieces a row; rows a group, a warp copies at once
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = warp >> 2, w = warp & 3, r = tid & 127, rows = (part.i1 - part.i0) * part.heads;
+    unsigned char* base = stages + ((1024 - (sm_addr(stages) & 1023)) & 1023);
+    const int tiles = (part.k1 - part.k0 + S::KEYS - 1) / S::KEYS, mine = (tiles - group + 1) / 2;      // this group's: group, group + 2, ...
+    const uint32_t ring = sm_addr(base) + S::Q + group * S::GROUP;
+    const int crow = r / CH, piece = r % CH, my_key = w * RW + lane % RW + (lane & 15) / RW * AT_ONCE;      // the key of a tile whose page this lane asks for
+    const uint32_t lane_dst = (piece >> 3) * S::PANEL + crow * 128 + (((piece & 7) ^ (crow & 7)) << 4);
+    const size_t to_values = (size_t)a.nkv * a.page_size * HD;
+    const __nv_bfloat16* cache = static_cast<const __nv_bfloat16*>(a.cache);
+    auto page_of = [&](int n) -> int {
+        const int k = part.k0 + (group + 2 * n) * S::KEYS + my_key;
+        return n < mine && k < part.k1 ? part.table[a.page_shift >= 0 ? k >> a.page_shift : k / a.page_size] : -1;
+    };
+    auto row_of = [&](int n, int page) -> uint32_t {           // the row of the pool that holds the key; none: ~0
+        const int k = part.k0 + (group + 2 * n) * S::KEYS + my_key, in_page = a.page_shift >= 0 ? k & (a.page_size - 1) : k % a.page_size;
+        return (uint32_t)page < (uint32_t)a.pages ? ((uint32_t)page * 2u * a.nkv + part.kvh) * a.page_size + in_page : 0xffffffffu;
+    };
+    auto copy = [&](int n, uint32_t from, uint32_t stage, size_t more) {      // a tile's keys, or values
+        if (n >= mine) return;
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const uint32_t row = __shfl_sync(0xffffffffu, from, i * RW + lane / CH);
+            const bool there = row != 0xffffffffu;
+            sm_copy16_or_zero(stage + lane_dst + i * AT_ONCE * 128, there ? cache + (size_t)row * HD + piece * 8 + more : cache, there);
+        }
+    };
+    auto landed = [&]() {                                      // all but the newest of this thread's copies have, and the tensor core may read them behind the group's meeting
+        asm volatile("cp.async.wait_group 1;\nfence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory");
+    };
+    auto wait = [&](uint64_t* bar, int phase) {                // once a wait has run out there are no more
+        if (!block.lost && !__all_sync(0xffffffffu, mbar_wait(bar, (uint32_t)phase & 1, wc.cycles))) {
+            block.lost = true;
+            if (lane == 0) give_up(wc.error, failed, 81);
+        }
+        tc_fence_after();
+    };
+    uint64_t *s_done = block.bars + group, *o_done = block.bars + 2 + group;
+    const uint32_t lanes = (uint32_t)(w * 32) << 16, s_at = block.tmem + group * S::KEYS, o_at = block.tmem + S::O_COL + group * HD;
+    const uint32_t s_desc = umma_idesc_bf16(S::ROWS, S::KEYS), o_desc = umma_idesc_bf16(S::ROWS, HD) | (1u << 16);      // (the values are N-major)
+    const float scale = a.scale_log2;
+    float m = -INFINITY, l = 0.0f;
+
+    // what the first tiles and the queries hang on is asked for before any of it is used
+    const int page0 = page_of(0), page1 = page_of(1);
+    int page = page_of(2);
+    const SmQueryOf query_of{a, p, part, HD};
+    uint4 queries[S::ROWS * CH / SA_THREADS];
+#pragma unroll
+    for (int i = 0; i < S::ROWS * CH / SA_THREADS; i++) {
+        const __nv_bfloat16* q = query_of(tid / CH + i * (SA_THREADS / CH));
+        queries[i] = q ? *reinterpret_cast<const uint4*>(q + tid % CH * 8) : make_uint4(0, 0, 0, 0);
+    }
+    uint32_t now = row_of(0, page0), next = row_of(1, page1);
+    copy(0, now, ring, 0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    copy(1, next, ring + S::TILE, 0);
+    copy(0, now, ring + 2 * S::TILE, to_values);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < S::ROWS * CH / SA_THREADS; i++) {
+        const int row = tid / CH + i * (SA_THREADS / CH), piece = tid % CH;
+        *reinterpret_cast<uint4*>(base + (piece >> 3) * S::Q_PANEL + row * 128 + (((piece & 7) ^ (row & 7)) << 4)) = queries[i];
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+#pragma unroll 1
+    for (int n = 0; n < mine; n++) {
+        landed();
+        if (w == 0) {
+            if (n > 0) wait(o_done, block.phase + n - 1);      // the scores take the place of weights that the tensor core has read
+            if (elect_one()) {
+                const uint32_t q_lo = umma_desc_lo(sm_addr(base)), k_lo = umma_desc_lo(ring + (n & 1) * S::TILE);
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < HD / 16; k++) umma_bf16_lo(s_at, q_lo + (k / 4) * (S::Q_PANEL >> 4) + 2 * (k % 4), k_lo + (k / 4) * (S::PANEL >> 4) + 2 * (k % 4), s_desc, k != 0);
+                if (n != wc.skip_stage) umma_commit(s_done);   // (a tile named by wc.skip_stage is never told of: a test of the give-up path)
+            }
+            __syncwarp();
+        }
+        const uint32_t after = row_of(n + 2, page);
+        page = page_of(n + 3);
+        wait(s_done, block.phase + n);                         // and so the keys' stage and the values' other one have been read
+        copy(n + 2, after, ring + (n & 1) * S::TILE, 0);
+        copy(n + 1, next, ring + (2 + ((n + 1) & 1)) * S::TILE, to_values);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next = after;
+        uint32_t s[S::KEYS];
+        tmem_ld32_nowait(s_at + lanes, s);
+        tmem_ld32_nowait(s_at + lanes + 32, s + 32);
+        tmem_wait_ld();
+        tmem_loaded(s);
+        tmem_loaded(s + 32);
+        const int left = part.k1 - (part.k0 + (group + 2 * n) * S::KEYS);
+        if (left < S::KEYS) {
+#pragma unroll
+            for (int j = 0; j < S::KEYS; j++)
+                if (j >= left) s[j] = 0xff800000u;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < S::KEYS; j++) top = fmaxf(top, __uint_as_float(s[j]));
+        top *= scale;
+        const bool ahead = top > m + SM_AHEAD;
+        if (__any_sync(0xffffffffu, ahead)) {
+            const float keep = ahead ? sa_ex2(m - top) : 1.0f;
+            l *= keep;
+            if (ahead) m = top;
+            if (n > 0) {
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(o_at + lanes + c, o);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                    sm_tmem_st16(o_at + lanes + c, o);
+                }
+            }
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;           // no score above -inf so far: p = 0
+        float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < S::KEYS; c += 32) {
+            uint32_t hi[16], lo[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const float p0 = sa_ex2(fmaf(__uint_as_float(s[c + 2 * j]), scale, -ref)), p1 = sa_ex2(fmaf(__uint_as_float(s[c + 2 * j + 1]), scale, -ref));
+                sum0 += p0;
+                sum1 += p1;
+                sm_split(p0, p1, hi[j], lo[j]);
+            }
+            sm_tmem_st16(s_at + lanes + c, hi);
+            sm_tmem_st16(s_at + lanes + c + 16, lo);
+        }
+        l += sum0 + sum1;
+        tmem_wait_st();
+        tc_fence_before();
+        landed();
+        if (w == 0) {
+            if (elect_one()) {
+                const uint32_t v_lo = ((ring + (2 + (n & 1)) * S::TILE) >> 4) | ((uint32_t)(S::PANEL >> 4) << 16);      // the panels' distance is the leading byte offset
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < S::KEYS / 16; k++) sm_umma_ts(o_at, s_at + 32 * (k / 2) + 8 * (k % 2), v_lo + k * (2048 >> 4), o_desc, n > 0 || k != 0);
+#pragma unroll
+                for (int k = 0; k < S::KEYS / 16; k++) sm_umma_ts(o_at, s_at + 32 * (k / 2) + 16 + 8 * (k % 2), v_lo + k * (2048 >> 4), o_desc, 1);
+                umma_commit(o_done);
+            }
+            __syncwarp();
+        }
+    }
+    if (mine > 0) wait(o_done, block.phase + mine - 1);
+    block.phase += mine;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                                           // both groups are past their tiles
+    float* out = reinterpret_cast<float*>(stages);
+    float2* ml = reinterpret_cast<float2*>(stages + S::OUT);
+#pragma unroll 1
+    for (int c = 0; c < HD; c += 16) {
+        uint32_t o[16];
+        tmem_ld16(o_at + lanes + c, o);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)                        // a group without a tile has nothing
+            *reinterpret_cast<uint4*>(out + tid * LD + c + j) = mine > 0 ? make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]) : make_uint4(0, 0, 0, 0);
+    }
+    ml[tid] = make_float2(m, l);
+    tc_fence_before();
+    __syncthreads();
+#pragma unroll 1
+    for (int c = tid; c < rows * (HD / 4); c += SA_THREADS) {
+        const int row = c / (HD / 4), d = c % (HD / 4) * 4;
+        const float2 x = ml[row], y = ml[S::ROWS + row];
+        const float most = fmaxf(x.x, y.x), ref = most == -INFINITY ? 0.0f : most, wx = sa_ex2(x.x - ref), wy = sa_ex2(y.x - ref);
+        const float4 u = *reinterpret_cast<const float4*>(out + row * LD + d), v = *reinterpret_cast<const float4*>(out + (S::ROWS + row) * LD + d);
+        const int at = part.row0 + row * part.stride;
+        *reinterpret_cast<float4*>(a.part_o + (size_t)at * HD + d) = make_float4(u.x * wx + v.x * wy, u.y * wx + v.y * wy, u.z * wx + v.z * wy, u.w * wx + v.w * wy);
+        if (d == 0) a.part_ml[at] = make_float2(most, x.y * wx + y.y * wy);
+    }
+}
+
 // What a warp's walk of an own part leaves: the result where the unit needs nobody else, else the part's row.
 template <int HD>
 __device__ __forceinline__ void sm_leave(const SaArgs& a, const SaPlan& p, const SaPart& part, bool alone, int row, int d, float x, float y) {
@@ -459,16 +687,38 @@ __device__ __forceinline__ void sm_leave(const SaArgs& a, const SaPlan& p, const
 }
 
 template <int HD>
-__global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared_mma_kernel(const SaArgs a) {
+__global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared_mma_kernel(const SaArgs a, const WaitCtl wc) {
     extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint64_t bars[4];
+    __shared__ uint32_t tmem_at;
+    __shared__ int failed;
+    constexpr bool TENSOR = HD == 128;
     SaPlan& p = *reinterpret_cast<SaPlan*>(smem);
     unsigned char* stages = smem + SmSmem<HD>::PLAN;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     sa_make_plan(a, p);                       // from the step's metadata, which no kernel writes
     dependency_wait();
+    const bool prefix = (int)blockIdx.x < p.prefix_blocks;
+    // tensor memory where some prefix has many rows, before the kernel after this one may come and want some
+    const bool tensor = TENSOR && prefix && __syncthreads_or(p.shared[threadIdx.x] > 0 && min(p.width[threadIdx.x], p.tile_members) * a.gq >= SM_TENSOR_ROWS);
+    SmTcBlock block = {0, bars, 0, false};
+    if (tensor) {
+        if (threadIdx.x == 0) {
+            failed = 0;
+            for (int b = 0; b < 4; b++) mbar_init(&bars[b], 1);
+            asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
+        }
+        if (warp == 0) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_addr(&tmem_at)), "r"(SmTc<HD>::TMEM) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        block.tmem = tmem_at;
+    }
     let_dependents_start();
     SaPart part;
-    const bool prefix = (int)blockIdx.x < p.prefix_blocks;
     int at = blockIdx.x * p.lp, end = prefix ? min(at + p.lp, p.pbase[SA_MAX_TOKENS]) : 0;
     while (at < end) {
         if (!sa_prefix_part(a, p, at, end, blockIdx.x, part)) continue;
@@ -477,8 +727,14 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
         else if (rows <= 16) sm_prefix<HD, 1>(a, p, part, stages);
         else if (rows <= 32) sm_prefix<HD, 2>(a, p, part, stages);
         else if (rows <= 64) sm_prefix<HD, 4>(a, p, part, stages);
+        else if constexpr (TENSOR) sm_prefix_tc<HD>(a, p, part, stages, block, wc, &failed);
         else sm_prefix<HD, 8>(a, p, part, stages);
         __syncthreads();
+    }
+    if (TENSOR && tensor && warp == 0) {
+        if (failed) __nanosleep(200000);      // after a failed wait: let products in flight end
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(block.tmem), "r"(SmTc<HD>::TMEM) : "memory");
     }
     // every warp by itself; neighbouring parts of the own keys go to different multiprocessors
     const int worker = prefix ? 0 : warp * ((int)gridDim.x - p.prefix_blocks) + (int)blockIdx.x - p.prefix_blocks;
@@ -618,7 +874,7 @@ int launch_attention_each_mma(const SaArgs& a, int multiprocessors, cudaStream_t
 #undef GO
 }
 
-int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream) {
+int launch_attention_shared_mma(SaArgs a, int multiprocessors, int* error, cudaStream_t stream) {
     a.prefix_rows = SM_PREFIX_ROWS;
     a.own_rows = 16;
     a.row_unit = 16.0f;
@@ -629,12 +885,14 @@ int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stre
     a.min_own = 4;
     a.prefix_cost = 16;
     a.own_cost = 8;
-#define GO(HD)                                                                                                                                  \
+    a.tensor_rows = a.hd == 128 ? SM_TENSOR_ROWS : 0x7fffffff;
+    a.tensor_unit = 1.0f;
+#define GO(HD)                                                                                                                                          \
     do {                                                                                                                                        \
-        auto kern = attention_shared_mma_kernel<HD>;                                                                                            \
+        auto kern = attention_shared_mma_kernel<HD>;                                                                                    \
         const int e = sa_allow_smem(kern, SmSmem<HD>::BYTES);                                                                                   \
         if (e != VK_OK) return e;                                                                                                               \
-        return launch_dependent(kern, dim3(blocks), dim3(SA_THREADS), SmSmem<HD>::BYTES, stream, a);                                            \
+        return launch_dependent(kern, dim3(blocks), dim3(SA_THREADS), SmSmem<HD>::BYTES, stream, a, wait_ctl(error, WAIT_FAMILY_ATTENTION_SHARED)); \
     } while (0)
     if (a.hd == 64) GO(64);
     GO(128);

@@ -38,7 +38,8 @@ struct SaArgs {
     float* part_o;                 // [rows][hd]
     int n, families, tokens, segments, pages, nh, nkv, gq, hd, page_size, page_shift, max_blocks;
     int prefix_rows, own_rows, blocks, own_per_block, min_prefix, min_own, prefix_cost, own_cost;      // own workers a block; the last four in tiles of keys
-    float scale_log2, row_unit;    // row_unit: the rows of a prefix's tile that cost as much as an own tile
+    float scale_log2, row_unit, tensor_unit;      // row_unit: the rows of a prefix's tile that cost as much as an own tile; tensor_unit: what a tile of tensor_rows or more rows costs, in own tiles
+    int tensor_rows;
 };
 
 // A row's parts: prefix_parts from prefix_row on and own_parts from own_row on; none: the row was written when it was walked, or its member is not there.
@@ -151,7 +152,8 @@ __device__ __forceinline__ void sa_make_plan(const SaArgs& a, SaPlan& p) {
     const int P = i < a.families ? common(i) : 0, width = p.width[i], tiles = (width + p.tile_members - 1) / p.tile_members;
     const int own = valid ? pos + 1 - common(g) : 0;
     int wp = P > 0 ? (sa_tiles(P) + a.prefix_cost) * tiles * a.nkv : 0, wo = own > 0 ? (sa_tiles(own) + a.own_cost) * p.own_tiles * a.nkv : 0, tp, to;
-    const float weight = warp_sum((float)wp * fmaxf(1.0f, (float)(min(width, p.tile_members) * a.gq) / a.row_unit));
+    const int rows = min(width, p.tile_members) * a.gq;
+    const float weight = warp_sum((float)wp * (rows >= a.tensor_rows ? a.tensor_unit : fmaxf(1.0f, (float)rows / a.row_unit)));
     if (lane == 0) p.weight[i >> 5] = weight;
     sa_scan2(p.scan[0], wp, wo, tp, to);
     p.shared[i] = P;                        // behind the barrier: until then it is what was claimed
@@ -376,7 +378,7 @@ template <typename... Args> inline int sa_allow_smem(void (*kernel)(Args...), si
 
 // attention_shared_mma.cu
 bool attention_shared_mma_takes(const SaArgs& a, int dtype);
-int launch_attention_shared_mma(SaArgs a, int multiprocessors, cudaStream_t stream);
+int launch_attention_shared_mma(SaArgs a, int multiprocessors, int* error, cudaStream_t stream);
 bool attention_each_mma_takes(const SaArgs& a);
 int launch_attention_each_mma(const SaArgs& a, int multiprocessors, cudaStream_t stream);
 

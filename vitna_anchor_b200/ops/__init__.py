@@ -395,7 +395,7 @@ def set_wait_limit_ms(ms: float) -> None:
         raise KernelError(f"set_wait_limit_ms: CUDA error {status}")
 
 
-WAIT_FAMILIES = {"linear_tcgen05": 1, "linear_tcgen05_wide": 2, "attention_prefill_tcgen05": 3, "attention_decode_tma": 4, "delta_chunked": 5}
+WAIT_FAMILIES = {"linear_tcgen05": 1, "linear_tcgen05_wide": 2, "attention_prefill_tcgen05": 3, "attention_decode_tma": 4, "delta_chunked": 5, "attention_shared": 6}
 
 
 def skip_stage_once(family: str, stage: int) -> None:
@@ -2273,7 +2273,7 @@ SHARED_MAX_TOKENS, SHARED_MAX_HEADS, SHARED_MAX_KV_HEADS = 256, 64, 128      # t
 
 
 # vk_attention_shared's arguments in one piece: a call with two dozen arguments of their own takes ctypes 3 us, this 1
-_SHARED_ARGS = struct.Struct("QQQQQQQQQQQiiiiiiiiiifi")
+_SHARED_ARGS = struct.Struct("QQQQQQQQQQQiiiiiiiiiifiQ")
 
 
 def attention_shared_takes(dtype: torch.dtype, nh: int, nkv: int, hd: int, tokens: int = 1, reach: int = 1) -> bool:
@@ -2338,7 +2338,7 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
     if starts.shape[0] != families + 1 or families > SHARED_MAX_TOKENS:
         raise KernelError("attention_shared: starts is not one longer than shared, or there are more than 256 families")
     args = _SHARED_ARGS.pack(pq, pc, pt, ps, pp, pm, pst, psh, po, _fit(scratch, "scratch", torch.uint8, 1, here), scratch.numel(), T, segments, n, families, pages, nh, nkv,
-                             hd, page_size, max_blocks, scale, dtype is torch.bfloat16)
+                             hd, page_size, max_blocks, scale, dtype is torch.bfloat16, error_word().data_ptr())
     _check(_entry("vk_attention_shared", "pp")(args, torch._C._cuda_getCurrentRawStream(here)), "attention_shared")
     add_launches(1)                       # the walk, and the launch that joins the rows' parts
     return out
