@@ -458,12 +458,14 @@ __device__ __forceinline__ void sm_prefix_few(const SaArgs& a, const SaPlan& p, 
 // tensor memory.  Keys and values come by cp.async into rows of 128 bytes, 16-byte pieces at piece ^ (key & 7) (the 128-byte swizzle): keys two tiles ahead, values one, each into the
 // stage that the product before is known to have read.  While one group's weights are worked out the other's products run.
 //
-// Where: heads of 128 and 65 rows or more.  16 members of 16 heads over 2 of 128 (128 rows) behind 32,000 positions 28.0 us against 36.1 with mma.sync, behind 8,000 19.3 / 20.0; 32 members behind
-// 4,000 18.2 / 18.4.  With fewer rows the lanes that stand for none cost as much as the others (40 rows behind 16,000: 19.9 / 19.4; 64 behind 8,000, 8 key-value heads: 24.3 / 22.7), and heads of
-// 64 have half the products for the same exponentials: 64 rows behind 2,000, 32 heads, 27.7 / 24.3; 96 rows behind 4,000, 5 heads, 17.0 / 15.6.
+// Where: heads of 128 and 65 rows or more.  16 members of 16 heads over 2 of 128 (128 rows) behind 32,000 positions, whole call, 28.0 us against 36.1 with mma.sync, behind 8,000 19.3 / 20.0;
+// 32 members behind 4,000 18.2 / 18.4 (the launch that joins the parts has become faster since, for both).  With fewer rows the lanes that stand for none cost as much as the others (40 rows behind
+// 16,000: 19.9 / 19.4; 64 behind 8,000, 8 key-value heads: 24.3 / 22.7), and heads of 64 have half the products for the same exponentials: 64 rows behind 2,000, 32 heads, 27.7 / 24.3; 96 rows
+// behind 4,000, 5 heads, 17.0 / 15.6.
 //
-// What bounds it.  A tile takes its group 2,800 cycles (S 220 from its issue, a thread's 64 weights 1,500, P V 700 until the next S may begin), two groups beside one another; four tiles a
-// group in the first of these cases.  Before them are the plan, 5,000, the queries, pages and first keys, behind them the groups' meeting, 4,000, and the launch that joins the parts.
+// What bounds it.  A tile takes its group 2,800 cycles (S 220 from its issue, a thread's 64 weights 1,500, P V 700 until the next S may begin), two groups beside one another, and in the first of
+// these cases (26.6 us now) a group has four tiles.  Before them are the plan, 5,000, and the queries, pages and first keys, behind them the groups' meeting, 4,000, and the join: a short
+// chain that meets most of its instructions for the first time (4.6 warps wait for them for each that issues; the tensor pipe is at 10 %).
 constexpr int SM_TENSOR_ROWS = 65;
 
 template <int HD> struct SmTc {
@@ -586,21 +588,24 @@ __device__ __forceinline__ void sm_prefix_tc(const SaArgs& a, const SaPlan& p, c
         copy(n + 1, next, ring + (2 + ((n + 1) & 1)) * S::TILE, to_values);
         asm volatile("cp.async.commit_group;" ::: "memory");
         next = after;
-        uint32_t s[S::KEYS];
-        tmem_ld32_nowait(s_at + lanes, s);
-        tmem_ld32_nowait(s_at + lanes + 32, s + 32);
-        tmem_wait_ld();
-        tmem_loaded(s);
-        tmem_loaded(s + 32);
+        // 32 scores at a time, in loops that are not unrolled: a block walks few tiles, and instructions that it meets for the first time cost it more than the second reading
         const int left = part.k1 - (part.k0 + (group + 2 * n) * S::KEYS);
-        if (left < S::KEYS) {
-#pragma unroll
-            for (int j = 0; j < S::KEYS; j++)
-                if (j >= left) s[j] = 0xff800000u;
-        }
         float top = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < S::KEYS; c += 32) {
+            uint32_t s[32];
+            tmem_ld32(s_at + lanes + c, s);
+            tmem_loaded(s);
+            if (left < c + 32) {
 #pragma unroll
-        for (int j = 0; j < S::KEYS; j++) top = fmaxf(top, __uint_as_float(s[j]));
+                for (int j = 0; j < 32; j++)
+                    if (c + j >= left) s[j] = 0xff800000u;
+                tmem_st32(s_at + lanes + c, s);
+                tmem_wait_st();
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j++) top = fmaxf(top, __uint_as_float(s[j]));
+        }
         top *= scale;
         const bool ahead = top > m + SM_AHEAD;
         if (__any_sync(0xffffffffu, ahead)) {
@@ -620,12 +625,14 @@ __device__ __forceinline__ void sm_prefix_tc(const SaArgs& a, const SaPlan& p, c
         }
         const float ref = m == -INFINITY ? 0.0f : m;           // no score above -inf so far: p = 0
         float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < S::KEYS; c += 32) {
-            uint32_t hi[16], lo[16];
+            uint32_t s[32], hi[16], lo[16];
+            tmem_ld32(s_at + lanes + c, s);
+            tmem_loaded(s);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-                const float p0 = sa_ex2(fmaf(__uint_as_float(s[c + 2 * j]), scale, -ref)), p1 = sa_ex2(fmaf(__uint_as_float(s[c + 2 * j + 1]), scale, -ref));
+                const float p0 = sa_ex2(fmaf(__uint_as_float(s[2 * j]), scale, -ref)), p1 = sa_ex2(fmaf(__uint_as_float(s[2 * j + 1]), scale, -ref));
                 sum0 += p0;
                 sum1 += p1;
                 sm_split(p0, p1, hi[j], lo[j]);
