@@ -267,6 +267,33 @@ def test_attention_shared_of_many_rows_bad_blocks_and_no_number(ops):
     assert bool(torch.isnan(got[b.members]).all())
 
 
+def test_attention_shared_of_many_rows_replayed_on_two_streams(ops):
+    """Two calls at once on two streams, whose blocks both want tensor memory; a captured one follows other lengths."""
+    bs = [Batch([(3000, [5, 60, 17, 9, 30]), (0, [9])], 16, 1, 128, 16, BF16, seed=3 + k).device() for k in (0, 1)]
+    streams, graphs = [torch.cuda.Stream() for _ in bs], []
+    scratch = [torch.zeros(ops.attention_shared_scratch_bytes(6, 16, 1, 128), dtype=torch.uint8, device="cuda") for _ in bs]
+    for b, room in zip(bs, scratch):
+        b.run(ops, room)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(8):
+                b.run(ops, room)
+        b.pos = [max(0, p - 3) if t in b.members else p for t, p in enumerate(b.pos)]
+        b.d["pos"].copy_(torch.tensor(b.pos, dtype=torch.int32))
+        b.d["shared"].copy_(torch.tensor([2990, 0], dtype=torch.int32))
+        b.d["out"].fill_(7.0)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    ops.check_device_errors()
+    for b in bs:
+        want, tol = b.want()
+        assert float(((b.d["out"].double().cpu() - want).abs() - tol).max()) <= 0
+
+
 @pytest.mark.parametrize("tile,shared", [(0, 4000), (1, 30000)])      # of 4,000 keys a group of warps has one tile at most, of 30,000 (over at most 148 blocks) three or more
 def test_attention_shared_gives_up_a_wait_and_says_so(ops, tile, shared):
     """A tile of keys whose scores are never told of (a hook for this test; nothing faults): the waits run out after the 5 ms set here, the kernel returns by itself with its
