@@ -1,0 +1,54 @@
+"""Where a decode step's attention goes when its requests hold pages in common; no GPU is needed."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from vitna_anchor_b200 import ops
+
+
+@pytest.fixture
+def went(monkeypatch):
+    """Which attention a call reaches: every one is replaced by a note of its name."""
+    names = []
+    for name in ["attention_shared", "attention_decode", "attention_rows", "attention_prefill"]:
+        monkeypatch.setattr(ops, name, lambda *a, _name=name, **k: names.append(_name))
+    for name in ["attention_shared_scratch_bytes", "attention_decode_scratch_bytes"]:
+        monkeypatch.setattr(ops, name, lambda *a: 16)
+    return names
+
+
+def _step(dtype, hd, context, members=True, window=0, tokens=4, nh=4, nkv=2, page=16):
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32)      # noqa: E731
+    meta = SimpleNamespace(block_tables=ints(tokens, 1).expand(tokens, context // page), members=ints(tokens) if members else None, starts=ints(tokens + 1), shared=ints(tokens))
+    ws = SimpleNamespace(max_context=context, max_segments=tokens, max_tokens=64, flat=lambda name, n, dtype, zero=False: torch.zeros(n, dtype=dtype))
+    ctx = SimpleNamespace(num_dec=tokens, num_pre=0, num_tokens=tokens, pre_tiles=None, pre_tiles_big=None, pre_tokens=None, dec_tokens=None, workspace=ws, token_seg=ints(tokens),
+                          positions=ints(tokens), max_context=context)
+    q = torch.zeros(tokens, nh * hd, dtype=dtype)
+    ops.attention(q, torch.zeros(3, 2, nkv, page, hd, dtype=dtype), meta, ctx, torch.empty_like(q), nh, nkv, hd, 0.1, window)
+
+
+@pytest.mark.parametrize("context", [256, 32768, 32784, 65536, 131072, 1 << 20])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_common_pages_are_read_once_at_every_context(went, hd, context):
+    _step(torch.bfloat16, hd, context)
+    assert went == ["attention_shared"]
+
+
+@pytest.mark.parametrize("kw,name", [
+    (dict(context=32768, members=False), "attention_decode"), (dict(context=32784, members=False), "attention_rows"), (dict(context=256, window=64), "attention_decode"),
+    (dict(context=65536, window=64), "attention_rows"), (dict(context=256, tokens=257), "attention_decode"), (dict(context=65536, tokens=257), "attention_rows"),
+    (dict(context=256, dtype=torch.float32), "attention_rows"), (dict(context=65536, dtype=torch.float32), "attention_rows")])
+def test_the_other_steps_go_where_they_went(went, kw, name):
+    _step(**{"dtype": torch.bfloat16, "hd": 64, **kw})
+    assert went == [name]
+
+
+@pytest.mark.parametrize("context", [256, 65536])
+def test_float32_reads_common_pages_once_in_the_fast_routing_alone(went, context):
+    before = ops.set_float32_exact(False)
+    try:
+        _step(torch.float32, 64, context)
+    finally:
+        ops.set_float32_exact(before)
+    assert went == ["attention_shared"]

@@ -1,0 +1,74 @@
+"""Decode steps of requests that hold pages in common, through the step function: that the attention which reads those once is what runs, at every context, and what it gives."""
+import numpy as np
+import pytest
+import torch
+
+from tiny_configs import TINIES, write_tiny
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dirs(tmp_path_factory):
+    root = tmp_path_factory.mktemp("steps")
+    made = {}
+    for nh, kv, hd in [(6, 2, 64), (6, 1, 128), (4, 2, 32)]:
+        cfg = dict(TINIES["tinyA"]["config"], hidden_size=256, num_attention_heads=nh, num_key_value_heads=kv, head_dim=hd, vocab_size=500, max_position_embeddings=131072)
+        made[hd] = write_tiny(str(root / f"heads{hd}"), dict(TINIES["tinyA"], config=cfg), std=0.1)
+    return made
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """How many calls each attention of single tokens got."""
+    from vitna_anchor_b200 import ops
+    made = {}
+    for name in ["attention_shared", "attention_decode", "attention_rows"]:
+        def count(*a, _name=name, _of=getattr(ops, name), **k):
+            made[_name] = made.get(_name, 0) + 1
+            return _of(*a, **k)
+        monkeypatch.setattr(ops, name, count)
+    return made
+
+
+def _play(model, context, members, prompt, mode, steps=6, graphs=True):
+    """Requests forked from one after its prompt, some steps of single tokens beside a stranger; every step's logits."""
+    from vitna_anchor_b200 import ops
+    from vitna_anchor_b200.engine.runner import ModelRunner, StepEntry
+    before = ops.set_attention_shared(mode)
+    try:
+        r = ModelRunner(model, page_size=16, max_requests=members + 1, max_batch_tokens=512, max_model_len=context, num_pages=100 + len(prompt) // 16 + members * 3, cuda_graphs=graphs)
+        r.open("s")
+        r.step([StepEntry("s", prompt[:30], [])])
+        r.open(0)
+        for at in range(0, len(prompt), 512):
+            r.step([StepEntry(0, prompt[at:at + 512], [])])
+        for i in range(1, members):
+            r.fork(0, i)
+        rng = np.random.default_rng(9)
+        order = ["s", *range(members)]
+        rng.shuffle(order)
+        order = [o if o == "s" else int(o) for o in order]
+        out = []
+        for _ in range(steps):
+            out.append(r.step([StepEntry(rid, [int(rng.integers(0, model.vocab_size))], [0]) for rid in order]).clone())
+        r.check()
+        r.cache.check()
+        return torch.stack(out)
+    finally:
+        ops.set_attention_shared(before)
+
+
+# tables so wide that the members are not walked one by one (heads of 64: 96 MB, of 128: 240 MB of them); rows of a key-value head's product: 48, 93; 102 (tcgen05 from 65 on)
+@pytest.mark.parametrize("hd,members,context", [(64, 16, 32768), (64, 31, 32768), (64, 31, 65536), (128, 17, 32768), (128, 17, 65536), (128, 9, 131072), (32, 5, 65536)])
+def test_common_pages_are_read_once_at_every_context(hd, members, context, dirs, calls):
+    """bfloat16, against the same steps with every request read by itself: 3e-2 of the logits' scale, as between two ways of cutting one request."""
+    from vitna_anchor_b200.engine.loading import load_model
+    model = load_model(dirs[hd], "bfloat16", "cuda")
+    prompt = [int(t) for t in np.random.default_rng(5).integers(0, model.vocab_size, 1203)]
+    a = _play(model, context, members, prompt, 1)
+    assert calls["attention_shared"] > 0 and "attention_decode" not in calls
+    shared, _ = calls.pop("attention_shared"), calls.pop("attention_rows", 0)
+    b = _play(model, context, members, prompt, 0)
+    assert "attention_shared" not in calls and calls["attention_decode" if context <= 32768 else "attention_rows"] >= shared
+    assert float((a - b).abs().max()) <= 3e-2 * float(b.abs().max())

@@ -746,14 +746,15 @@ def attention_prefill_tcgen05(q: torch.Tensor, cache_layer: torch.Tensor, block_
 def attention(q: torch.Tensor, pages: torch.Tensor, meta, ctx, out: torch.Tensor, nh: int, nkv: int, hd: int,
               scale: float, window: int = 0) -> torch.Tensor:
     """Causal attention of a mixed batch over the paged cache; `meta` is the page group's GroupMeta.
-    Single decoded tokens take the split-key kernel, or, where requests hold pages in common, the one that reads those once for all of them; tokens of prompt portions take the tensor-core kernel
-    (bfloat16, head sizes it is built for); whatever is left takes attention_rows, which takes every size."""
-    dec_ok = (bool(ctx.num_dec) and attention_decode_takes(q.dtype, hd, ctx.workspace.max_context)
-              and not (q.dtype == torch.float32 and _float32_exact))
+    Single decoded tokens take the split-key kernel (contexts of up to 32,768 positions), or, where requests hold pages in common, the one that reads those once for all of them
+    (every context); tokens of prompt portions take the tensor-core kernel (bfloat16, head sizes it is built for); whatever is left takes attention_rows, which takes every size."""
+    twins = q.dtype != torch.float32 or not _float32_exact       # the serving kernels; exact float32 has attention_rows alone
+    shared_ok = (bool(ctx.num_dec) and twins and meta.members is not None and window == 0 and q.data_ptr() % 16 == 0
+                 and attention_shared_takes(q.dtype, nh, nkv, hd, ctx.num_tokens, meta.block_tables.shape[1] * pages.shape[3]))
+    dec_ok = shared_ok or (bool(ctx.num_dec) and twins and attention_decode_takes(q.dtype, hd, ctx.workspace.max_context))
     pre_ok = (bool(ctx.num_pre) and q.dtype == torch.bfloat16 and hd in PREFILL_HEAD_SIZES and ctx.pre_tiles is not None
               and q.data_ptr() % 16 == 0)
-    if dec_ok and meta.members is not None and window == 0 and attention_shared_takes(q.dtype, nh, nkv, hd, ctx.num_tokens, meta.block_tables.shape[1] * pages.shape[3]) \
-            and q.data_ptr() % 16 == 0:
+    if shared_ok:
         ws = ctx.workspace
         scratch = ws.flat(f"att.shared/{nh}/{hd}", attention_shared_scratch_bytes(min(ws.max_segments, SHARED_MAX_TOKENS), nh, nkv, hd), torch.uint8)
         attention_shared(q, pages, meta.block_tables, ctx.token_seg, ctx.positions, meta.members, meta.starts, meta.shared, out, scratch, nh, nkv, hd, scale)
