@@ -52,3 +52,55 @@ def test_float32_reads_common_pages_once_in_the_fast_routing_alone(went, context
     finally:
         ops.set_float32_exact(before)
     assert went == ["attention_shared"]
+
+
+class _Builder:
+    """A ContextBuilder over tables alone, on the host."""
+
+    def __new__(cls, monkeypatch, groups, page_size=4, requests=6, model_len=64):
+        from vitna_anchor_b200.cache import CacheManager
+        from vitna_anchor_b200.engine import context
+        staging = context._Staging
+        monkeypatch.setattr(context, "_Staging", lambda n, pinned: staging(n, False))
+        monkeypatch.setattr(context.ContextBuilder, "_send", lambda self, st, words: self.meta_dev[:words].copy_(st.host[:words]))
+        cache = CacheManager(groups, page_size=page_size, num_pages=200, max_requests=requests, dtype=torch.bfloat16, device="cpu", allocate=False)
+        return context.ContextBuilder(cache, torch.bfloat16, None, max_batch_tokens=32, max_segments=requests, max_model_len=model_len, device="cpu")
+
+
+def _advance(cache, rid, n):
+    cache.reserve_step([(rid, n)])
+    cache.commit_step([(rid, n)])
+
+
+@pytest.mark.parametrize("build", ["build", "build_decode"])
+def test_a_step_of_single_tokens_names_its_families(monkeypatch, build):
+    """With and without graphs: who holds what in common, in groups without a window."""
+    from vitna_anchor_b200.cache import KVSpec
+    b = _Builder(monkeypatch, [KVSpec(2, 64), KVSpec(2, 64, window=5)])
+    c = b.cache
+    for rid, n in [("a", 11), ("x", 3), ("p", 8)]:
+        c.open(rid)
+        _advance(c, rid, n)
+    for source, rid in [("a", "b"), ("p", "q"), ("a", "c")]:
+        c.tables.fork(source, rid)
+    _advance(c, "b", 6)
+    order = ["c", "p", "x", "a", "q", "b"]
+    before = ops.set_attention_shared(1)
+    try:
+        c.reserve_step([(rid, 1) for rid in order])
+        if build == "build":
+            ctx, _ = b.build([(rid, [1], [0]) for rid in order])
+            assert b.build([(rid, [1], [0]) for rid in order], for_graph=True)[0].groups[0].members is None
+        else:
+            ctx, _ = b.build_decode(order, [1] * 6, 6, families=b.families(order))
+    finally:
+        ops.set_attention_shared(before)
+    meta, window = ctx.groups
+    assert window.members is None
+    assert meta.members.tolist() == [0, 3, 5, 1, 4, 2] and meta.starts.tolist() == [0, 3, 5, 6, 6, 6, 6]
+    assert meta.shared.tolist() == [8, 8, 0, 0, 0, 0]           # two whole pages of four of a's eleven positions, both of p's
+    for f, shared in zip(([0, 3, 5], [1, 4]), (8, 8)):
+        tables = meta.block_tables[f][:, :shared // 4]
+        assert bool((tables == tables[0]).all())
+    c.rollback_step([(rid, 1) for rid in order])
+    c.check()

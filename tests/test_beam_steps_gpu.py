@@ -72,3 +72,18 @@ def test_common_pages_are_read_once_at_every_context(hd, members, context, dirs,
     b = _play(model, context, members, prompt, 0)
     assert "attention_shared" not in calls and calls["attention_decode" if context <= 32768 else "attention_rows"] >= shared
     assert float((a - b).abs().max()) <= 3e-2 * float(b.abs().max())
+
+
+@pytest.mark.parametrize("hd,context", [(64, 32768), (128, 65536), (32, 256)])
+def test_common_pages_are_read_once_without_graphs(hd, context, dirs, calls):
+    """Steps that are issued launch by launch, against every request read by itself (the tolerance of the test above)."""
+    from vitna_anchor_b200.engine.loading import load_model
+    model = load_model(dirs[hd], "bfloat16", "cuda")
+    members = 5 if hd == 32 else 17
+    prompt = [int(t) for t in np.random.default_rng(6).integers(0, model.vocab_size, 150 if hd == 32 else 1203)]
+    a = _play(model, context, members, prompt, 1, graphs=False)
+    assert calls["attention_shared"] > 0 and "attention_decode" not in calls
+    calls.pop("attention_shared")
+    b = _play(model, context, members, prompt, 0, graphs=False)
+    assert "attention_shared" not in calls
+    assert float((a - b).abs().max()) <= 3e-2 * float(b.abs().max())

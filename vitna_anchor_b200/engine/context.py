@@ -67,7 +67,8 @@ class ContextBuilder:
         self.max_blocks = -(-max_model_len // self.page_size)
         self.max_segments = max_segments
         n_groups = len(cache.groups)
-        decode_words = 7 * max_segments + 1 + n_groups * (max_segments + max_segments * self.max_blocks + 3 * max_segments + 1)
+        # batches of single tokens with their families (build: 8 S + 1 and up to 3 of alignment; build_decode: 7 S + 1)
+        decode_words = 8 * max_segments + 4 + n_groups * (max_segments + max_segments * self.max_blocks + 3 * max_segments + 1)
         self.meta_len = max(meta_words(max_batch_tokens, max_segments, self.max_blocks, n_groups), decode_words) + 8
         self._staging = [_Staging(self.meta_len, True) for _ in range(4)]
         self._turn = 0
@@ -158,10 +159,15 @@ class ContextBuilder:
                 row = np.where(row == UNMAPPED, 0, row)      # pages behind a window are never read
                 bt[i, :len(row)] = row
             group_slices.append((put(sm, T), put(bt.reshape(-1), S * maxb)))
+        # (a captured batch of these counts has none: what requests share is not among the counts)
+        families = self.families([rid for rid, _, _ in segments]) if not for_graph and T == S else None
+        family_slices = [put(self._family_words(families, S, S, g), 3 * S + 1) for g in range(len(self.cache.groups))] if families else []
         self._send(st, off)
 
         dev = self.meta_dev
         groups = [GroupMeta(dev[a], dev[b].view(S, maxb), maxb) for a, b in group_slices]
+        for g, sl in enumerate(family_slices):
+            self._set_families(groups[g], g, dev[sl], S)
         ctx = StepContext(
             num_tokens=T, num_segments=S, dtype=self.dtype, tokens=dev[s_tokens], positions=dev[s_pos],
             token_seg=dev[s_seg], seg_starts=dev[s_starts], seg_context=dev[s_ctx], seg_slots=dev[s_slots], groups=groups,
@@ -189,6 +195,21 @@ class ContextBuilder:
             if ops.attention_shared_pays(saved, group.num_kv_heads, group.head_dim):
                 return out
         return None
+
+    @staticmethod
+    def _family_words(families: List[Tuple[List[int], List[int]]], S: int, B: int, g: int) -> np.ndarray:
+        """A page group's members [B], starts [B + 1] and shared [B] of a batch of S single tokens padded to B: a padding token is a family of its own."""
+        words = np.zeros(3 * B + 1, dtype=np.int32)
+        sizes = [len(f) for f, _ in families] + [1] * (B - S)
+        words[:B] = [i for f, _ in families for i in f] + list(range(S, B))
+        words[B + 1:B + 1 + len(sizes)] = np.cumsum(sizes)
+        words[B + 1 + len(sizes):2 * B + 1] = B
+        words[2 * B + 1:2 * B + 1 + len(families)] = [shared[g] for _, shared in families]
+        return words
+
+    def _set_families(self, meta: GroupMeta, g: int, words: torch.Tensor, B: int) -> None:
+        if self.cache.groups[g].window == 0:
+            meta.members, meta.starts, meta.shared = words[:B], words[B:2 * B + 1], words[2 * B + 1:]
 
     def build_decode(self, requests: Sequence[Hashable], tokens: Sequence[int], B: int, views: bool = True, reach: int = 0,
                      families: Optional[List[Tuple[List[int], List[int]]]] = None):
@@ -234,12 +255,7 @@ class ContextBuilder:
                 bt[i, :len(row)] = row
             if families:
                 o = o_families + g * (3 * B + 1)
-                order = [i for f, _ in families for i in f] + list(range(S, B))
-                sizes = [len(f) for f, _ in families] + [1] * (B - S)
-                buf[o:o + B] = order
-                buf[o + B + 1:o + B + 1 + len(sizes)] = np.cumsum(sizes)
-                buf[o + B + 1 + len(sizes):o + 2 * B + 1] = B
-                buf[o + 2 * B + 1:o + 2 * B + 1 + len(families)] = [shared[g] for _, shared in families]
+                buf[o:o + 3 * B + 1] = self._family_words(families, S, B, g)
         self._send(st, total)
         if not views:               # a replay needs the arrays in place, not their description
             return None, None
@@ -248,9 +264,9 @@ class ContextBuilder:
         for g in range(n_groups):
             o_sm = o_groups + g * (B + B * maxb)
             meta = GroupMeta(dev[o_sm:o_sm + B], dev[o_sm + B:o_sm + B + B * maxb].view(B, maxb), maxb)
-            if families and self.cache.groups[g].window == 0:
+            if families:
                 o = o_families + g * (3 * B + 1)
-                meta.members, meta.starts, meta.shared = dev[o:o + B], dev[o + B:o + 2 * B + 1], dev[o + 2 * B + 1:o + 3 * B + 1]
+                self._set_families(meta, g, dev[o:o + 3 * B + 1], B)
             groups.append(meta)
         ctx = StepContext(
             num_tokens=B, num_segments=B, dtype=self.dtype, tokens=dev[o_tok:o_tok + B], positions=dev[o_pos:o_pos + B],
