@@ -57,14 +57,14 @@ def test_float32_reads_common_pages_once_in_the_fast_routing_alone(went, context
 class _Builder:
     """A ContextBuilder over tables alone, on the host."""
 
-    def __new__(cls, monkeypatch, groups, page_size=4, requests=6, model_len=64):
+    def __new__(cls, monkeypatch, groups, page_size=4, requests=6, model_len=64, dtype=torch.bfloat16, **kw):
         from vitna_anchor_b200.cache import CacheManager
         from vitna_anchor_b200.engine import context
         staging = context._Staging
         monkeypatch.setattr(context, "_Staging", lambda n, pinned: staging(n, False))
         monkeypatch.setattr(context.ContextBuilder, "_send", lambda self, st, words: self.meta_dev[:words].copy_(st.host[:words]))
-        cache = CacheManager(groups, page_size=page_size, num_pages=200, max_requests=requests, dtype=torch.bfloat16, device="cpu", allocate=False)
-        return context.ContextBuilder(cache, torch.bfloat16, None, max_batch_tokens=32, max_segments=requests, max_model_len=model_len, device="cpu")
+        cache = CacheManager(groups, page_size=page_size, num_pages=200, max_requests=requests, dtype=dtype, device="cpu", allocate=False)
+        return context.ContextBuilder(cache, dtype, None, max_batch_tokens=32, max_segments=requests, max_model_len=model_len, device="cpu", **kw)
 
 
 def _advance(cache, rid, n):
@@ -104,3 +104,42 @@ def test_a_step_of_single_tokens_names_its_families(monkeypatch, build):
         assert bool((tables == tables[0]).all())
     c.rollback_step([(rid, 1) for rid in order])
     c.check()
+
+
+def _named(monkeypatch, n, dtype=torch.bfloat16, heads=(32, 32, 64), requests=2):
+    """Whether a step of requests that hold `n` positions of 32 heads of 64 in common names its families."""
+    from vitna_anchor_b200.cache import KVSpec
+    b = _Builder(monkeypatch, [KVSpec(32, 64)], page_size=512, requests=requests, model_len=131072, dtype=dtype, common_heads=heads and {0: heads})
+    b.cache.open(0)
+    _advance(b.cache, 0, n)
+    for i in range(1, requests):
+        b.cache.tables.fork(0, i)
+    return b.families(list(range(requests))) is not None
+
+
+def test_families_are_named_only_where_an_attention_reads_them(monkeypatch):
+    """A model none of whose attentions can, a type whose routing has another kernel, more tokens than the kernel takes: no second graph, and no words that nobody reads."""
+    assert _named(monkeypatch, 8192) and not _named(monkeypatch, 8192 - 512)                   # 64 MB from 8,192 positions on in bfloat16
+    assert not _named(monkeypatch, 32768, heads=None)
+    assert not _named(monkeypatch, 32768, dtype=torch.float32)
+    before = ops.set_float32_exact(False)
+    try:
+        assert _named(monkeypatch, 4096, dtype=torch.float32) and not _named(monkeypatch, 4096 - 512, dtype=torch.float32)      # and from 4,096 in float32
+    finally:
+        ops.set_float32_exact(before)
+    assert _named(monkeypatch, 8192, requests=256) and not _named(monkeypatch, 8192, requests=257)
+    ops.set_attention_shared(1)
+    try:
+        assert _named(monkeypatch, 512, heads=None)                                             # every step that shares, whatever reads it
+    finally:
+        ops.set_attention_shared(2)
+
+
+def test_which_attentions_can_read_common_pages_once():
+    from vitna_anchor_b200.parts.attention import PagedAttention
+    from vitna_anchor_b200.parts.base import Mixer
+    w, wo = torch.zeros(4 * 16 + 2 * 2 * 16, 8), torch.zeros(8, 4 * 16)
+    assert PagedAttention(8, 4, 2, 16, w, wo, None).common_heads() == (4, 2, 16)
+    assert PagedAttention(8, 4, 2, 16, w, wo, None, window=9).common_heads() is None
+    assert PagedAttention(8, 4, 2, 16, w, wo, None, qk_norm_eps=1e-6).common_heads() is None
+    assert Mixer().common_heads() is None

@@ -95,6 +95,11 @@ class PagePool:
     def is_shared(self, page: int) -> bool:
         return page in self._more
 
+    @property
+    def has_shared(self) -> bool:
+        """Whether any page has several holders."""
+        return bool(self._more)
+
     def owner(self, page: int) -> Optional[Hashable]:
         return self._owner[page]
 

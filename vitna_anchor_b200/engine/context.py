@@ -10,7 +10,7 @@ they see the same layout the step function produces.
 """
 from __future__ import annotations
 
-from typing import Hashable, List, Optional, Sequence, Tuple
+from typing import Dict, Hashable, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -59,13 +59,16 @@ def words_used(lens: Sequence[int], wanted: int, max_blocks: int, n_groups: int)
 
 class ContextBuilder:
     def __init__(self, cache: CacheManager, dtype: torch.dtype, workspace: Workspace, *, max_batch_tokens: int,
-                 max_segments: int, max_model_len: int, device):
+                 max_segments: int, max_model_len: int, device, common_heads: Optional[Dict[int, Tuple[int, int, int]]] = None):
+        # common_heads: by cache layer, of the attentions that can read common pages once (DecoderModel.common_heads)
         self.cache, self.dtype, self.workspace = cache, dtype, workspace
         self.device = torch.device(device)
         self.page_size = cache.page_size
         self.max_model_len = max_model_len
         self.max_blocks = -(-max_model_len // self.page_size)
         self.max_segments = max_segments
+        heads = common_heads or {}
+        self._common_heads = [sorted({heads[c] for c in group.cache_ids if c in heads}) for group in cache.groups]
         n_groups = len(cache.groups)
         # batches of single tokens with their families (build: 8 S + 1 and up to 3 of alignment; build_decode: 7 S + 1)
         decode_words = 8 * max_segments + 4 + n_groups * (max_segments + max_segments * self.max_blocks + 3 * max_segments + 1)
@@ -183,8 +186,10 @@ class ContextBuilder:
     # -- single tokens, padded to a fixed number of segments -----------------------------------------------
     def families(self, requests: Sequence[Hashable]) -> Optional[List[Tuple[List[int], List[int]]]]:
         """What requests of a batch of single tokens hold in common: for every family its places in the batch and the positions it shares in each page
-        group (0 in groups with a window).  None where reading those once is not worth it (ops.attention_shared_pays)."""
+        group (0 in groups with a window).  None where no attention would read those once, or it is not worth it (ops.attention_shared_serves, ops.attention_shared_pays)."""
         tables, ps = self.cache.tables, self.page_size
+        if not any(pool.has_shared for pool in tables.pools):
+            return None
         by_family = tables.families(requests)
         if len(by_family) == len(requests):
             return None
@@ -192,7 +197,8 @@ class ContextBuilder:
                for f in by_family]
         for g, group in enumerate(self.cache.groups):
             saved = sum((len(f) - 1) * shared[g] for f, shared in out)
-            if ops.attention_shared_pays(saved, group.num_kv_heads, group.head_dim):
+            read = any(ops.attention_shared_serves(self.dtype, *heads, len(requests), self.max_blocks * ps) for heads in self._common_heads[g])
+            if ops.attention_shared_pays(saved, group.num_kv_heads, group.head_dim, self.dtype, read):
                 return out
         return None
 

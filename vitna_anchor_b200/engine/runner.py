@@ -92,7 +92,8 @@ class ModelRunner:
         self.workspace = Workspace(self.device, max_batch_tokens, max_requests, self.max_model_len)
         self.max_segments = max_requests
         self.builder = ContextBuilder(self.cache, model.dtype, self.workspace, max_batch_tokens=max_batch_tokens,
-                                      max_segments=max_requests, max_model_len=self.max_model_len, device=self.device)
+                                      max_segments=max_requests, max_model_len=self.max_model_len, device=self.device,
+                                      common_heads=getattr(model, "common_heads", None))
         self._meta_dev = self.builder.meta_dev
         self._fail_at: Optional[int] = None
         self._fail_after_run: Optional[int] = None

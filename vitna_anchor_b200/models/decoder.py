@@ -19,7 +19,7 @@ with).  Such a part sees the embedding output once, right after it is made (reme
 from __future__ import annotations
 
 from dataclasses import dataclass, replace
-from typing import List, Optional, Sequence
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -111,6 +111,12 @@ class DecoderModel:
                     out |= of(sub)
             return out
         return sorted(set().union(*(of(p) for p in self.parts() if p is not None)))
+
+    @property
+    def common_heads(self) -> Dict[int, Tuple[int, int, int]]:
+        """By cache layer, for those that an attention reads which can read common pages once (Mixer.common_heads)."""
+        heads = ((run.cache, self.blocks[run.block].mixer.common_heads()) for run in self.schedule if run.cache >= 0)
+        return {cache: h for cache, h in heads if h is not None}
 
     def forward(self, ctx: StepContext, logit_rows: Optional[torch.Tensor], out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """Run the batch; float32 logits [len(logit_rows), vocab] for the flat token indices in logit_rows

@@ -748,10 +748,10 @@ def attention(q: torch.Tensor, pages: torch.Tensor, meta, ctx, out: torch.Tensor
     """Causal attention of a mixed batch over the paged cache; `meta` is the page group's GroupMeta.
     Single decoded tokens take the split-key kernel (contexts of up to 32,768 positions), or, where requests hold pages in common, the one that reads those once for all of them
     (every context); tokens of prompt portions take the tensor-core kernel (bfloat16, head sizes it is built for); whatever is left takes attention_rows, which takes every size."""
-    twins = q.dtype != torch.float32 or not _float32_exact       # the serving kernels; exact float32 has attention_rows alone
-    shared_ok = (bool(ctx.num_dec) and twins and meta.members is not None and window == 0 and q.data_ptr() % 16 == 0
-                 and attention_shared_takes(q.dtype, nh, nkv, hd, ctx.num_tokens, meta.block_tables.shape[1] * pages.shape[3]))
-    dec_ok = shared_ok or (bool(ctx.num_dec) and twins and attention_decode_takes(q.dtype, hd, ctx.workspace.max_context))
+    shared_ok = (bool(ctx.num_dec) and meta.members is not None and window == 0 and q.data_ptr() % 16 == 0
+                 and attention_shared_serves(q.dtype, nh, nkv, hd, ctx.num_tokens, meta.block_tables.shape[1] * pages.shape[3]))
+    dec_ok = shared_ok or (bool(ctx.num_dec) and attention_decode_takes(q.dtype, hd, ctx.workspace.max_context)
+                           and not (q.dtype == torch.float32 and _float32_exact))
     pre_ok = (bool(ctx.num_pre) and q.dtype == torch.bfloat16 and hd in PREFILL_HEAD_SIZES and ctx.pre_tiles is not None
               and q.data_ptr() % 16 == 0)
     if shared_ok:
@@ -2284,25 +2284,30 @@ def attention_shared_takes(dtype: torch.dtype, nh: int, nkv: int, hd: int, token
             and (reach // 16 + 64) * tokens * nh < 1 << 31 and tokens * nh * hd * 4 < 1 << 31)      # the kernels count tiles of 16 keys and rows of outputs in 31 bits
 
 
+def attention_shared_serves(dtype: torch.dtype, nh: int, nkv: int, hd: int, tokens: int, reach: int) -> bool:
+    """Whether ops.attention gives a decode step of these sizes that names its families to attention_shared (exact float32 has attention_rows alone)."""
+    return not (dtype == torch.float32 and _float32_exact) and attention_shared_takes(dtype, nh, nkv, hd, tokens, reach)
+
+
 _shared_mode = 2
 
 
 def set_attention_shared(mode: int) -> int:
-    """Which decode steps of requests with pages in common go through attention_shared: 0 none, 1 all, 2 those that its rule gives it (the default).
-    Returns the mode that was in force."""
+    """Which decode steps of requests with pages in common name what those share, so that an attention that can reads it once: 0 none, 1 all (whatever reads them), 2 those that the
+    rule gives to attention_shared (the default).  Returns the mode that was in force."""
     global _shared_mode
     before, _shared_mode = _shared_mode, int(mode)
     return before
 
 
-def attention_shared_pays(saved: int, nkv: int, hd: int) -> bool:
+def attention_shared_pays(saved: int, nkv: int, hd: int, dtype: torch.dtype = torch.bfloat16, read: bool = True) -> bool:
     """Whether a decode step whose requests would read `saved` cached positions again and again goes through attention_shared rather than attention_decode: from 64 MB of
-    them on (bfloat16).  Whole steps of a beam search, this way against the other: 8 beams of 2,000 positions, 32 heads of 64 over 24 layers (115 MB), 1.70 ms against 1.84, 64 of 8,000
+    them on, where an attention would read them once (`read`).  Whole steps of a beam search, this way against the other: 8 beams of 2,000 positions, 32 heads of 64 over 24 layers (115 MB), 1.70 ms against 1.84, 64 of 8,000
     (4.1 GB) 4.5 / 16.0; 16 of 4,000, 5 heads, 32 layers (77 MB) 1.68 / 1.72; 4 of 2,000, 32 heads (49 MB) 1.61 / 1.49, 16 of 500 (61 MB) 1.77 / 1.71; 32 of 500, 3 heads, 30 layers
     (12 MB) 1.38 / 1.20.  Below, at 3 and 5 heads and 4,000 positions and more, up to 0.2 ms of 1.4 are left."""
     if _shared_mode != 2:
         return _shared_mode == 1 and saved > 0
-    return saved * nkv * hd * 4 >= 64 << 20
+    return read and saved * nkv * hd * 2 * dtype.itemsize >= 64 << 20
 
 
 def attention_shared_scratch_bytes(tokens: int, nh: int, nkv: int, hd: int) -> int:

@@ -82,6 +82,9 @@ class PagedAttention(Mixer):
     def cache_spec(self):
         return KVSpec(self.nkv, self.hd, self.window, self.vd if self.vd != self.hd else 0)
 
+    def common_heads(self):
+        return None if self.unrotated or self.window else (self.nh, self.nkv, self.hd)
+
     def fuses_norm(self, norm, ctx: StepContext) -> bool:
         return (not self.unrotated and norm.as_rms() is not None
                 and ops.fused_norm_takes(ctx.dtype, ctx.num_tokens, self.hidden, self.qd + 2 * self.kvd))

@@ -216,6 +216,11 @@ class Mixer(Part):
         run of such a mixer names a second cache layer for it, and forward() finds it in cache.state."""
         return None
 
+    def common_heads(self) -> Optional[Tuple[int, int, int]]:
+        """(heads, key-value heads, size of a head) of an attention that can read what requests hold in common once (ops.attention with the
+        families of GroupMeta); None: it reads every request's pages by themselves, whatever the batch says of families."""
+        return None
+
     def forward(self, xn: torch.Tensor, ctx: StepContext, cache: Optional[LayerCacheView], residual: torch.Tensor,
                 write_cache: bool = True, norm: Optional["Norm"] = None) -> None:
         """xn [T, hidden] in the compute dtype; adds the result into residual (float32 [T, hidden]).
