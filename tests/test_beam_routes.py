@@ -106,10 +106,10 @@ def test_a_step_of_single_tokens_names_its_families(monkeypatch, build):
     c.check()
 
 
-def _named(monkeypatch, n, dtype=torch.bfloat16, heads=(32, 32, 64), requests=2):
+def _named(monkeypatch, n, dtype=torch.bfloat16, heads=(32, 32, 64), requests=2, model_len=32768):
     """Whether a step of requests that hold `n` positions of 32 heads of 64 in common names its families."""
     from vitna_anchor_b200.cache import KVSpec
-    b = _Builder(monkeypatch, [KVSpec(32, 64)], page_size=512, requests=requests, model_len=131072, dtype=dtype, common_heads=heads and {0: heads})
+    b = _Builder(monkeypatch, [KVSpec(32, 64)], page_size=512, requests=requests, model_len=model_len, dtype=dtype, common_heads=heads and {0: heads})
     b.cache.open(0)
     _advance(b.cache, 0, n)
     for i in range(1, requests):
@@ -127,6 +127,7 @@ def test_families_are_named_only_where_an_attention_reads_them(monkeypatch):
         assert _named(monkeypatch, 4096, dtype=torch.float32) and not _named(monkeypatch, 4096 - 512, dtype=torch.float32)      # and from 4,096 in float32
     finally:
         ops.set_float32_exact(before)
+    assert _named(monkeypatch, 512, model_len=65536) and not _named(monkeypatch, 512, heads=None, model_len=65536)              # 4 MB of what the general attention would read again
     assert _named(monkeypatch, 8192, requests=256) and not _named(monkeypatch, 8192, requests=257)
     ops.set_attention_shared(1)
     try:
@@ -143,3 +144,18 @@ def test_which_attentions_can_read_common_pages_once():
     assert PagedAttention(8, 4, 2, 16, w, wo, None, window=9).common_heads() is None
     assert PagedAttention(8, 4, 2, 16, w, wo, None, qk_norm_eps=1e-6).common_heads() is None
     assert Mixer().common_heads() is None
+
+
+# (positions that would be read again, key-value heads, their size, type, context): both sides of every line, from the measured ones
+@pytest.mark.parametrize("sizes,once", [
+    ((7 * 2000, 32, 64, torch.bfloat16, 4096), True), ((3 * 2000, 32, 64, torch.bfloat16, 4096), False), ((15 * 4000, 5, 64, torch.bfloat16, 8192), True), ((31 * 500, 3, 64, torch.bfloat16, 8192), False),
+    ((15 * 2000, 8, 128, torch.bfloat16, 4096), True), ((3 * 2000, 8, 128, torch.bfloat16, 16384), False),
+    ((7 * 2000, 32, 96, torch.bfloat16, 4608), False), ((63 * 8000, 4, 96, torch.bfloat16, 8192), False), ((63 * 8000, 4, 32, torch.bfloat16, 8192), False), ((63 * 8000, 4, 16, torch.bfloat16, 8192), False),
+    ((3 * 4000, 32, 256, torch.bfloat16, 4096), False), ((15 * 4000, 4, 80, torch.bfloat16, 4096), True), ((63 * 4000, 4, 24, torch.bfloat16, 4096), True), ((3 * 4000, 4, 80, torch.bfloat16, 4096), False),
+    ((31 * 2000, 3, 64, torch.float32, 4096), True), ((7 * 2000, 3, 64, torch.float32, 4096), False), ((3 * 2000, 32, 64, torch.float32, 4096), True), ((15 * 2000, 4, 128, torch.float32, 4096), True),
+    ((3 * 2000, 5, 64, torch.bfloat16, 65536), True), ((3 * 8000, 32, 32, torch.bfloat16, 65536), True), ((500, 32, 256, torch.bfloat16, 65536), True), ((96, 32, 256, torch.bfloat16, 65536), False),
+    ((48, 2, 64, torch.bfloat16, 65536), False), ((3 * 2000, 5, 64, torch.bfloat16, 32768), False)])
+def test_where_reading_common_pages_once_was_measured_to_be_faster(sizes, once):
+    saved, nkv, hd, dtype, context = sizes
+    assert ops.attention_shared_pays(saved, nkv, hd, dtype, True, context) == once
+    assert not ops.attention_shared_pays(saved, nkv, hd, dtype, False, context)

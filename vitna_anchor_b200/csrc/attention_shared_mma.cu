@@ -459,7 +459,9 @@ __device__ __forceinline__ void sm_prefix_few(const SaArgs& a, const SaPlan& p, 
 // stage that the product before is known to have read.  While one group's weights are worked out the other's products run.
 //
 // Where: heads of 128 and 65 rows or more.  16 members of 16 heads over 2 of 128 (128 rows) behind 32,000 positions, whole call, 28.0 us against 36.1 with mma.sync, behind 8,000 19.3 / 20.0;
-// 32 members behind 4,000 18.2 / 18.4 (the launch that joins the parts has become faster since, for both).  With fewer rows the lanes that stand for none cost as much as the others (40 rows behind
+// 32 members behind 4,000 18.2 / 18.4 (the launch that joins the parts has become faster since, for both).  Between 64 and 128 rows, eight of them a member: over 2 heads behind 16,000 and 32,000
+// 72 rows 20.6 / 22.7 and 26.0 / 31.6, 96 rows 20.1 / 23.5 and 26.8 / 32.3, 120 rows 20.6 / 24.0 and 26.6 / 33.6, over 8 heads 34.5 / 48.9 and 51.4 / 79.4, 36.9 / 49.7 and 51.9 / 79.7, 36.8 / 50.2
+// and 54.8 / 89.4; behind 4,000 both the same within 3 %, but 120 rows over 8 heads 25.1 / 22.8.  With up to 64 rows the lanes that stand for none cost as much as the others (40 rows behind
 // 16,000: 19.9 / 19.4; 64 behind 8,000, 8 key-value heads: 24.3 / 22.7), and heads of 64 have half the products for the same exponentials: 64 rows behind 2,000, 32 heads, 27.7 / 24.3; 96 rows
 // behind 4,000, 5 heads, 17.0 / 15.6.
 //
@@ -861,6 +863,9 @@ bool attention_shared_mma_takes(const SaArgs& a, int dtype) {
 // 32 of 2,048, 5 heads (87 MB), 12.7 / 14.4; 8 of 2,048, 5 heads (44 MB), 6.6 / 9.8; 4 of 2,048, 32 heads (70 MB), 8.8 / 10.6; 16 of 512, 32 heads (78 MB), 10.3 / 11.3; 16 of 8,000, 3 heads
 // (99 MB), 13.8 / 12.7; 64 of 128, 32 heads (109 MB), 20.4 / 15.6; 8 of 2,048, 32 heads (139 MB), 12.7 / 11.4; 64 of 512, 32 heads (310 MB), 34 / 17.  Heads of 128 (2 of them, 8 queries
 // each): 16 of 8,000 (132 MB) 14.8 / 19.5, 64 of 2,048 (139 MB) 13.6 / 21.8, 32 of 8,000 (265 MB) 23.5 / 23.3, 64 of 8,000 (530 MB) 40 / 35.
+// attention_decode, which reads every member's table too but in runs of 256 keys that meet through memory, has 4 key-value heads of four queries each, in tables of 4,096, so (this way / it):
+// heads of 64, 4 members of 500 common positions 4.7 / 4.1 us, of 2,000 5.5 / 4.6, 8 of 2,000 6.3 / 5.3, 16 of 500 5.2 / 4.8, of 2,000 7.1 / 10.2; heads of 128, 4 of 500 5.3 / 5.0, of 2,000 7.0 / 5.9,
+// 8 of 2,000 7.5 / 11.7, 16 of 500 6.0 / 11.0, of 2,000 9.6 / 22.9.  ops.attention chooses between the two by whole steps (attention_shared_pays).
 bool attention_each_mma_takes(const SaArgs& a) {
     return (long long)a.n * a.max_blocks * a.page_size * a.nkv * a.hd * 4 <= (a.hd == 64 ? 96ll << 20 : 240ll << 20);
 }

@@ -198,7 +198,7 @@ class ContextBuilder:
         for g, group in enumerate(self.cache.groups):
             saved = sum((len(f) - 1) * shared[g] for f, shared in out)
             read = any(ops.attention_shared_serves(self.dtype, *heads, len(requests), self.max_blocks * ps) for heads in self._common_heads[g])
-            if ops.attention_shared_pays(saved, group.num_kv_heads, group.head_dim, self.dtype, read):
+            if ops.attention_shared_pays(saved, group.num_kv_heads, group.head_dim, self.dtype, read, self.max_model_len):
                 return out
         return None
 

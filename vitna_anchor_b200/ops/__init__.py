@@ -2300,14 +2300,29 @@ def set_attention_shared(mode: int) -> int:
     return before
 
 
-def attention_shared_pays(saved: int, nkv: int, hd: int, dtype: torch.dtype = torch.bfloat16, read: bool = True) -> bool:
-    """Whether a decode step whose requests would read `saved` cached positions again and again goes through attention_shared rather than attention_decode: from 64 MB of
-    them on, where an attention would read them once (`read`).  Whole steps of a beam search, this way against the other: 8 beams of 2,000 positions, 32 heads of 64 over 24 layers (115 MB), 1.70 ms against 1.84, 64 of 8,000
-    (4.1 GB) 4.5 / 16.0; 16 of 4,000, 5 heads, 32 layers (77 MB) 1.68 / 1.72; 4 of 2,000, 32 heads (49 MB) 1.61 / 1.49, 16 of 500 (61 MB) 1.77 / 1.71; 32 of 500, 3 heads, 30 layers
-    (12 MB) 1.38 / 1.20.  Below, at 3 and 5 heads and 4,000 positions and more, up to 0.2 ms of 1.4 are left."""
+def attention_shared_pays(saved: int, nkv: int, hd: int, dtype: torch.dtype = torch.bfloat16, read: bool = True, context: int = 0) -> bool:
+    """Whether a decode step whose requests would read `saved` cached positions again and again goes through attention_shared, where an attention would read them once (`read`),
+    rather than through what it takes otherwise, which `context`, the most positions that a request may reach, decides.
+
+    Against attention_decode, from 64 MB of them on.  Whole steps of a beam search, this way against the other.  Heads of 64: 8 beams of 2,000 positions, 32 heads over 24 layers (115 MB),
+    1.70 ms against 1.84, 64 of 8,000 (4.1 GB) 4.5 / 16.0; 16 of 4,000, 5 heads, 32 layers (77 MB) 1.68 / 1.72; 4 of 2,000, 32 heads (49 MB) 1.61 / 1.49, 16 of 500 (61 MB) 1.77 / 1.71; 32 of
+    500, 3 heads, 30 layers (12 MB) 1.38 / 1.20.  Heads of 128: 32 over 8, 16 layers, 16 beams of 2,000 (117 MB) 1.47 / 1.85, 8 of 2,000 (55 MB) 1.32 / 1.35, 4 of 2,000 (23 MB) 1.23 / 1.10.
+    float32: 32 beams of 2,000, 3 heads of 64 (91 MB), 5.15 / 5.78, 8 of 2,000 (21 MB) 2.40 / 2.35.  Other sizes up to 128, which both have on float32 units: 4 to 16 members from 70 MB on
+    1.3 to 4.2 times as fast a layer.
+    Not at all in bfloat16 with heads of 16, 32 and 96, which attention_decode has on the tensor cores and attention_shared on float32 units (8 beams of 2,000, 32 heads of 96, 164 MB, 2.33 ms a
+    step against 1.70; a layer of 64 members behind 8,000, four queries a key-value head of 4, heads of 96 208 us / 177, of 32 91 / 79; with many members and a query a head it would be the
+    faster one, 16 of 4,000 with 32 heads of 32 1.62 ms / 2.09), nor with heads above 128 (4 members of 4,000, 32 heads of 256: 463 us / 309).
+
+    Against attention_rows, which contexts of more than 32,768 positions take, from 4 MB on: 4 beams of 500, 5 heads of 64, 32 layers (2 MB) 1.16 ms a step / 2.73, 4 of 8,000, 32 heads of
+    32 (94 MB) 1.40 / 11.5; a layer of 2 members of 100, 32 heads of 256 (3 MB), 55 us / 36, of 500 (15 MB) 96 / 166."""
     if _shared_mode != 2:
         return _shared_mode == 1 and saved > 0
-    return read and saved * nkv * hd * 2 * dtype.itemsize >= 64 << 20
+    least = 64 << 20
+    if not attention_decode_takes(dtype, hd, context):
+        least = 4 << 20
+    elif hd > 128 or (dtype == torch.bfloat16 and hd in (16, 32, 96)):
+        return False
+    return read and saved * nkv * hd * 2 * dtype.itemsize >= least
 
 
 def attention_shared_scratch_bytes(tokens: int, nh: int, nkv: int, hd: int) -> int:
