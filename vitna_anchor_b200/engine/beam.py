@@ -130,7 +130,7 @@ def beam_search(runner: ModelRunner, selector: BeamSelector, ids: Sequence[int],
             requests, pairs, left = plan_moves([row for row, _, _ in chosen], [b.request_id for b in live])
             for rid in left:
                 runner.close(rid)
-            runner.cache.adopt(pairs)
+            runner.adopt(pairs)
             for i, (row, _, _) in enumerate(chosen):
                 if requests[i] is None:                  # more beams than requests: only while the search widens
                     requests[i] = new_request()

@@ -124,8 +124,21 @@ class ModelRunner:
         self.cache.close(request_id)
 
     def fork(self, source_id: Hashable, request_id: Hashable) -> int:
-        """Open a request that goes on from where another stands (CacheManager.fork)."""
+        """Open a request that goes on from where another stands (CacheManager.fork).  Steps that are not known to have worked are waited for and
+        checked first, as check() does: what they wrote may have to be undone, and of what goes on from there nobody would know."""
+        self._settle()
         return self.cache.fork(source_id, request_id)
+
+    def adopt(self, pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
+        """For every (request, source): the request forgets what it has and goes on from where the source stands (CacheManager.adopt); checked as fork()."""
+        self._settle()
+        self.cache.adopt(pairs)
+
+    def _settle(self) -> None:
+        if self._issued:
+            self.check(sync=False)
+        if self._issued:
+            self.check(sync=True)
 
     def length(self, request_id: Hashable) -> int:
         return self.cache.length(request_id)
