@@ -264,3 +264,64 @@ def test_command_line_of_a_search():
     for argv in [["generate", "--model", "x", "--ids", "1", "--length-penalty", "1"], ["generate", "--model", "x", "--ids", "1", "--beams", "2", "--temperature", "0.5"],
                  ["generate", "--model", "x", "--ids", "1", "--beams", "2", "--logits-out", "f"], ["generate", "--model", "x", "--ids", "1", "--beams", "two"]]:
         assert main(argv) == 1
+
+
+def test_many_forks_are_one_move(monkeypatch):
+    """Every (request, source), the copies of all together: one launch for each group of pages and each shape of states; nothing is changed where one cannot be."""
+    specs = [KVSpec(1, 8), KVSpec(2, 8), StateSpec((3,))]
+    c = CacheManager(specs, page_size=4, num_pages=[7, 9], max_requests=6, dtype=torch.float32, device="cpu")
+    for rid, n in [("a", 6), ("b", 4)]:
+        c.open(rid)
+        c.reserve_step([(rid, n)])
+        c.commit_step([(rid, n)])
+    moves = []
+    monkeypatch.setattr(ops, "copy_rows", lambda arena, src, dst: moves.append((tuple(arena.shape[:2]), list(src), list(dst))))
+
+    def refused(pairs, error=CacheError):
+        before = c.free_pages(), {r: [list(t.blocks) for t in rc.tables.values()] for r, rc in c.tables.requests.items()}, c.tables.slots.free_slots
+        with pytest.raises(error):
+            c.fork_many(pairs)
+        assert before == (c.free_pages(), {r: [list(t.blocks) for t in rc.tables.values()] for r, rc in c.tables.requests.items()}, c.tables.slots.free_slots) and not moves
+        c.check()
+
+    refused([("c", "a"), ("c", "b")])
+    refused([("c", "a"), ("a", "b")])
+    refused([("c", "a"), ("d", "c")])                        # a source that is not open yet
+    refused([("c", "a"), ("d", "q")])
+    refused([(i, "b") for i in range(5)])                    # four slots
+    refused([(i, "a") for i in range(5)], OutOfPages)        # and four pages of the smaller group
+    c.fork_many([])
+    assert not moves
+    c.fork_many([("c", "a"), ("d", "b"), ("e", "a")])
+    slot, page = c.slot, lambda r, g: c.tables.get(r).tables[g].blocks[1]      # noqa: E731
+    assert moves == [((1, 7), [page("a", 0)] * 2, [page("c", 0), page("e", 0)]), ((1, 9), [page("a", 1)] * 2, [page("c", 1), page("e", 1)]),
+                     ((1, 6), [slot("a"), slot("b"), slot("a")], [slot("c"), slot("d"), slot("e")])]
+    assert [c.length(r) for r in "cde"] == [6, 4, 6]
+    c.check()
+
+
+def test_pages_of_many_holders_cost_no_more_than_those_of_few():
+    """Comparisons of holders' names while a request of 400 pages gets as many holders: as many as there are holders and pages, not their squares."""
+    class Name:
+        seen = 0
+
+        def __init__(self, i):
+            self.i = i
+
+        def __hash__(self):
+            return hash(self.i)
+
+        def __eq__(self, other):
+            Name.seen += 1
+            return isinstance(other, Name) and self.i == other.i
+
+    t = PageTables([PageGroup((0,), 1, 8, 0)], 4, [500], 41)
+    names = [Name(i) for i in range(41)]
+    t.open(names[0])
+    t.reserve(names[0], 1600)
+    t.commit(names[0])
+    Name.seen = 0
+    t.fork_many([(n, names[0]) for n in names[1:]])
+    for n in names:
+        t.close(n)
+    assert Name.seen <= 4 * 41 * 400 and t.pools[0].free_pages == 500

@@ -15,7 +15,8 @@ KVSpec form a group that shares page ids and has a pool of its own:
 A request holds one slot from open() to close(); its state rows are zeroed
 when the slot is taken.  fork() and adopt() let requests go on from where others
 stand: full pages are held in common, the page in the middle and the state rows are
-copied, one launch for each group of pages and each shape of states.
+copied, one launch for each group of pages and each shape of states.  (They read what is
+there: ModelRunner's forms see to it that the steps which wrote it have worked.)
 """
 from __future__ import annotations
 
@@ -138,9 +139,13 @@ class CacheManager:
 
     def fork(self, source_id: Hashable, request_id: Hashable) -> int:
         """Open request_id as one that goes on from where source_id stands (its keys, values and states); returns its slot."""
-        copies = self.tables.fork(source_id, request_id)
-        self._copy(copies, [(request_id, source_id)])
+        self.fork_many([(request_id, source_id)])
         return self.tables.get(request_id).slot
+
+    def fork_many(self, pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
+        """fork() for every (request, source), all of them or nothing; the moves of all in one launch for each group of pages and each shape of states."""
+        if pairs:
+            self._copy(self.tables.fork_many(list(pairs)), pairs)
 
     def adopt(self, pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
         """For every (request, source): the request forgets what it has and goes on from where the source stands.  No request is named

@@ -35,8 +35,7 @@ class OutOfPages(CacheError):
 
 
 class PagePool:
-    """`num_pages` page ids with an owner tag each, and further holders where a page is shared.  alloc/free are O(1) (free of a
-    shared page: in its holders)."""
+    """`num_pages` page ids with an owner tag each, and further holders where a page is shared.  alloc, share and free are O(1)."""
 
     def __init__(self, num_pages: int):
         if num_pages < 1:
@@ -44,7 +43,7 @@ class PagePool:
         self.num_pages = num_pages
         self._free: List[int] = list(range(num_pages - 1, -1, -1))  # pop() gives 0 first
         self._owner: List[Optional[Hashable]] = [None] * num_pages
-        self._more: Dict[int, List[Hashable]] = {}                  # shared pages: who holds them besides the owner
+        self._more: Dict[int, Dict[Hashable, None]] = {}            # shared pages: who holds them besides the owner
 
     @property
     def free_pages(self) -> int:
@@ -68,9 +67,9 @@ class PagePool:
         if self._owner[page] != owner:
             if more is None or owner not in more:
                 raise CacheError(f"page {page} belongs to {self._owner[page]!r}, not to {owner!r}")
-            more.remove(owner)
+            del more[owner]
         elif more is not None:
-            self._owner[page] = more.pop(0)
+            self._owner[page] = more.popitem()[0]
         else:
             self._owner[page] = None
             self._free.append(page)
@@ -84,9 +83,10 @@ class PagePool:
             raise CacheError("a page needs an owner")
         if not (0 <= page < self.num_pages) or self._owner[page] is None:
             raise CacheError(f"page {page} is held by nobody")
-        if owner in self.holders(page):
+        more = self._more.setdefault(page, {})
+        if owner == self._owner[page] or owner in more:
             raise CacheError(f"page {page} is held by {owner!r} already")
-        self._more.setdefault(page, []).append(owner)
+        more[owner] = None
 
     def holders(self, page: int) -> List[Hashable]:
         """Who holds the page (nobody: it is free)."""
@@ -230,13 +230,30 @@ class PageTables:
     def fork(self, source_id: Hashable, request_id: Hashable) -> List[tuple]:
         """Open request_id as a request that goes on from where source_id stands.  Returns (group, from page, to page) for the
         pages whose content has to be copied.  Pages and a slot are there, or nothing is changed."""
-        source = self.get(source_id)
-        if source.reserved:
+        return self.fork_many([(request_id, source_id)])
+
+    def fork_many(self, pairs: Sequence[tuple]) -> List[tuple]:
+        """fork() for every (request, source): all of them, or nothing is changed."""
+        requests = [r for r, _ in pairs]
+        if len(set(requests)) != len(requests):
+            raise CacheError("a request is opened twice")
+        for request_id in requests:
+            if request_id in self.requests:
+                raise CacheError(f"request {request_id!r} is already open")
+        sources = [self.get(s) for _, s in pairs]
+        if any(source.reserved for source in sources):
             raise CacheError("fork during a step")
-        for g in self._tail_copies(source):
-            if self.pools[g].free_pages < 1:
-                raise OutOfPages(f"group {g} has no page for the end of request {request_id!r}")
-        return self._continue(self.open(request_id), source, [0] * len(self.groups))
+        tails = [self._tail_copies(source) for source in sources]
+        for g, pool in enumerate(self.pools):
+            need = sum(1 for t in tails if g in t)
+            if need > pool.free_pages:
+                raise OutOfPages(f"group {g} needs {need} pages for the ends of requests {requests!r} and has {pool.free_pages}")
+        if len(requests) > self.slots.free_slots:
+            raise CacheError("no free request slot")
+        copies = []
+        for request_id, source in zip(requests, sources):
+            copies += self._continue(self.open(request_id), source, [0] * len(self.groups))
+        return copies
 
     def adopt(self, pairs: List[tuple]) -> List[tuple]:
         """For every (request, source): the request forgets what it holds and goes on from where the source stands.  No request is named

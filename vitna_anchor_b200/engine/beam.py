@@ -131,10 +131,12 @@ def beam_search(runner: ModelRunner, selector: BeamSelector, ids: Sequence[int],
             for rid in left:
                 runner.close(rid)
             runner.adopt(pairs)
+            wider = []
             for i, (row, _, _) in enumerate(chosen):
                 if requests[i] is None:                  # more beams than requests: only while the search widens
                     requests[i] = new_request()
-                    runner.fork(live[row].request_id, requests[i])
+                    wider.append((requests[i], live[row].request_id))
+            runner.fork_many(wider)
             live = [_Beam(rid, live[row].ids + [token], lp) for rid, (row, token, lp) in zip(requests, chosen)]
             logits = runner.step([StepEntry(b.request_id, [b.ids[-1]], [0]) for b in live])
         finished.sort(key=lambda r: -r.score)

@@ -129,6 +129,11 @@ class ModelRunner:
         self._settle()
         return self.cache.fork(source_id, request_id)
 
+    def fork_many(self, pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
+        """fork() for every (request, source), the moves of all together (CacheManager.fork_many)."""
+        self._settle()
+        self.cache.fork_many(pairs)
+
     def adopt(self, pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
         """For every (request, source): the request forgets what it has and goes on from where the source stands (CacheManager.adopt); checked as fork()."""
         self._settle()
