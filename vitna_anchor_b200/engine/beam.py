@@ -2,9 +2,10 @@
 
 A search keeps the `beams` most likely continuations of one prompt.  Its beams are requests of one family: the prompt runs once, the others
 are forked from it and hold its pages in common, so that a step's attention reads the prompt once for all of them.  Every step the model
-gives the live beams' logits, the 2 x beams best (beam, token) pairs are chosen on the device, and the host takes from them, in order: a token
-that ends the text finishes a result if it is among the first `beams`, every other one is a live beam until there are `beams` of them.  A beam that
-several go on from keeps its request; the others of them take over requests that nothing goes on from.
+gives the live beams' logits, and the host takes the (beam, token) pairs in order, best first: a token that ends the text finishes a result if
+it is among the first `beams`, every other one is a live beam until there are `beams` of them.  The 2 x beams best are chosen on the device.  With
+one token that ends the text they are always enough; where several do, and fewer than `beams` of them go on, the host orders all there are.  A beam
+that several go on from keeps its request; the others of them take over requests that nothing goes on from.
 
 A result's score is its sum of log probabilities divided by length ** length_penalty (length: its new tokens, the stop token counted).
 The search ends when max_new tokens are reached, when no beam lives, or when `beams` results are finished and no live beam can reach the worst of
@@ -17,6 +18,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 from typing import Hashable, Iterable, List, Optional, Sequence, Set
 
+import numpy as np
 import torch
 
 from .. import ops
@@ -43,7 +45,7 @@ class BeamSelector:
 
     def __init__(self, vocab: int, beams: int, device):
         self.vocab, self.beams = vocab, beams
-        self.keep = min(2 * beams, vocab)            # of one row there may be fewer tokens than are kept
+        self.keep = min(2 * beams, beams * vocab)
         self._scratch = torch.zeros(ops.beam_select_scratch_bytes(beams, vocab, self.keep), dtype=torch.uint8, device=device)
         self._out = torch.empty((3, self.keep), dtype=torch.int32, device=device)
         self._scores = torch.empty(beams, dtype=torch.float32, device=device)
@@ -53,13 +55,28 @@ class BeamSelector:
     def choose(self, logits: torch.Tensor, log_probs: Sequence[float]) -> List[tuple]:
         """(log probability, row, token) of the best continuations, in descending order; waits for them."""
         n = len(log_probs)
+        keep = min(self.keep, n * self.vocab)        # of one row there may be fewer tokens than are kept
         self._scores_host[:n] = torch.tensor(list(log_probs), dtype=torch.float32)
         self._scores[:n].copy_(self._scores_host[:n], non_blocking=True)
-        out = (self._out[0:1].view(torch.float32), self._out[1:2], self._out[2:3])
-        ops.beam_select(logits, self._scores[:n], n, self.keep, out, self._scratch)
+        out = (self._out[0:1, :keep].view(torch.float32), self._out[1:2, :keep], self._out[2:3, :keep])
+        ops.beam_select(logits, self._scores[:n], n, keep, out, self._scratch)
         self._out_host.copy_(self._out, non_blocking=True)
         torch.cuda.current_stream().synchronize()
-        return list(zip(self._out_host[0].view(torch.float32).tolist(), self._out_host[1].tolist(), self._out_host[2].tolist()))
+        return list(zip(self._out_host[0, :keep].view(torch.float32).tolist(), self._out_host[1, :keep].tolist(), self._out_host[2, :keep].tolist()))
+
+
+def all_in_order(logits: torch.Tensor, log_probs: Sequence[float], count: int) -> List[tuple]:
+    """What BeamSelector.choose gives, for any count of continuations, on the host in 64 bits."""
+    x = logits[:len(log_probs)].cpu().numpy().astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        c = np.asarray(log_probs, dtype=np.float64)[:, None] + x - np.logaddexp.reduce(x, axis=1, keepdims=True)
+    c[~np.isfinite(c).any(axis=1) | np.isnan(c).any(axis=1) | (c == np.inf).any(axis=1)] = -np.inf
+    c = c.reshape(-1)
+    count = min(count, c.size)
+    least = np.partition(c, c.size - count)[c.size - count]
+    at = np.flatnonzero(c >= least)
+    at = at[np.argsort(-c[at], kind="stable")][:count]
+    return [(float(np.float32(v)), int(i) // x.shape[1], int(i) % x.shape[1]) for v, i in zip(c[at], at)]
 
 
 def normalised(log_prob: float, length: int, length_penalty: float) -> float:
@@ -69,6 +86,19 @@ def normalised(log_prob: float, length: int, length_penalty: float) -> float:
 def attainable(log_prob: float, length: int, max_new: int, length_penalty: float) -> float:
     """The best score that a live beam of this sum and length can still end with: its sum stays, at the length that divides it most kindly."""
     return max(normalised(log_prob, length, length_penalty), normalised(log_prob, max_new, length_penalty))
+
+
+def take(best: Sequence[tuple], beams: int, stop: Set[int]) -> tuple:
+    """Of continuations (log probability, row, token), best first: the (row, token, log probability) that end among the first `beams`, and the first `beams` that go on."""
+    ended, chosen = [], []
+    for rank, (log_prob, row, token) in enumerate(best):
+        if log_prob == float("-inf") or len(chosen) == beams:
+            break
+        if token not in stop:
+            chosen.append((row, token, log_prob))
+        elif rank < beams:
+            ended.append((row, token, log_prob))
+    return ended, chosen
 
 
 def plan_moves(parents: Sequence[int], live: Sequence[Hashable]) -> tuple:
@@ -92,7 +122,7 @@ def plan_moves(parents: Sequence[int], live: Sequence[Hashable]) -> tuple:
 
 def beam_search(runner: ModelRunner, selector: BeamSelector, ids: Sequence[int], *, beams: int, max_new: int, length_penalty: float,
                 stop_ids: Iterable[int], name: Hashable) -> List[BeamResult]:
-    stop = set(stop_ids)
+    stop = {t for t in stop_ids if 0 <= t < selector.vocab}
     opened: List[Hashable] = []
 
     def new_request() -> Hashable:
@@ -111,15 +141,12 @@ def beam_search(runner: ModelRunner, selector: BeamSelector, ids: Sequence[int],
         for length in range(1, max_new + 1):
             best = selector.choose(logits, [b.log_prob for b in live])
             runner.check(sync=False)                     # the choice has arrived, so every kernel of the step is done
-            chosen = []
-            for rank, (log_prob, row, token) in enumerate(best):
-                if log_prob == float("-inf") or len(chosen) == beams:
-                    break
-                if token in stop:
-                    if rank < beams:
-                        finished.append(BeamResult(live[row].ids + [token], normalised(log_prob, length, length_penalty), log_prob, "stop"))
-                else:
-                    chosen.append((row, token, log_prob))
+            ended, chosen = take(best, beams, stop)
+            there = len(live) * selector.vocab
+            if len(chosen) < beams and len(best) < there and best[-1][0] != float("-inf"):
+                best = all_in_order(logits, [b.log_prob for b in live], beams + len(live) * len(stop))
+                ended, chosen = take(best, beams, stop)
+            finished += [BeamResult(live[row].ids + [token], normalised(log_prob, length, length_penalty), log_prob, "stop") for row, token, log_prob in ended]
             finished.sort(key=lambda r: -r.score)        # stable: among equals what was finished first
             del finished[beams:]
             if length == max_new:
