@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from vitna_anchor_b200.engine import beam
-from vitna_anchor_b200.engine.beam import BeamResult, beam_search
+from vitna_anchor_b200.engine.beam import beam_search
 
 
 class Runner:
@@ -63,8 +63,9 @@ class Selector:
 
     def choose(self, logits, log_probs):
         x = logits.numpy().astype(np.float64)
-        c = (np.asarray(log_probs)[:, None] + x - np.logaddexp.reduce(x, axis=1, keepdims=True))
-        c[~np.isfinite(np.logaddexp.reduce(x, axis=1))] = -np.inf
+        with np.errstate(invalid="ignore"):
+            lse = np.logaddexp.reduce(x, axis=1, keepdims=True)
+            c = np.where(np.isfinite(lse), np.asarray(log_probs)[:, None] + x - lse, -np.inf)
         c = c.reshape(-1)
         at = np.argsort(-c, kind="stable")[:min(self.keep, c.size)]
         return [(float(np.float32(c[i])), int(i) // self.vocab, int(i) % self.vocab) for i in at]
@@ -140,3 +141,25 @@ def test_all_in_order():
     assert len(got) == 24 and beam.all_in_order(x, [0.0, 0.0, 0.0, 0.0, 0.0, -inf], 3) == got[:3]
     e = np.exp(1.0)
     assert abs(got[0][0] - np.log(e / (1 + 2 * e))) <= 2.0 ** -24 and abs(got[2][0] - np.log(e / (2 + 2 * e))) <= 2.0 ** -23
+
+
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("behind", [3, 5])
+def test_logits_that_are_no_numbers_end_the_search_with_an_error(behind, what):
+    """From the prompt's step on, or from a later one: no empty list, and nothing is left open."""
+    from vitna_anchor_b200.engine.runner import StepFailed
+    r = Runner(50, spoil=(behind, 50, what))
+    with pytest.raises(StepFailed, match="no numbers"):
+        search(r, [3, 1, 4], 3, 6)
+    assert not r.requests
+    r = Runner(50, spoil=(behind, 49, float("-inf")))         # one token is left: as many beams as there are rows
+    assert [g.ids[-1] for g in search(r, [3, 1, 4], 3, 6)] == [49] * (1 if behind == 3 else 3)
+
+
+def test_beams_whose_logits_are_no_numbers_die():
+    r = Runner(50)
+    of = r.logits_of
+    r.logits_of = lambda ids: np.full(50, np.nan, dtype=np.float32) if ids[3:4] == [top] else of(ids)
+    top = int(np.argmax(of([3, 1, 4])))
+    got = search(r, [3, 1, 4], 4, 5)
+    assert len(got) == 4 and all(g.ids[0] != top for g in got)

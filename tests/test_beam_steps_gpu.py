@@ -87,3 +87,16 @@ def test_common_pages_are_read_once_without_graphs(hd, context, dirs, calls):
     b = _play(model, context, members, prompt, 0, graphs=False)
     assert "attention_shared" not in calls
     assert float((a - b).abs().max()) <= 3e-2 * float(b.abs().max())
+
+
+def test_logits_that_are_no_numbers_end_a_search_with_an_error(dirs):
+    """A final norm's weight that is no number: Engine.beam_search raises and frees everything."""
+    from vitna_anchor_b200.engine.engine import Engine
+    from vitna_anchor_b200.engine.runner import StepFailed
+    eng = Engine(dirs[64], dtype="float32", parallel=4, ctx=128)
+    assert len(eng.beam_search([1, 2, 3], beams=3, max_new=4)) == 3
+    eng.model.final_norm.tensors()[0].fill_(float("nan"))
+    free = eng.runner.cache.free_pages()
+    with pytest.raises(StepFailed, match="no numbers"):
+        eng.beam_search([1, 2, 3], beams=3, max_new=4)
+    assert eng.runner.cache.free_pages() == free and not eng.runner.cache.tables.requests

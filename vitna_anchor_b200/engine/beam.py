@@ -9,7 +9,7 @@ that several go on from keeps its request; the others of them take over requests
 
 A result's score is its sum of log probabilities divided by length ** length_penalty (length: its new tokens, the stop token counted).
 The search ends when max_new tokens are reached, when no beam lives, or when `beams` results are finished and no live beam can reach the worst of
-them any more (log probabilities only add up downwards).
+them any more (log probabilities only add up downwards).  Beams whose logits are no numbers die; where that is all of them the search fails (StepFailed).
 
 The reference has no beam search; its choice of a token (engine/src/sampler.c:31-38) is what one beam does.
 """
@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from .. import ops
-from .runner import ModelRunner, StepEntry
+from .runner import ModelRunner, StepEntry, StepFailed
 
 
 @dataclass
@@ -141,6 +141,8 @@ def beam_search(runner: ModelRunner, selector: BeamSelector, ids: Sequence[int],
         for length in range(1, max_new + 1):
             best = selector.choose(logits, [b.log_prob for b in live])
             runner.check(sync=False)                     # the choice has arrived, so every kernel of the step is done
+            if best[0][0] == float("-inf"):              # (of a row that has a softmax the largest value is offered, at a finite sum)
+                raise StepFailed(f"the logits behind {len(live)} beam(s) of {len(live[0].ids)} new tokens are no numbers that a token can be chosen by (a NaN, an infinity, nothing above -inf)")
             ended, chosen = take(best, beams, stop)
             there = len(live) * selector.vocab
             if len(chosen) < beams and len(best) < there and best[-1][0] != float("-inf"):
