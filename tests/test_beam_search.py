@@ -163,3 +163,25 @@ def test_beams_whose_logits_are_no_numbers_die():
     top = int(np.argmax(of([3, 1, 4])))
     got = search(r, [3, 1, 4], 4, 5)
     assert len(got) == 4 and all(g.ids[0] != top for g in got)
+
+
+def test_penalties_whose_powers_no_float_holds():
+    """Lengths to a power beyond a float's range were an OverflowError, or a division by zero, in the middle of a search."""
+    for penalty in (400.0, -400.0, 1e300, -1e300, float("inf"), float("nan")):
+        assert not beam.penalty_fits(penalty, 10)
+    for penalty, max_new in [(1.0, 131072), (-1.0, 131072), (50.0, 131072), (-50.0, 131072), (1e6, 1), (0.0, 1 << 30), (600.0, 2)]:
+        assert beam.penalty_fits(penalty, max_new)
+        for length in (1, max_new):
+            for log_prob in (-1e9, -1e-7, 0.0):
+                assert np.isfinite(beam.normalised(log_prob, length, penalty)) and np.isfinite(beam.attainable(log_prob, length, max_new, penalty))
+
+
+def test_the_engine_refuses_such_a_penalty():
+    from types import SimpleNamespace
+    from vitna_anchor_b200.engine.engine import Engine, RequestRefused
+    eng = Engine.__new__(Engine)
+    eng.model, eng.ctx = SimpleNamespace(vocab_size=50), 64
+    eng.runner = SimpleNamespace(cache=SimpleNamespace(max_requests=4))
+    for penalty in (400.0, -400.0, float("nan"), float("-inf")):
+        with pytest.raises(RequestRefused, match="length_penalty"):
+            eng.beam_search([1], beams=2, max_new=20, length_penalty=penalty)

@@ -15,6 +15,7 @@ The reference has no beam search; its choice of a token (engine/src/sampler.c:31
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Hashable, Iterable, List, Optional, Sequence, Set
 
@@ -81,6 +82,11 @@ def all_in_order(logits: torch.Tensor, log_probs: Sequence[float], count: int) -
 
 def normalised(log_prob: float, length: int, length_penalty: float) -> float:
     return log_prob / float(length) ** length_penalty
+
+
+def penalty_fits(length_penalty: float, max_new: int) -> bool:
+    """Whether every length's power, and a sum of log probabilities divided by it, is a number that a float holds (a sum is below 2^30: tokens times the largest difference of logits that count)."""
+    return math.isfinite(length_penalty) and abs(length_penalty) * math.log(max_new) <= 600.0
 
 
 def attainable(log_prob: float, length: int, max_new: int, length_penalty: float) -> float:

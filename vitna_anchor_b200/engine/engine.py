@@ -11,7 +11,6 @@ engine/src/api.c:48-49, 2216-2224).
 """
 from __future__ import annotations
 
-import math
 import time
 from typing import Dict, Hashable, Iterable, List, Optional, Sequence, Union
 
@@ -21,7 +20,7 @@ import torch
 from .. import ops
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler
-from .beam import BeamResult, BeamSelector, beam_search
+from .beam import BeamResult, BeamSelector, beam_search, penalty_fits
 from .loading import load_model
 from .runner import DeviceStepFailed, ModelRunner, StepEntry, StepFailed
 from .scheduler import PENDING, Planned, Request, RequestRefused, Scheduler  # noqa: F401
@@ -256,8 +255,8 @@ class Engine:
             raise RequestRefused(f"the prompt ({len(ids)} tokens) and max_new ({max_new}) do not fit the context of {self.ctx} positions")
         if self.model.vocab_size > ops.BEAM_MAX_VOCAB:
             raise RequestRefused(f"a vocabulary of {self.model.vocab_size} is more than the {ops.BEAM_MAX_VOCAB} that the choice takes")
-        if not math.isfinite(length_penalty):
-            raise RequestRefused("length_penalty is a number")
+        if not penalty_fits(length_penalty, max_new):
+            raise RequestRefused(f"length_penalty {length_penalty} is not a number whose power of {max_new} tokens can be told from 0 and infinity")
         if self.scheduler.has_work() or self._inflight is not None:
             raise RequestRefused("requests are running; a beam search has the engine to itself")
         selector = self._selectors.get(beams)
