@@ -100,3 +100,40 @@ def test_logits_that_are_no_numbers_end_a_search_with_an_error(dirs):
     with pytest.raises(StepFailed, match="no numbers"):
         eng.beam_search([1, 2, 3], beams=3, max_new=4)
     assert eng.runner.cache.free_pages() == free and not eng.runner.cache.tables.requests
+
+
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
+def test_lists_written_by_the_kernel_just_before(dtype, hd, wide):
+    """Positions, or the members, that a kernel of the library writes right before the call: what it wrote is what is read, launched one by one and replayed."""
+    from test_beam_ops_gpu import Batch
+    from vitna_anchor_b200 import ops
+    b = Batch([(500, [20, 3, 41, 9]), (64, [7, 30])], 8, 2, hd, 16, dtype, seed=3).device(wide)
+    want, tol = b.want()
+    d, n = b.d, len(b.pos)
+    scratch = torch.zeros(ops.attention_shared_scratch_bytes(n, 8, 2, hd), dtype=torch.uint8, device="cuda")
+    for name in ("pos", "members"):
+        right = d[name].clone()
+        slow = torch.zeros((n, 1 << 18), device="cuda")              # a search for the largest of many: it lets the kernel after it begin at once, and writes at its end
+        slow[torch.arange(n, device="cuda"), right.long()] = 1.0
+
+        def call():
+            d[name].zero_()
+            d["out"].fill_(7.0)
+            ops.argmax_rows(slow, d[name])
+            return b.run(ops, scratch)
+        outs = [call().clone() for _ in range(10)]
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            call()
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                call()
+            for _ in range(10):
+                graph.replay()
+                outs.append(d["out"].clone())
+        torch.cuda.synchronize()
+        assert torch.equal(d[name], right)
+        for out in outs:
+            assert float(((out.double().cpu() - want).abs() - tol).max()) <= 0

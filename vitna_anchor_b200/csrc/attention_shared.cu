@@ -238,8 +238,7 @@ __global__ void __launch_bounds__(SA_THREADS, DIMS == 2 ? 2 : 1) attention_share
     w.v = nullptr;
     w.warps = 1;
     w.place = w.barrier = 0;
-    sa_make_plan(a, p);                       // from the step's metadata, which no kernel writes
-    dependency_wait();
+    sa_make_plan(a, p);                       // and the wait for the kernel before this one
     let_dependents_start();
     SaPart r;
     const bool prefix = (int)blockIdx.x < p.prefix_blocks;
@@ -312,11 +311,7 @@ __global__ void __launch_bounds__(SE_WARPS * 32) attention_each_kernel(const SaA
     const int warp = threadIdx.x >> 5, vec = a.hd / N;
     SaPart part;
     int token;
-    if (!sa_each_part(a, SG_ROWS, part, token)) {
-        dependency_wait();                                  // (the kernel after this one may take it that the one before has finished)
-        return;
-    }
-    dependency_wait();
+    if (!sa_each_part(a, SG_ROWS, part, token)) return;     // the wait for the kernel before this one is in there
     let_dependents_start();
     const T* q = static_cast<const T*>(a.q) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * a.hd;
     for (int c = threadIdx.x; c < SG_ROWS * vec; c += SE_WARPS * 32) {

@@ -705,8 +705,7 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
     SaPlan& p = *reinterpret_cast<SaPlan*>(smem);
     unsigned char* stages = smem + SmSmem<HD>::PLAN;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    sa_make_plan(a, p);                       // from the step's metadata, which no kernel writes
-    dependency_wait();
+    sa_make_plan(a, p);                       // and the wait for the kernel before this one
     const bool prefix = (int)blockIdx.x < p.prefix_blocks;
     // tensor memory where some prefix has many rows, before the kernel after this one may come and want some
     const bool tensor = TENSOR && prefix && __syncthreads_or(p.shared[threadIdx.x] > 0 && min(p.width[threadIdx.x], p.tile_members) * a.gq >= SM_TENSOR_ROWS);
@@ -805,17 +804,13 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_each_m
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     SaPart part;
     int token;
-    if (!sa_each_part(a, 16, part, token)) {                                              // from the step's metadata, which no kernel writes
-        dependency_wait();                                                                // (the kernel after this one may take it that the one before has finished)
-        return;
-    }
+    if (!sa_each_part(a, 16, part, token)) return;                                        // the wait for the kernel before this one is in there
     const __nv_bfloat16* queries = static_cast<const __nv_bfloat16*>(a.q) + ((size_t)token * a.nh + part.kvh * a.gq + part.h0) * HD;
     auto query_of = [&](int row) -> const __nv_bfloat16* { return row < part.heads ? queries + row * HD : nullptr; };
     float* out = reinterpret_cast<float*>(stages);                                        // the warps' outputs, over the stages: [8][16][LD]
     float2 (*ml)[16] = reinterpret_cast<float2 (*)[16]>(stages + SmSmem<HD>::OUT);
     float* whole = reinterpret_cast<float*>(stages + SmSmem<HD>::OUT + SmSmem<HD>::ML);      // and the block's: [16][HD]
     static_assert(SmSmem<HD>::OUT + SmSmem<HD>::ML + 16 * HD * 4 <= SM_STAGES * SmSmem<HD>::STAGE, "the block's output lies behind the warps'");
-    dependency_wait();
     let_dependents_start();
     if (part.heads <= 8) {
         uint32_t qb[HD / 16][2];

@@ -14,7 +14,9 @@
 // place among its unit's parts is the worker's number minus that of the unit's first worker.  A part leaves an unnormalised output, a
 // maximum and a sum for each of its rows, and a second launch joins a row's parts.
 //
-// Lengths are read from the step's metadata on the device, so that a captured graph follows them.
+// Lengths are read from the step's metadata on the device, so that a captured graph follows them.  They are read, and the parts found, while the kernel before this one may still run (2 us that
+// nobody waits for).  What that kernel writes can be seen only behind the wait for it, so the lists are read again there, past the first-level cache, and the parts are found again if any of
+// them has changed: a trip to the second-level cache and a barrier for every launch, and right whoever writes the lists.
 #pragma once
 
 #include "common.cuh"
@@ -96,18 +98,38 @@ __device__ __forceinline__ int sa_find(const int* base, int n, int at) {
     return lo;
 }
 
+// What a thread has of the lists: of member, family and start threadIdx.x (thread 0 the 257th start too).
+struct SaLists { int token, seg, at, shared, start, last; };
+
+__device__ __forceinline__ bool sa_there(const SaArgs& a, int token) { return token >= 0 && token < a.tokens; }
+__device__ __forceinline__ SaLists sa_read_lists(const SaArgs& a) {
+    const int i = threadIdx.x;
+    SaLists l;
+    l.token = i < a.n ? __ldcg(a.members + i) : -1;
+    l.shared = i < a.families ? __ldcg(a.shared + i) : 0;
+    l.start = i <= a.families ? __ldcg(a.starts + i) : 0;
+    l.last = i == 0 && a.families == SA_MAX_TOKENS ? __ldcg(a.starts + SA_MAX_TOKENS) : 0;
+    l.seg = sa_there(a, l.token) ? __ldcg(a.token_seg + l.token) : -1;
+    l.at = sa_there(a, l.token) ? __ldcg(a.positions + l.token) : -1;
+    return l;
+}
+// Whether the lists are still what they were, for the whole block alike.  All of it is asked for at once: a token that has changed says so by itself.
+__device__ __forceinline__ bool sa_same_lists(const SaArgs& a, const SaLists& l) {
+    const int i = threadIdx.x;
+    const int token = i < a.n ? __ldcg(a.members + i) : -1, shared = i < a.families ? __ldcg(a.shared + i) : 0, start = i <= a.families ? __ldcg(a.starts + i) : 0;
+    const int last = i == 0 && a.families == SA_MAX_TOKENS ? __ldcg(a.starts + SA_MAX_TOKENS) : 0;
+    const int seg = sa_there(a, l.token) ? __ldcg(a.token_seg + l.token) : -1, at = sa_there(a, l.token) ? __ldcg(a.positions + l.token) : -1;
+    return !__syncthreads_or((token != l.token) | (shared != l.shared) | (start != l.start) | (last != l.last) | (seg != l.seg) | (at != l.at));
+}
+
 // Filled by all SA_THREADS threads of a block.  Numbers that cannot be (a member beyond the batch, a negative position, starts
 // that go back) are taken as members that are not there and runs of no length: nothing is read or written for them.
-__device__ __forceinline__ void sa_make_plan(const SaArgs& a, SaPlan& p) {
-    const int i = threadIdx.x, lane = i & 31;
-    const int token = i < a.n ? a.members[i] : -1;
-    const int shared_i = i < a.families ? a.shared[i] : 0, start_i = i <= a.families ? a.starts[i] : 0;
-    const bool there = token >= 0 && token < a.tokens;
-    const int seg = there ? a.token_seg[token] : -1, at = there ? a.positions[token] : -1;
-    p.start[i] = start_i;                   // zeros behind the last, so that groups of four count no more
-    if (i < 4) p.start[SA_MAX_TOKENS + i] = a.families == SA_MAX_TOKENS && i == 0 ? a.starts[SA_MAX_TOKENS] : 0;
-    p.shared[i] = shared_i;
-    p.tok[i] = token;
+__device__ __forceinline__ void sa_find_parts(const SaArgs& a, const SaLists& lists, SaPlan& p) {
+    const int i = threadIdx.x, lane = i & 31, seg = lists.seg, at = lists.at;
+    p.start[i] = lists.start;               // zeros behind the last, so that groups of four count no more
+    if (i < 4) p.start[SA_MAX_TOKENS + i] = lists.last;
+    p.shared[i] = lists.shared;
+    p.tok[i] = lists.token;
     p.count[i] = p.width[i] = 0;
     p.begin[i] = p.first[i] = SA_MAX_TOKENS;
     p.least[i] = 0x7fffffff;
@@ -176,6 +198,19 @@ __device__ __forceinline__ void sa_make_plan(const SaArgs& a, SaPlan& p) {
     p.prow[i] = rp;
     p.orow[i] = tp + ro;          // behind the prefix rows
     __syncthreads();
+}
+
+// The plan, and the wait for the kernel before this one.
+__device__ __forceinline__ void sa_make_plan(const SaArgs& a, SaPlan& p) {
+#pragma unroll 1
+    for (int again = 0; again < 2; again++) {
+        const SaLists lists = sa_read_lists(a);
+        sa_find_parts(a, lists, p);
+        if (again == 0) {
+            dependency_wait();
+            if (sa_same_lists(a, lists)) break;
+        }
+    }
 }
 
 // A part of a unit: what a worker walks before it leaves rows behind.
@@ -283,15 +318,18 @@ __device__ __forceinline__ void sa_cluster_meet() {
 }
 
 // The member, tile of `rows` heads and run of keys of a block of such a launch (grid: blocks of a cluster, tiles of heads of every key-value head, members); false: nothing of it is there, for the
-// whole cluster alike.
+// whole cluster alike.  The lists are read behind the wait for the kernel before this one, which may have written them (before it and once more behind it, as for the plan, is the slower way here, 11.2 us
+// against ten for six requests of five beams; before it alone was 9.6).
 __device__ __forceinline__ bool sa_each_part(const SaArgs& a, int rows, SaPart& part, int& token) {
     const int i = blockIdx.z, tid = threadIdx.x, ranks = gridDim.x;
+    dependency_wait();
     token = a.members[i];
     const bool there = token >= 0 && token < a.tokens;
-    const int seg = there ? a.token_seg[token] : -1, at = there ? a.positions[token] : -1;
+    const int seg = there ? a.token_seg[token] : -1, at = there ? a.positions[token] : -1, first = a.starts[0];
     bool behind = false;
     for (int f = tid; f < a.families; f += blockDim.x) behind |= a.starts[f + 1] > i;
-    if (!__syncthreads_or(behind) || a.starts[0] > i || seg < 0 || seg >= a.segments || at < 0) return false;
+    behind = __syncthreads_or(behind);
+    if (!behind || first > i || seg < 0 || seg >= a.segments || at < 0) return false;
     const int keys = (int)min((long long)at, (long long)a.max_blocks * a.page_size - 1) + 1;
     const int tiles = (a.gq + rows - 1) / rows, run = (sa_tiles(keys) + ranks - 1) / ranks * SA_TILE;
     part.kvh = blockIdx.y / tiles;

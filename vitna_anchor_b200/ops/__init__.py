@@ -2342,8 +2342,7 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
     may have one member or none.  Every token reads the positions 0 .. positions[t] of its own request, as in attention_decode; rows of `out` whose token
     is in no family are left as they were.  Block numbers outside the pool are not followed (their keys and values count as zeros).
     A value that is infinite or no number where it counts makes its dim of the output no number.
-    scratch: a byte buffer of attention_shared_scratch_bytes(members, ...) or more, whatever it holds, for launches of one stream at a time.  The lists and
-    lengths are read while the kernel before this one in the stream may still run: that must not be a kernel of this library which writes them.
+    scratch: a byte buffer of attention_shared_scratch_bytes(members, ...) or more, whatever it holds, for launches of one stream at a time.
     A wait inside the kernel that runs out sets the error word (check_device_errors)."""
     here, dtype, i32 = torch._C._cuda_getDevice(), q.dtype, torch.int32
     pq, pc, po = _fit(q, "q", dtype, 2, here), _fit(cache_layer, "cache_layer", dtype, 5, here), _fit(out, "out", dtype, 2, here)
