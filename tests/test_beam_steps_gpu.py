@@ -105,24 +105,28 @@ def test_logits_that_are_no_numbers_end_a_search_with_an_error(dirs):
 @pytest.mark.parametrize("wide", [True, False])
 @pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
 def test_lists_written_by_the_kernel_just_before(dtype, hd, wide):
-    """Positions, or the members, that a kernel of the library writes right before the call: what it wrote is what is read, launched one by one and replayed."""
+    """Positions, or the members, that a kernel of the library writes right before the call: what it wrote is what is read, launched one by one and replayed.
+    The kernel is a norm of one long row of ones, which leaves its weights as they are (a mean square of 1, no epsilon): the numbers are their bits.  It lets the kernel
+    after it begin at once and takes some hundred microseconds to its end, where the numbers are."""
     from test_beam_ops_gpu import Batch
     from vitna_anchor_b200 import ops
     b = Batch([(500, [20, 3, 41, 9]), (64, [7, 30])], 8, 2, hd, 16, dtype, seed=3).device(wide)
     want, tol = b.want()
-    d, n = b.d, len(b.pos)
+    d, n, long = b.d, len(b.pos), 1 << 20
     scratch = torch.zeros(ops.attention_shared_scratch_bytes(n, 8, 2, hd), dtype=torch.uint8, device="cuda")
+    ones, weights, row = torch.ones(1, long, device="cuda"), torch.zeros(long, device="cuda"), torch.zeros(1, long, device="cuda")
     for name in ("pos", "members"):
-        right = d[name].clone()
-        slow = torch.zeros((n, 1 << 18), device="cuda")              # a search for the largest of many: it lets the kernel after it begin at once, and writes at its end
-        slow[torch.arange(n, device="cuda"), right.long()] = 1.0
+        right, kept = d[name].clone(), d[name]
+        weights.view(torch.int32)[-n:] = right
+        d[name] = row.view(torch.int32)[0, -n:]
 
         def call():
             d[name].zero_()
             d["out"].fill_(7.0)
-            ops.argmax_rows(slow, d[name])
+            ops.rmsnorm_rows(ones, weights, 0.0, row)
             return b.run(ops, scratch)
         outs = [call().clone() for _ in range(10)]
+        torch.cuda.synchronize()                                  # (one scratch: one stream at a time)
         side = torch.cuda.Stream()
         with torch.cuda.stream(side):
             call()
@@ -137,3 +141,4 @@ def test_lists_written_by_the_kernel_just_before(dtype, hd, wide):
         assert torch.equal(d[name], right)
         for out in outs:
             assert float(((out.double().cpu() - want).abs() - tol).max()) <= 0
+        d[name] = kept
