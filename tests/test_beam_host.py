@@ -325,3 +325,25 @@ def test_pages_of_many_holders_cost_no_more_than_those_of_few():
     for n in names:
         t.close(n)
     assert Name.seen <= 4 * 41 * 400 and t.pools[0].free_pages == 500
+
+
+def test_what_the_kernels_count_stays_within_31_bits():
+    """Of sizes that are taken: the ends of a walk's keys (a unit's empty tiles counted, and four tiles of 128 asked for ahead), a line's tiles and where the last of its workers
+    begins (at most 16 on each of two blocks of 160 multiprocessors).  Tables of nearly 2^31 positions, which passed them, are refused by the entry and by attention_shared_takes alike."""
+    lib, null, some = ops.lib(), ctypes.c_void_p(0), 64
+
+    def entry(n, nh, hd, reach):
+        args = ctypes.create_string_buffer(ops._SHARED_ARGS.pack(*[some] * 9, some, 0, 4, 4, n, 1, 10, nh, nh, hd, 16, reach // 16, 0.1, 1, some))
+        return lib.vk_attention_shared(args, null)
+
+    rng = random.Random(4)
+    sizes = [(1, 1, 64, (1 << 31) - 16), (1, 1, 64, 1 << 30), (1, 1, 64, (1 << 30) + 16), (16, 1, 64, (1 << 30) - 1024), (16, 1, 64, (1 << 30) + 16), (256, 8, 128, 1 << 23), (2, 8, 128, 1 << 30), (8, 2, 64, 1 << 30)]
+    sizes += [(rng.choice([1, 2, 3, 16, 100, 256]), rng.choice([1, 2, 5, 32, 64]), 64, 16 << rng.randint(0, 26)) for _ in range(300)]
+    taken = 0
+    for n, nh, hd, reach in sizes:
+        assert entry(n, nh, hd, reach) == (-4 if ops.attention_shared_takes(torch.bfloat16, nh, nh, hd, n, reach) else -3), (n, nh, hd, reach)      # -4: no room in the scratch is what stops it
+        if ops.attention_shared_takes(torch.bfloat16, nh, nh, hd, n, reach):
+            line = n * nh * (-(-reach // 16) + 16)
+            assert reach + 16 * 16 + 4 * 128 < 1 << 31 and line + 160 * 2 * 16 * 2 < 1 << 31
+            taken += 1
+    assert taken > 100 and not ops.attention_shared_takes(torch.bfloat16, 1, 1, 64, 1, (1 << 31) - 16)

@@ -544,10 +544,10 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
     if (n > SA_MAX_TOKENS || families > SA_MAX_TOKENS || nkv > SA_MAX_KV_HEADS || hd > 256) return VK_TOO_LARGE;
     const int vec = dtype == 0 ? 4 : 8;
     if (nkv <= 0 || nh <= 0 || nh % nkv || nh / nkv > SA_MAX_HEADS || hd <= 0 || hd % vec || page_size <= 0 || max_blocks <= 0 || pages <= 0 || !error) return VK_BAD_SHAPE;
-    if ((long long)max_blocks * page_size > 0x7fffffffLL) return VK_TOO_LARGE;
-    // the lines' tiles and the parts' rows are counted in 31 bits
-    const long long tiles = (long long)max_blocks * page_size / SA_TILE + 64, units = (long long)n * nh;
-    if (tiles * units > 0x7fffffffLL || units * 4 * hd > 0x7fffffffLL) return VK_TOO_LARGE;
+    // positions, the lines' tiles and the parts' rows are counted in 31 bits: a walk asks a few tiles behind its part's end and a unit's empty tiles stand behind its keys, the last worker
+    // begins up to a tile a worker behind the line's end, so half of what 31 bits hold
+    const long long reach = (long long)max_blocks * page_size, tiles = reach / SA_TILE + 64, units = (long long)n * nh;
+    if (reach > 1 << 30 || tiles * units > 1 << 30 || units * 4 * hd > 0x7fffffffLL) return VK_TOO_LARGE;
     if (((uintptr_t)q | (uintptr_t)cache | (uintptr_t)out | (uintptr_t)scratch) % 16) return VK_BAD_ALIGNMENT;
     if (scratch_bytes < vk_attention_shared_scratch_bytes(n, nh, nkv, hd)) return VK_SMALL_SCRATCH;
     const int sms = sa_multiprocessors();

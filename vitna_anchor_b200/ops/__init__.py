@@ -2281,7 +2281,7 @@ def attention_shared_takes(dtype: torch.dtype, nh: int, nkv: int, hd: int, token
     """Whether attention_shared takes these sizes, `reach` positions a block table (else the members' tables are read one by one, by attention_decode or attention_rows)."""
     return (dtype in (torch.float32, torch.bfloat16) and 0 < hd <= 256 and hd % (4 if dtype == torch.float32 else 8) == 0 and 0 < nkv <= SHARED_MAX_KV_HEADS
             and nh % nkv == 0 and 0 < nh // nkv <= SHARED_MAX_HEADS and tokens <= SHARED_MAX_TOKENS
-            and (reach // 16 + 64) * tokens * nh < 1 << 31 and tokens * nh * hd * 4 < 1 << 31)      # the kernels count tiles of 16 keys and rows of outputs in 31 bits
+            and reach <= 1 << 30 and (reach // 16 + 64) * tokens * nh <= 1 << 30 and tokens * nh * hd * 4 < 1 << 31)      # what the kernels count in 31 bits stays within
 
 
 def attention_shared_serves(dtype: torch.dtype, nh: int, nkv: int, hd: int, tokens: int, reach: int) -> bool:
