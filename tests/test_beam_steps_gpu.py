@@ -142,3 +142,46 @@ def test_lists_written_by_the_kernel_just_before(dtype, hd, wide):
         for out in outs:
             assert float(((out.double().cpu() - want).abs() - tol).max()) <= 0
         d[name] = kept
+
+
+def test_launches_are_counted_as_they_are(dirs):
+    """One for members walked by themselves, two for the walk and its join, none where nobody asks for anything; a move a 128; and so for a step that is replayed."""
+    from test_beam_ops_gpu import Batch
+    from vitna_anchor_b200 import ops
+
+    def count(fn):
+        before = ops.launch_count()
+        fn()
+        return ops.launch_count() - before
+
+    for dtype in (torch.bfloat16, torch.float32):
+        for wide, kernels in ((True, 2), (False, 1)):
+            b = Batch([(500, [20, 3])], 8, 2, 64, 16, dtype, seed=1).device(wide)
+            assert count(lambda: b.run(ops)) == kernels
+            b.d.update(members=b.d["members"][:0], starts=b.d["starts"][:1], shared=b.d["shared"][:0])
+            assert count(lambda: b.run(ops)) == 0
+    arena = torch.zeros(2, 400, 16, device="cuda")
+    for moves, kernels in [(0, 0), (1, 1), (128, 1), (129, 2), (200, 2)]:
+        assert count(lambda: ops.copy_rows(arena, list(range(moves)), list(range(200, 200 + moves)))) == kernels
+    none = lambda t: torch.empty((0, 3), dtype=t, device="cuda")      # noqa: E731
+    assert count(lambda: ops.beam_select(torch.empty(0, 50, device="cuda"), torch.empty(0, device="cuda"), 2, 3, (none(torch.float32), none(torch.int32), none(torch.int32)),
+                                         torch.zeros(4096, dtype=torch.uint8, device="cuda"))) == 0
+    # whole steps: with the walk and its join a layer has one launch more than with attention_decode's one
+    from vitna_anchor_b200.engine.loading import load_model
+    from vitna_anchor_b200.engine.runner import ModelRunner, StepEntry
+    model = load_model(dirs[64], "bfloat16", "cuda")
+    layers = len(model.schedule)
+    r = ModelRunner(model, page_size=16, max_requests=16, max_batch_tokens=256, max_model_len=32768, num_pages=100)
+    r.open(0)
+    r.step([StepEntry(0, [int(t) for t in np.random.default_rng(1).integers(0, model.vocab_size, 200)], [])])
+    r.fork_many([(i, 0) for i in range(1, 16)])
+    per_step = {}
+    for mode in (0, 1):
+        before = ops.set_attention_shared(mode)
+        try:
+            counts = [count(lambda: r.step([StepEntry(i, [3], [0]) for i in range(16)])) for _ in range(3)]
+        finally:
+            ops.set_attention_shared(before)
+        assert len(set(counts)) == 1                                  # eager and captured, replayed, replayed
+        per_step[mode] = counts[0]
+    assert per_step[1] - per_step[0] == layers

@@ -512,6 +512,8 @@ static int sa_multiprocessors() {
     return n;
 }
 
+static int launched(int status, int kernels) { return status == VK_OK ? VK_LAUNCHED + kernels : status; }
+
 // Rows of parts that a launch can need: a unit of so many tiles of keys and up to R rows leaves at most R (tiles / L + 2), L is at least the line's
 // length / workers, and the units' rows are n nh together.  R is 128 for prefixes here and the workers a multiprocessor's blocks (2) and warps (16), which covers
 // both kernels.
@@ -536,6 +538,8 @@ struct VkAttentionShared {
     int32_t dtype;
     int* error;                    // set where a wait inside the kernel runs out
 };
+
+// Returns VK_LAUNCHED + 1 (every member by itself) or + 2 (the walk, and the launch that joins the parts); VK_OK where nobody asks for anything.
 
 VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t stream) {
     const auto [q, cache, block_tables, token_seg, positions, members, starts, shared, out, scratch, scratch_bytes, tokens, segments, n, families, pages, nh, nkv, hd, page_size,
@@ -565,11 +569,11 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
     for (int b = 0; b < 30; b++) if ((1 << b) == page_size) a.page_shift = b;
     a.scale_log2 = scale * 1.4426950408889634f;
     if (attention_shared_mma_takes(a, dtype)) {
-        if (attention_each_mma_takes(a)) return launch_attention_each_mma(a, sms, stream);
+        if (attention_each_mma_takes(a)) return launched(launch_attention_each_mma(a, sms, stream), 1);
         const int status = launch_attention_shared_mma(a, sms, error, stream);
-        return status != VK_OK ? status : launch_join(a, dtype, stream);
+        return status != VK_OK ? status : launched(launch_join(a, dtype, stream), 2);
     }
-    if (each_takes(a, dtype)) return launch_each(a, dtype, sms, stream);
+    if (each_takes(a, dtype)) return launched(launch_each(a, dtype, sms, stream), 1);
     a.prefix_rows = SG_PREFIX_ROWS;
     a.own_rows = SG_ROWS;
     a.row_unit = 16.0f;
@@ -586,7 +590,7 @@ VK_API int vk_attention_shared(const VkAttentionShared* args, cudaStream_t strea
         const int e = sa_allow_smem(kern, smem);                                                                                        \
         if (e != VK_OK) return e;                                                                                                       \
         const int status = launch_dependent(kern, dim3(a.blocks), dim3(SA_THREADS), smem, stream, a);                                        \
-        return status != VK_OK ? status : launch_join(a, dtype, stream);                                                                \
+        return status != VK_OK ? status : launched(launch_join(a, dtype, stream), 2);                                                   \
     } while (0)
     if (dtype == 0) {
         if (hd <= 64) GO(float, 2);

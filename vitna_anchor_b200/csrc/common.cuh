@@ -21,6 +21,9 @@
 #define VK_TOO_LARGE (-3)      // beyond a stated maximum
 #define VK_SMALL_SCRATCH (-4)  // fewer bytes of scratch than the call needs
 
+// What an entry whose launches depend on the sizes returns where all went well: this + the kernels that it launched (CUDA's errors are smaller numbers; VK_OK: none was needed).
+#define VK_LAUNCHED 0x100000
+
 namespace vk {
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);

@@ -91,6 +91,18 @@ def _check(status: int, what: str) -> None:
     raise KernelError(f"{what}: CUDA error {status}: {text}")
 
 
+_LAUNCHED = 0x100000      # VK_LAUNCHED
+
+
+def _check_launches(status: int, what: str) -> None:
+    """_check for an entry that says how many kernels it launched (0: none)."""
+    if status > _LAUNCHED:
+        _check(0, what)
+        add_launches(status - _LAUNCHED - 1)
+    elif status != 0:
+        _check(status, what)
+
+
 def kernel_times(fn) -> dict:
     """Run fn() with an event behind every launch of this library and return {launch name: (count, milliseconds)}: the time
     from the end of the launch before it to its own end.  Exact where the stream stays busy (a prompt's step, issued eagerly);
@@ -2360,8 +2372,7 @@ def attention_shared(q: torch.Tensor, cache_layer: torch.Tensor, block_tables: t
         raise KernelError("attention_shared: starts is not one longer than shared, or there are more than 256 families")
     args = _SHARED_ARGS.pack(pq, pc, pt, ps, pp, pm, pst, psh, po, _fit(scratch, "scratch", torch.uint8, 1, here), scratch.numel(), T, segments, n, families, pages, nh, nkv,
                              hd, page_size, max_blocks, scale, dtype is torch.bfloat16, error_word().data_ptr())
-    _check(_entry("vk_attention_shared", "pp")(args, torch._C._cuda_getCurrentRawStream(here)), "attention_shared")
-    add_launches(1)                       # the walk, and the launch that joins the rows' parts
+    _check_launches(_entry("vk_attention_shared", "pp")(args, torch._C._cuda_getCurrentRawStream(here)), "attention_shared")
     return out
 
 
@@ -2392,6 +2403,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
         raise KernelError("beam_select: rows are not whole requests, scores are not one a row, or more is kept than there is")
     if best.shape != (R // beams, keep) or parent.shape != best.shape or token.shape != best.shape:
         raise KernelError("beam_select: out is not three of [requests, keep]")
+    if R == 0:
+        return out
     fn = _entry("vk_beam_select", "ppppppziiilip")
     _check(fn(logits.data_ptr(), ps, pb, pp, pt, _fit(scratch, "scratch", torch.uint8, 1, here), scratch.numel(), R, beams, V, logits.stride(0) if R > 1 else V, keep,
               torch._C._cuda_getCurrentRawStream(here)), "beam_select")
@@ -2428,4 +2441,5 @@ def copy_rows(arena: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> to
     fn = _entry("vk_copy_rows", "piilllppip")
     _check(fn(arena.data_ptr(), L, N, layer * size if L > 1 else 0, row * size, numbers * size, s.buffer_info()[0], d.buffer_info()[0], n,
               torch._C._cuda_getCurrentRawStream(here)), "copy_rows")
+    add_launches((n - 1) // 128)
     return arena
