@@ -185,3 +185,27 @@ def test_launches_are_counted_as_they_are(dirs):
         assert len(set(counts)) == 1                                  # eager and captured, replayed, replayed
         per_step[mode] = counts[0]
     assert per_step[1] - per_step[0] == layers
+
+
+@pytest.mark.parametrize("vocab", [512, 49152, 262144])
+@pytest.mark.parametrize("kind", ["flat", "normal", "wide", "likely", "rising", "high"])
+def test_a_rows_log_sum(kind, vocab):
+    """What the order across beams hangs on: the best token's continuation at a sum that makes it nearly 0, where float32 holds it to 2^-40, is off by the row's log sum alone.  A thread adds
+    up to 128 terms of relative error 2^-22 + 2^-24 of their arguments (weighted by the terms at most 13, the logarithm of their number), 127 steps of 2^-24, and 8 + 2 x 26 exponentials of 2^-22 of
+    new maxima and joins: 2^-15 together."""
+    from vitna_anchor_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = torch.randn(64, vocab, generator=g, device="cuda") * {"flat": 1e-3, "wide": 5.0}.get(kind, 2.0)
+    if kind == "likely":
+        at = torch.randint(0, vocab, (64, 200), generator=g, device="cuda")
+        x.scatter_add_(1, at, torch.rand(at.shape, generator=g, device="cuda") * 9)
+    elif kind == "rising":
+        x = x.sort(dim=1).values
+    elif kind == "high":
+        x += 200
+    top, lse = x.max(1).values.double(), torch.logsumexp(x.double(), 1)
+    scores = (lse - top).float()
+    out = tuple(torch.empty((64, 1), dtype=t, device="cuda") for t in (torch.float32, torch.int32, torch.int32))
+    ops.beam_select(x, scores, 1, 1, out, torch.zeros(ops.beam_select_scratch_bytes(64, vocab, 1), dtype=torch.uint8, device="cuda"))
+    assert torch.equal(out[2][:, 0].long(), x.argmax(1))
+    assert float((out[0][:, 0].double() - (scores.double() + top - lse)).abs().max()) <= 2.0 ** -15

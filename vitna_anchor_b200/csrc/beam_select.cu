@@ -7,8 +7,10 @@
 //
 // One launch, one read of the logits.  A block walks a stretch of a row, 4,096 values at a time in registers (float32, as the logits come) with the next ones on their way, and leaves
 // the values' maximum, their sum of exponentials against it and their `keep` best in order: within a row c and x have the same order, so neither needs the row's sum.
-// The block that completes a request joins the sums and merges its lists; c is computed there, in float64, for the few values that are left, so that two
-// beams' candidates are told apart where float32 sums would tie.
+// The block that completes a request joins the sums and merges its lists; c is computed there, in float64, for the few values that are left, so that a row's candidates keep the
+// order of its values and none is lost to the rounding of score + x.  Across rows the order is as good as the rows' log sums, whose sums of exponentials are float32: off by 5e-7 at most in
+// what was measured (512 to 262,144 tokens, values that are normal, equal, rising, flat, a few hundred far above the rest), and by less than 2^-15 whatever the values are (up to 128 terms added
+// one after the other by a thread, 8 times a new maximum, some 26 joins, each exponential to 2^-22 and 2^-24 of its argument): candidates of two rows that lie closer may change places.
 //
 // Choosing `keep` of many, without sorting them: the block's threads make 32 to 256 groups, at least twice as many as are kept; the keep-th largest of the groups'
 // best is a bound that at least `keep` values reach and few others do (17 values of 4,096 normal ones above the bound for keep = 8, 150 for 64).  Every thread knows its largest value of each
