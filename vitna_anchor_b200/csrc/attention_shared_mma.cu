@@ -15,10 +15,10 @@
 //
 // A member's own keys are walked by single warps with the same routines (R = 1): up to 16 rows of heads.
 //
-// What bounds it.  64 requests behind 6,000 positions with up to 700 of their own, 32 heads of 64 (214 MB): 49 us, 4.4 TB/s; the common keys' blocks do 64 rows a key, 16,000 cycles of the tensor
+// What bounds it.  64 requests behind 6,000 positions with up to 700 of their own, 32 heads of 64 (214 MB): 48.5 us, 4.4 TB/s; the common keys' blocks do 64 rows a key, 16,000 cycles of the tensor
 // cores' legacy path, and take 37,000 (a group's warps do scores, softmax and p v in step, 4 warps a scheduler), while the own keys' blocks beside them wait for memory.  One kind after the
-// other in every block: 57 us.  Eight beams of 2,048 positions, 32 heads of 64 (20 MB): 11.6 us, of which finding the parts is 2 (it runs before the wait for the kernel
-// before) and joining them 3.
+// other in every block: 57 us.  Eight beams of 2,048 positions, 32 heads of 64 (20 MB): 12.1 us, of which finding the parts is 2 (it runs before the wait for the kernel
+// before), looking behind the wait whether they hold 0.3, and joining them 3.
 #include "attention_shared_plan.cuh"
 #include "tcgen05_common.cuh"
 
@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(SA_THREADS, HD == 64 ? 2 : 1) attention_shared
 //
 // Where the members' tables are short and few, reading common keys once is worth less than what it takes to find out who has which in common and to bring the two kinds of parts
 // together: a cluster of blocks walks a member's whole table for one tile of heads, a run of its keys a block, its eight warps in turn, and the blocks' outputs meet through
-// each other's shared memory.  One launch, nothing in scratch memory.  Four beams of 512 positions, 9 heads over 3 of 64: 4.0 us (8.2 the other way); the launch, five dependent trips to
+// each other's shared memory.  One launch, nothing in scratch memory.  Four beams of 512 positions, 9 heads over 3 of 64: 4.7 us in a captured graph, caches cold (with the lists read before the wait 4.2, and 8.2 the other way); the launch, six dependent trips to
 // memory and the cluster's two meetings are all of it.
 
 template <int HD>
@@ -859,8 +859,8 @@ bool attention_shared_mma_takes(const SaArgs& a, int dtype) {
 // (99 MB), 13.8 / 12.7; 64 of 128, 32 heads (109 MB), 20.4 / 15.6; 8 of 2,048, 32 heads (139 MB), 12.7 / 11.4; 64 of 512, 32 heads (310 MB), 34 / 17.  Heads of 128 (2 of them, 8 queries
 // each): 16 of 8,000 (132 MB) 14.8 / 19.5, 64 of 2,048 (139 MB) 13.6 / 21.8, 32 of 8,000 (265 MB) 23.5 / 23.3, 64 of 8,000 (530 MB) 40 / 35.
 // attention_decode, which reads every member's table too but in runs of 256 keys that meet through memory, has 4 key-value heads of four queries each, in tables of 4,096, so (this way / it):
-// heads of 64, 4 members of 500 common positions 4.7 / 4.1 us, of 2,000 5.5 / 4.6, 8 of 2,000 6.3 / 5.3, 16 of 500 5.2 / 4.8, of 2,000 7.1 / 10.2; heads of 128, 4 of 500 5.3 / 5.0, of 2,000 7.0 / 5.9,
-// 8 of 2,000 7.5 / 11.7, 16 of 500 6.0 / 11.0, of 2,000 9.6 / 22.9.  ops.attention chooses between the two by whole steps (attention_shared_pays).
+// heads of 64, 4 members of 500 common positions 5.1 / 4.1 us, of 2,000 5.9 / 4.6, 8 of 2,000 6.6 / 5.3, 16 of 500 5.5 / 4.8, of 2,000 7.2 / 10.2; heads of 128, 4 of 500 5.8 / 5.0, of 2,000 7.5 / 5.9,
+// 8 of 2,000 7.8 / 11.7, 16 of 500 6.3 / 11.0, of 2,000 10.0 / 23.0.  ops.attention chooses between the two by whole steps (attention_shared_pays).
 bool attention_each_mma_takes(const SaArgs& a) {
     return (long long)a.n * a.max_blocks * a.page_size * a.nkv * a.hd * 4 <= (a.hd == 64 ? 96ll << 20 : 240ll << 20);
 }

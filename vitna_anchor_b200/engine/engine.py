@@ -238,7 +238,7 @@ class Engine:
     def beam_search(self, ids: Sequence[int], *, beams: int = 4, max_new: int = 64, length_penalty: float = 1.0,
                     stop_ids: Iterable[int] = ()) -> List[BeamResult]:
         """The `beams` best continuations of one prompt, best first (engine/beam.py says what is best and when the search ends; fewer where
-        the vocabulary or the stop ids leave fewer).  The beams take `beams` of the engine's request slots and run by themselves: while requests that were
+        the vocabulary or the stop ids leave fewer; StepFailed where the logits are no numbers).  The beams take `beams` of the engine's request slots and run by themselves: while requests that were
         added are not finished the search is refused."""
         ids = [int(t) for t in ids]
         if not ids:

@@ -2318,7 +2318,7 @@ def attention_shared_pays(saved: int, nkv: int, hd: int, dtype: torch.dtype = to
 
     Against attention_decode, from 64 MB of them on.  Whole steps of a beam search, this way against the other.  Heads of 64: 8 beams of 2,000 positions, 32 heads over 24 layers (115 MB),
     1.70 ms against 1.84, 64 of 8,000 (4.1 GB) 4.5 / 16.0; 16 of 4,000, 5 heads, 32 layers (77 MB) 1.68 / 1.72; 4 of 2,000, 32 heads (49 MB) 1.61 / 1.49, 16 of 500 (61 MB) 1.77 / 1.71; 32 of
-    500, 3 heads, 30 layers (12 MB) 1.38 / 1.20.  Heads of 128: 32 over 8, 16 layers, 16 beams of 2,000 (117 MB) 1.47 / 1.85, 8 of 2,000 (55 MB) 1.32 / 1.35, 4 of 2,000 (23 MB) 1.23 / 1.10.
+    500, 3 heads, 30 layers (12 MB) 1.38 / 1.20; on the wrong side 64 of 2,000, 3 heads (92 MB), 2.06 / 1.98, and 8 of 8,000 (41 MB) 1.10 / 1.28.  Heads of 128: 32 over 8, 16 layers, 16 beams of 2,000 (117 MB) 1.47 / 1.85, 8 of 2,000 (55 MB) 1.32 / 1.35, 4 of 2,000 (23 MB) 1.23 / 1.10.
     float32: 32 beams of 2,000, 3 heads of 64 (91 MB), 5.15 / 5.78, 8 of 2,000 (21 MB) 2.40 / 2.35.  Other sizes up to 128, which both have on float32 units: 4 to 16 members from 70 MB on
     1.3 to 4.2 times as fast a layer.
     Not at all in bfloat16 with heads of 16, 32 and 96, which attention_decode has on the tensor cores and attention_shared on float32 units (8 beams of 2,000, 32 heads of 96, 164 MB, 2.33 ms a
