@@ -347,3 +347,19 @@ def test_what_the_kernels_count_stays_within_31_bits():
             assert reach + 16 * 16 + 4 * 128 < 1 << 31 and line + 160 * 2 * 16 * 2 < 1 << 31
             taken += 1
     assert taken > 100 and not ops.attention_shared_takes(torch.bfloat16, 1, 1, 64, 1, (1 << 31) - 16)
+
+
+def test_a_refused_holder_leaves_a_page_unshared():
+    pool = PagePool(2)
+    a = pool.alloc("x")
+    with pytest.raises(CacheError):
+        pool.share(a, "x")
+    assert not pool.is_shared(a) and not pool.has_shared
+    pool.share(a, "y")
+    with pytest.raises(CacheError):
+        pool.share(a, "y")
+    pool.free(a, "y")
+    assert not pool.is_shared(a) and not pool.has_shared and pool.holders(a) == ["x"]
+    pool.free(a, "x")
+    pool.check()
+    assert pool.free_pages == 2

@@ -83,10 +83,9 @@ class PagePool:
             raise CacheError("a page needs an owner")
         if not (0 <= page < self.num_pages) or self._owner[page] is None:
             raise CacheError(f"page {page} is held by nobody")
-        more = self._more.setdefault(page, {})
-        if owner == self._owner[page] or owner in more:
+        if owner == self._owner[page] or owner in self._more.get(page, ()):
             raise CacheError(f"page {page} is held by {owner!r} already")
-        more[owner] = None
+        self._more.setdefault(page, {})[owner] = None
 
     def holders(self, page: int) -> List[Hashable]:
         """Who holds the page (nobody: it is free)."""
