@@ -159,3 +159,13 @@ def test_where_reading_common_pages_once_was_measured_to_be_faster(sizes, once):
     saved, nkv, hd, dtype, context = sizes
     assert ops.attention_shared_pays(saved, nkv, hd, dtype, True, context) == once
     assert not ops.attention_shared_pays(saved, nkv, hd, dtype, False, context)
+
+
+def test_a_model_says_which_of_its_cache_layers_are_read_so():
+    """By cache layer; a mixer that knows nothing of it (a class of its own) reads every request by itself."""
+    from vitna_anchor_b200.models.decoder import DecoderModel, LayerRun
+    can, cannot, own = SimpleNamespace(common_heads=lambda: (4, 2, 16)), SimpleNamespace(common_heads=lambda: None), SimpleNamespace()
+    m = DecoderModel.__new__(DecoderModel)
+    m.blocks = [SimpleNamespace(mixer=x) for x in (can, cannot, own)]
+    m.schedule = [LayerRun(0, 0), LayerRun(1, 1), LayerRun(2, 2), LayerRun(0, 3), LayerRun(1, -1)]
+    assert m.common_heads == {0: (4, 2, 16), 3: (4, 2, 16)}

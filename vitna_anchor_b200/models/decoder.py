@@ -115,8 +115,13 @@ class DecoderModel:
     @property
     def common_heads(self) -> Dict[int, Tuple[int, int, int]]:
         """By cache layer, for those that an attention reads which can read common pages once (Mixer.common_heads)."""
-        heads = ((run.cache, self.blocks[run.block].mixer.common_heads()) for run in self.schedule if run.cache >= 0)
-        return {cache: h for cache, h in heads if h is not None}
+        found = {}
+        for run in self.schedule:
+            mixer = self.blocks[run.block].mixer
+            heads = mixer.common_heads() if run.cache >= 0 and hasattr(mixer, "common_heads") else None
+            if heads is not None:
+                found[run.cache] = heads
+        return found
 
     def forward(self, ctx: StepContext, logit_rows: Optional[torch.Tensor], out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """Run the batch; float32 logits [len(logit_rows), vocab] for the flat token indices in logit_rows
