@@ -154,7 +154,7 @@ def test_which_attentions_can_read_common_pages_once():
     ((3 * 4000, 32, 256, torch.bfloat16, 4096), False), ((15 * 4000, 4, 80, torch.bfloat16, 4096), True), ((63 * 4000, 4, 24, torch.bfloat16, 4096), True), ((3 * 4000, 4, 80, torch.bfloat16, 4096), False),
     ((31 * 2000, 3, 64, torch.float32, 4096), True), ((7 * 2000, 3, 64, torch.float32, 4096), False), ((3 * 2000, 32, 64, torch.float32, 4096), True), ((15 * 2000, 4, 128, torch.float32, 4096), True),
     ((3 * 2000, 5, 64, torch.bfloat16, 65536), True), ((3 * 8000, 32, 32, torch.bfloat16, 65536), True), ((500, 32, 256, torch.bfloat16, 65536), True), ((96, 32, 256, torch.bfloat16, 65536), False),
-    ((48, 2, 64, torch.bfloat16, 65536), False), ((3 * 2000, 5, 64, torch.bfloat16, 32768), False)])
+    ((6000, 4, 256, torch.float32, 4096), True), ((100, 4, 256, torch.float32, 4096), False), ((48, 2, 64, torch.bfloat16, 65536), False), ((3 * 2000, 5, 64, torch.bfloat16, 32768), False)])
 def test_where_reading_common_pages_once_was_measured_to_be_faster(sizes, once):
     saved, nkv, hd, dtype, context = sizes
     assert ops.attention_shared_pays(saved, nkv, hd, dtype, True, context) == once

@@ -2325,8 +2325,9 @@ def attention_shared_pays(saved: int, nkv: int, hd: int, dtype: torch.dtype = to
     step against 1.70; a layer of 64 members behind 8,000, four queries a key-value head of 4, heads of 96 208 us / 177, of 32 91 / 79; with many members and a query a head it would be the
     faster one, 16 of 4,000 with 32 heads of 32 1.62 ms / 2.09), nor with heads above 128 (4 members of 4,000, 32 heads of 256: 463 us / 309).
 
-    Against attention_rows, which contexts of more than 32,768 positions take, from 4 MB on: 4 beams of 500, 5 heads of 64, 32 layers (2 MB) 1.16 ms a step / 2.73, 4 of 8,000, 32 heads of
-    32 (94 MB) 1.40 / 11.5; a layer of 2 members of 100, 32 heads of 256 (3 MB), 55 us / 36, of 500 (15 MB) 96 / 166."""
+    Against attention_rows, which contexts of more than 32,768 positions take, and float32 heads above 128, from 4 MB on: 4 beams of 500, 5 heads of 64, 32 layers (2 MB) 1.16 ms a step / 2.73, 4 of 8,000, 32 heads of
+    32 (94 MB) 1.40 / 11.5; a layer of 2 members of 100, 32 heads of 256 (3 MB), 55 us / 36, of 500 (15 MB) 96 / 166; in
+    float32, 32 heads of 256, 2 of 100 (6 MB) 36 / 41, 4 of 2,000 (375 MB) 160 / 697."""
     if _shared_mode != 2:
         return _shared_mode == 1 and saved > 0
     least = 64 << 20
