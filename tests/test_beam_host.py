@@ -363,3 +363,21 @@ def test_a_refused_holder_leaves_a_page_unshared():
     pool.free(a, "x")
     pool.check()
     assert pool.free_pages == 2
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0), (2, 3, 0, 5), (2, 3, 4, 0), (0, 3, 4), (2, 3, 5)])
+def test_rows_of_no_numbers_are_not_moved(monkeypatch, shape):
+    """An empty row's stride is one number in torch: nothing is launched for it (there is no memory behind it)."""
+    calls = []
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0, raising=False)
+    monkeypatch.setattr(ops, "_entry", lambda name, types: lambda *a: calls.append(a) or 0)
+    arena = torch.zeros(shape)
+    assert ops.copy_rows(arena, [0], [2]) is arena
+    assert len(calls) == (1 if arena.numel() else 0)
+    if arena.numel():
+        assert calls[0][1:3] == shape[:2] and calls[0][5] == shape[2] * 4          # layers, rows, bytes a row
+    if arena.shape[0]:
+        for src, dst in [([0], [3]), ([-1], [1]), ([0, 1], [2])]:
+            with pytest.raises(ops.KernelError):
+                ops.copy_rows(arena, src, dst)

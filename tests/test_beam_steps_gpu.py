@@ -163,6 +163,7 @@ def test_launches_are_counted_as_they_are(dirs):
     arena = torch.zeros(2, 400, 16, device="cuda")
     for moves, kernels in [(0, 0), (1, 1), (128, 1), (129, 2), (200, 2)]:
         assert count(lambda: ops.copy_rows(arena, list(range(moves)), list(range(200, 200 + moves)))) == kernels
+    assert count(lambda: ops.copy_rows(torch.empty(2, 3, 0, device="cuda"), [0], [2])) == 0
     none = lambda t: torch.empty((0, 3), dtype=t, device="cuda")      # noqa: E731
     assert count(lambda: ops.beam_select(torch.empty(0, 50, device="cuda"), torch.empty(0, device="cuda"), 2, 3, (none(torch.float32), none(torch.int32), none(torch.int32)),
                                          torch.zeros(4096, dtype=torch.uint8, device="cuda"))) == 0

@@ -2435,10 +2435,10 @@ def copy_rows(arena: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> to
     n, written = len(src), set(dst)
     if len(dst) != n or len(written) != n or not written.isdisjoint(src):
         raise KernelError("copy_rows: src and dst differ in length, or a row is written twice, or read and written")
-    if n == 0 or L == 0 or numbers == 0:
-        return arena
-    if min(src) < 0 or min(dst) < 0 or max(src) >= N or max(dst) >= N:
+    if n and (min(src) < 0 or min(dst) < 0 or max(src) >= N or max(dst) >= N):
         raise KernelError(f"copy_rows: a row is outside the arena's {N}")
+    if n == 0 or arena.numel() == 0:             # (the stride of a row of no numbers is not 0)
+        return arena
     s, d = array.array("i", src), array.array("i", dst)
     fn = _entry("vk_copy_rows", "piilllppip")
     _check(fn(arena.data_ptr(), L, N, layer * size if L > 1 else 0, row * size, numbers * size, s.buffer_info()[0], d.buffer_info()[0], n,
