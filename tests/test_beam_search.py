@@ -181,7 +181,19 @@ def test_the_engine_refuses_such_a_penalty():
     from vitna_anchor_b200.engine.engine import Engine, RequestRefused
     eng = Engine.__new__(Engine)
     eng.model, eng.ctx = SimpleNamespace(vocab_size=50), 64
-    eng.runner = SimpleNamespace(cache=SimpleNamespace(max_requests=4))
+    eng.runner = SimpleNamespace(cache=SimpleNamespace(max_requests=4), max_batch_tokens=64)
     for penalty in (400.0, -400.0, float("nan"), float("-inf")):
         with pytest.raises(RequestRefused, match="length_penalty"):
             eng.beam_search([1], beams=2, max_new=20, length_penalty=penalty)
+
+
+def test_the_engine_refuses_more_beams_than_a_step_takes_tokens():
+    """A step of more single tokens than the step limit was refused in the middle of the search, when it widened."""
+    from types import SimpleNamespace
+    from vitna_anchor_b200.engine.engine import Engine, RequestRefused
+    eng = Engine.__new__(Engine)
+    eng.model, eng.ctx = SimpleNamespace(vocab_size=50), 64
+    eng.runner = SimpleNamespace(cache=SimpleNamespace(max_requests=16), max_batch_tokens=4)
+    for beams in (0, 5, 16, 17):
+        with pytest.raises(RequestRefused, match="between 1 and 4"):
+            eng.beam_search([1], beams=beams, max_new=20)

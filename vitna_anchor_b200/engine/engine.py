@@ -246,9 +246,9 @@ class Engine:
         for t in ids:
             if not (0 <= t < self.model.vocab_size):
                 raise RequestRefused(f"token id {t} is outside the vocabulary of {self.model.vocab_size}")
-        most = min(self.runner.cache.max_requests, ops.BEAM_MAX_BEAMS)
+        most = min(self.runner.cache.max_requests, self.runner.max_batch_tokens, ops.BEAM_MAX_BEAMS)
         if not (1 <= beams <= most):
-            raise RequestRefused(f"beams is between 1 and {most} (the engine's parallel requests)")
+            raise RequestRefused(f"beams is between 1 and {most} (the engine's parallel requests, the tokens of a step)")
         if max_new < 1:
             raise RequestRefused("max_new must be at least 1")
         if len(ids) + max_new > self.ctx:
