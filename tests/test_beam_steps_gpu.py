@@ -210,3 +210,53 @@ def test_a_rows_log_sum(kind, vocab):
     ops.beam_select(x, scores, 1, 1, out, torch.zeros(ops.beam_select_scratch_bytes(64, vocab, 1), dtype=torch.uint8, device="cuda"))
     assert torch.equal(out[2][:, 0].long(), x.argmax(1))
     assert float((out[0][:, 0].double() - (scores.double() + top - lse)).abs().max()) <= 2.0 ** -15
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.5, 1e-3, 1.0])
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64), (torch.bfloat16, 40)])
+def test_other_scales(dtype, hd, wide, scale):
+    """None (every key alike), one that turns the order round, which the tensor-core kernels do not take, a small and a large one.  The tolerance is that of test_beam_ops_gpu with
+    the scores' size at this scale: hd products of 32 bits a score, p as two bfloat16 parts and 2^x by the special-function unit, sums in 32 bits, the output's rounding."""
+    from test_beam_ops_gpu import Batch
+    from vitna_anchor_b200 import ops
+    nh, nkv = 8, 2
+    b = Batch([(300, [20, 3, 41, 9]), (64, [7, 30])], nh, nkv, hd, 16, dtype, seed=5).device(wide)
+    d, n = b.d, len(b.pos)
+    scratch = torch.zeros(ops.attention_shared_scratch_bytes(n, nh, nkv, hd), dtype=torch.uint8, device="cuda")
+    got = ops.attention_shared(d["q"], d["cache"], d["tables"], d["seg"], d["pos"], d["members"], d["starts"], d["shared"], d["out"], scratch, nh, nkv, hd, scale).double().cpu()
+    for t in b.members:
+        at = torch.arange(b.pos[t] + 1)
+        kv = b.cache[torch.tensor(b.tables[t])[at // 16], :, :, at % 16].double()
+        k, v = (kv[:, i].repeat_interleave(nh // nkv, dim=1) for i in (0, 1))
+        q = b.q[t].double().view(nh, hd)
+        o = torch.einsum("hp,phd->hd", torch.softmax(torch.einsum("phd,hd->hp", k, q) * scale, 1), v)
+        size = (torch.einsum("phd,hd->hp", k.abs(), q.abs()) * abs(scale)).amax(1)
+        slack = (2 * hd * 2.0 ** -23 * size + 2.0 ** -16 + 64 * 2.0 ** -23) * v.abs().amax((0, 2))
+        off = (got[t].view(nh, hd) - o).abs() - torch.finfo(dtype).eps / 2 * o.abs() - slack[:, None]
+        assert float(off.max()) <= 0
+
+
+@pytest.mark.parametrize("beams,stops", [(2, 6), (4, 40), (1, 3), (3, 200), (5, 1)])
+def test_a_search_with_many_ends_of_the_text(dirs, beams, stops):
+    """The tokens that the first steps like best end the text: the results of the plain search, which walks every continuation until enough go on (float32, whose logits are the
+    same bits however the work is cut)."""
+    from types import SimpleNamespace
+    from test_beam_search import plain_search
+    from vitna_anchor_b200.engine import beam
+    from vitna_anchor_b200.engine.engine import Engine
+    eng = Engine(dirs[64], dtype="float32", parallel=6, ctx=128, kv_block=4)
+    prompt = [int(t) for t in np.random.default_rng(11).integers(0, 500, 17)]
+    plain = SimpleNamespace(vocab=500, logits_of=lambda ids: eng.logits(ids)[-1].cpu().numpy())
+    stop = {int(t) for t in np.argsort(-plain.logits_of(prompt))[:stops]}
+    wide, all_in_order = [], beam.all_in_order
+    beam.all_in_order = lambda *a: wide.append(1) or all_in_order(*a)
+    try:
+        for penalty in (1.0, 0.0):
+            got = eng.beam_search(prompt, beams=beams, max_new=6, length_penalty=penalty, stop_ids=stop)
+            want = plain_search(plain, prompt, beams, 6, penalty, stop)
+            assert [(r.ids, r.finish_reason) for r in got] == [(ids, why) for ids, _, why in want]
+    finally:
+        beam.all_in_order = all_in_order
+    assert bool(wide) == (stops > beams)
+    assert not eng.runner.cache.tables.requests
