@@ -381,3 +381,15 @@ def test_rows_of_no_numbers_are_not_moved(monkeypatch, shape):
         for src, dst in [([0], [3]), ([-1], [1]), ([0, 1], [2])]:
             with pytest.raises(ops.KernelError):
                 ops.copy_rows(arena, src, dst)
+
+
+def test_pairs_may_come_one_by_one(monkeypatch):
+    """Any iterable of pairs: the states are moved too."""
+    c = CacheManager([StateSpec((3,))], page_size=4, num_pages=4, max_requests=4, dtype=torch.float32, device="cpu")
+    moves = []
+    monkeypatch.setattr(ops, "copy_rows", lambda arena, src, dst: moves.append((list(src), list(dst))))
+    c.open("a")
+    c.fork_many((r, "a") for r in "bc")
+    c.adopt((r, "a") for r in "cb")
+    a, b, d = (c.slot(r) for r in "abc")
+    assert moves == [([a, a], [b, d]), ([a, a], [d, b])]

@@ -144,14 +144,16 @@ class CacheManager:
 
     def fork_many(self, pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
         """fork() for every (request, source), all of them or nothing; the moves of all in one launch for each group of pages and each shape of states."""
+        pairs = list(pairs)
         if pairs:
-            self._copy(self.tables.fork_many(list(pairs)), pairs)
+            self._copy(self.tables.fork_many(pairs), pairs)
 
     def adopt(self, pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
         """For every (request, source): the request forgets what it has and goes on from where the source stands.  No request is named
         twice, or as a source too."""
+        pairs = list(pairs)
         if pairs:
-            self._copy(self.tables.adopt(list(pairs)), pairs)
+            self._copy(self.tables.adopt(pairs), pairs)
 
     def _copy(self, pages: Sequence[tuple], pairs: Sequence[Tuple[Hashable, Hashable]]) -> None:
         from .. import ops
