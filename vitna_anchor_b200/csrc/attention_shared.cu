@@ -341,10 +341,11 @@ __global__ void __launch_bounds__(SE_WARPS * 32) attention_each_kernel(const SaA
 // A row's parts meet: weights 2^(own maximum - row maximum), sums in the parts' order within a lane, then over the lanes, then over the warps, the same in every launch of
 // the same lengths.  WARPS warps a row: one where the rows alone fill the machine, four, eight (up to 256 rows) or sixteen (up to 128) where few rows have many parts, whole calls with 4 / 8 /
 // 16: 256 rows of 70 parts 30.0 / 27.5 / 27.5 us, of 4 parts 11.6 / 11.8 / 12.7, 512 rows 19.9 / 20.6 / 22.7, 128 rows 17.4 / 16.1 / 15.5, 80 rows 19.7 / 17.4 / 16.6.  A part's row is read as 16-byte pieces by
-// L = 2, 4 .. 32 neighbouring lanes, 32 / L parts at once and four of those in flight.
+// L = 2, 4 .. 32 neighbouring lanes, 32 / L parts at once and four of those in flight.  (No pointer is __restrict__: what the walk, or a kernel before it, has written is not constant for a launch that
+// begins beside it, and a load that may be taken for one need not stay behind the wait.)
 template <typename T, int WARPS>
-__global__ void __launch_bounds__(WARPS > 4 ? WARPS * 32 : 128) attention_shared_join_kernel(const SaRow* __restrict__ rows, const float2* __restrict__ part_ml, const float* __restrict__ part_o,
-                                                                    const int32_t* __restrict__ members, T* __restrict__ out, int n_rows, int nh, int hd, int lanes) {
+__global__ void __launch_bounds__(WARPS > 4 ? WARPS * 32 : 128) attention_shared_join_kernel(const SaRow* rows, const float2* part_ml, const float* part_o,
+                                                                    const int32_t* members, T* out, int n_rows, int nh, int hd, int lanes) {
     constexpr int PIECES = 2, FLIGHT = 4;          // pieces of 16 bytes a lane has of a row of up to 256
     constexpr int ROWS = WARPS > 4 ? 1 : 4 / WARPS;      // of a block
     __shared__ float2 warp_ml[ROWS * WARPS];
