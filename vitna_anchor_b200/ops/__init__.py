@@ -2416,7 +2416,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, keep: in
 def copy_rows(arena: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> torch.Tensor:
     """arena[l, dst[i]] = arena[l, src[i]] for every layer l and move i, in one launch (one a 128 moves).  arena [layers, rows, ...], any type; a row's
     elements lie together, rows and layers may lie apart.  src and dst are row numbers on the host: no row is written twice, or read and written.
-    A captured graph repeats the moves it was captured with."""
+    A captured graph repeats the moves it was captured with.  The next launch in the stream must not be an attention_decode over these rows, which asks for the keys of earlier
+    steps while the kernel in front of it may still run (in a model's step other kernels lie between)."""
     here = torch._C._cuda_getDevice()
     if arena.get_device() != here or arena.dim() < 2:
         raise KernelError("copy_rows: the arena is not a tensor [layers, rows, ...] on the current CUDA device")
